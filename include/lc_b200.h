@@ -585,6 +585,75 @@ int lc_silu_mul(const void* gate, const void* up, int dtype, int64_t n, void* ou
 int lc_rmsnorm(const void* x, const void* weight, int dtype, int64_t rows, int64_t cols, float mean_factor,
                float eps, void* out, lc_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------
+ * A deployed W8A8 decoder block: the 8-bit integer linear and the operators around it.
+ *
+ * The reference's VllmQuantLinearInt8 (llmc/compression/quantization/module_utils.py:145-209) runs a
+ * pre-quantised int8 checkpoint through two third-party calls, a per-token quantisation of the activations
+ * and a scaled product; the norms, rotary embedding and gated activation around them are stock module code.
+ * ------------------------------------------------------------------------------------------ */
+
+/* Per-token 8-bit codes of x (rows x cols of `dtype`, element (r, c) at x[r * ldx + c], any alignment):
+ *   zeros NULL   a = max(max|x|, 1e-5), scales = a / 127, codes = rint(x * (127 / a))
+ *   zeros given  lo = min(min x, 0), hi = max(max x, 0), d = max(hi - lo, 1e-5), r = 255 / d: scales = d / 255,
+ *                zeros = -128 - rint(lo * r), codes = clamp(rint(x * r) + zeros, -128, 127)
+ * scales and r are fp32 (one IEEE division each), x * r is rounded once, half to even.  A row that holds a NaN or
+ * an infinity (or whose hi - lo overflows fp32) gets scale NaN and codes 0.  codes: row r at codes + r * ldc; the
+ * bytes behind a row's `cols` are left as they were.  scales: rows fp32; zeros: rows int32. */
+int lc_int8_act_quant(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, int8_t* codes, int64_t ldc,
+                      float* scales, int32_t* zeros, lc_stream_t stream);
+
+/* The same for act(gate) * up, formed in fp32 and not rounded before it is quantised. */
+#define LC_ACT_SILU 1      /* x / (1 + exp(-x)) */
+#define LC_ACT_GELU 2      /* x (1 + erf(x / sqrt 2)) / 2 */
+#define LC_ACT_GELU_TANH 3 /* x (1 + tanh(sqrt(2 / pi) (x + 0.044715 x^3))) / 2 */
+int lc_int8_gated_act_quant(const void* gate, const void* up, int dtype, int64_t rows, int64_t cols, int64_t ldg,
+                            int64_t ldu, int act, int8_t* codes, int64_t ldc, float* scales, int32_t* zeros,
+                            lc_stream_t stream);
+
+/* c[m][n] = float(sum_k (a[m][k] - a_z[m]) b[n][k]) * a_s[m] * b_s[n] (+ bias[n]): a M x K and b N x K int8, rows lda /
+ * ldb bytes apart; a_s M and b_s N fp32; a_z (M int32) may be NULL, and with it b_sum, the N int32 sums of b's rows;
+ * bias N values of out_dtype or NULL; c M x N of out_dtype, contiguous.  The sum is exact in 32 bits, then come two fp32
+ * multiplications and an addition, in that order, and one rounding.  a, b and c are 16-byte aligned, lda and ldb multiples
+ * of 16 (LC_ERR_ALIGN); K at most 131071, with zero points 65793 (LC_ERR_SHAPE).  *status (may be NULL) receives
+ * LC_ERR_TIMEOUT if a bounded pipeline wait expires; outputs that could then not be formed are NaN. */
+int lc_int8_gemm(const int8_t* a, int64_t lda, const float* a_s, const int32_t* a_z, const int8_t* b, int64_t ldb,
+                 const float* b_s, const int32_t* b_sum, const void* bias, int64_t M, int64_t N, int64_t K, void* c,
+                 int out_dtype, int32_t* status, lc_stream_t stream);
+
+/* lc_int8_act_quant and lc_int8_gemm as one call: c = x b^T with x M x K of `dtype` quantised on the way (sym != 0:
+ * without zero points), c and bias of the same dtype.  scratch: lc_int8_linear_scratch(M, K) bytes, 16-byte aligned;
+ * its contents are not kept from one call to the next. */
+int64_t lc_int8_linear_scratch(int64_t M, int64_t K);
+int lc_int8_linear(const void* x, int dtype, int64_t ldx, const int8_t* b, int64_t ldb, const float* b_s,
+                   const int32_t* b_sum, const void* bias, int64_t M, int64_t N, int64_t K, int sym, void* c,
+                   void* scratch, int64_t scratch_bytes, int32_t* status, lc_stream_t stream);
+
+/* The residual add of a decoder block with the norms on both sides of it:
+ *   t = x, or x * rsqrt(mean(x^2) + eps) * (post_weight + weight_offset) when post_weight is given
+ *   h = residual + scale * gate * t, rounded to `dtype`            (residual, gate: NULL = left out)
+ *   y = h * rsqrt(mean(h^2) + eps) * (weight + weight_offset)      (weight NULL: no y)
+ * in fp32 between the loads and the roundings; y is formed from the rounded h.  y is written as `dtype` (y), or
+ * quantised from fp32 like lc_int8_act_quant (codes / scales / zeros), or both.  x and residual: rows x cols, rows ldx /
+ * ldr elements apart; gate: gate_rows x cols contiguous, row r using gate row r / (rows / gate_rows); h, y contiguous.
+ * h may be NULL when x itself is the stream (no residual, post_weight or gate, scale 1): then y is x's norm. */
+int lc_residual_norm(const void* x, const void* residual, const void* post_weight, const void* gate, int64_t gate_rows,
+                     const void* weight, int dtype, int64_t rows, int64_t cols, int64_t ldx, int64_t ldr, float scale,
+                     float eps, float weight_offset, void* h, void* y, int8_t* codes, int64_t ldc, float* scales,
+                     int32_t* zeros, lc_stream_t stream);
+
+/* Rotary embedding of q and k from positions: with angle = positions[b][t] * inv_freq[i], the pair (x1, x2) number i of
+ * the first rotary_dim elements of a head becomes scale * (x1 cos - x2 sin, x2 cos + x1 sin); pairs are
+ * (i, i + rotary_dim / 2), or (2i, 2i + 1) when interleaved; the other elements of the head are copied.  The angle is
+ * formed in fp64, so that far positions (|position| < 2^31) lose nothing; results are rounded once.
+ *   q, k        element (b, t, h, d) at [b * q_b + t * q_t + h * q_h + d]; k_heads 0: no k
+ *   q_out       (batch, tokens, heads, head_dim) without gaps, or q itself (in place, q's strides); k_out likewise
+ *   positions   int64, (b, t) at [b * pos_b + t] (pos_b 0: one row for all);  inv_freq: rotary_dim / 2 fp32 */
+int lc_rotary_embed(const void* q, void* q_out, int q_heads, int64_t q_b, int64_t q_t, int64_t q_h, const void* k,
+                    void* k_out, int k_heads, int64_t k_b, int64_t k_t, int64_t k_h, const int64_t* positions,
+                    int64_t pos_b, const float* inv_freq, int dtype, int64_t batch, int64_t tokens, int head_dim,
+                    int rotary_dim, int interleaved, float scale, lc_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -11,5 +11,6 @@ from .rtn import RTN  # noqa: F401
 from .awq import Awq  # noqa: F401
 from .blockwise import GPTQBlockwise, FakeQuantLinear, llama_subsets  # noqa: F401
 from .streaming import HostStagedGPTQ  # noqa: F401
+from .int8_linear import Int8Linear  # noqa: F401
 
-__all__ = ['IntegerQuantizer', 'FloatQuantizer', 'Weight48IntegerQuantizer', 'GPTQ', 'SpQR', 'RTN', 'Awq', 'GPTQBlockwise', 'FakeQuantLinear', 'llama_subsets', 'HostStagedGPTQ']
+__all__ = ['IntegerQuantizer', 'FloatQuantizer', 'Weight48IntegerQuantizer', 'GPTQ', 'SpQR', 'RTN', 'Awq', 'GPTQBlockwise', 'FakeQuantLinear', 'llama_subsets', 'HostStagedGPTQ', 'Int8Linear']

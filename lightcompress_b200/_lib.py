@@ -81,6 +81,14 @@ SIGNATURES = {
     'lc_rope_apply': [_p, _p, _p, _i, _i64, _i, _i, _i64, _p, _p],
     'lc_silu_mul': [_p, _p, _i, _i64, _p, _p],
     'lc_rmsnorm': [_p, _p, _i, _i64, _i64, _f, _f, _p, _p],
+    'lc_int8_act_quant': [_p, _i, _i64, _i64, _i64, _p, _i64, _p, _p, _p],
+    'lc_int8_gated_act_quant': [_p, _p, _i, _i64, _i64, _i64, _i64, _i, _p, _i64, _p, _p, _p],
+    'lc_int8_gemm': [_p, _i64, _p, _p, _p, _i64, _p, _p, _p, _i64, _i64, _i64, _p, _i, _p, _p],
+    'lc_int8_linear_scratch': [_i64, _i64],
+    'lc_int8_linear': [_p, _i, _i64, _p, _i64, _p, _p, _p, _i64, _i64, _i64, _i, _p, _p, _i64, _p, _p],
+    'lc_residual_norm': [_p, _p, _p, _p, _i64, _p, _i, _i64, _i64, _i64, _i64, _f, _f, _f, _p, _p, _p, _i64, _p, _p, _p],
+    'lc_rotary_embed': [_p, _p, _i, _i64, _i64, _i64, _p, _p, _i, _i64, _i64, _i64, _p, _i64, _p, _i, _i64, _i64, _i, _i,
+                        _i, _f, _p],
     'lc_awq_clip_search': [_p, _p, _i, _i64, _i64, _i64, _i64, _i64, _i, _i, _i, _i, _d, _p, _p, _p, _p],
     'lc_awq_clip_search_cuda_cores': [_p, _p, _i, _i64, _i64, _i64, _i64, _i64, _i, _i, _i, _i, _d, _p, _p, _p, _p],
 }
@@ -107,6 +115,7 @@ def _load():
         fn.argtypes = argtypes
         fn.restype = {'lc_status_string': ctypes.c_char_p,
                       'lc_gptq_factor_workspace_floats': ctypes.c_int64,
+                      'lc_int8_linear_scratch': ctypes.c_int64,
                       'lc_gptq_factor_split': ctypes.c_int64,
                       'lc_gptq_factor_vt_offset': ctypes.c_int64}.get(name, ctypes.c_int)
     return lib
@@ -150,3 +159,34 @@ def stream_of(t):
 
 def call(name, *args):
     check(name, getattr(lib, name)(*args))
+
+
+def launch(t, name, *args):
+    """call(name, *args, stream) on t's device and torch's current stream there, whichever device is current; the
+    caller's current device is what it was afterwards."""
+    dev, cur = t.get_device(), torch.cuda.current_device()
+    fn = getattr(lib, name)
+    if dev == cur:
+        lib.lc_set_device(dev)
+        code = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            try:
+                check('lc_set_device', lib.lc_set_device(dev))
+                code = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+            finally:
+                lib.lc_set_device(cur)
+    if code != LC_OK:
+        check(name, code)
+
+
+def require_inference(name, *tensors):
+    """The kernels have no backward pass: a call that would silently cut a graph is refused."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f'{name} has no backward pass: call it under torch.no_grad(), or on detached tensors')
+
+
+def require_same_device(name, t, **others):
+    for key, o in others.items():
+        if o is not None and o.device != t.device:
+            raise ValueError(f'{name}: {key} is on {o.device}, not on {t.device}')

@@ -8,14 +8,21 @@ kernel each.  The kernels round after every op of the chain they replace (the RM
 associates its sum of squares like torch's row reduction); before a swap is used it is compared
 bit for bit with the stock code on random data, and the stock code is kept if they differ (another
 rotary convention, activation or norm, or a torch build that reduces in another order).
+
+The second half of the file are the operators of a deployed block that such a check cannot cover, because
+they round once instead of after every op: residual_norm (the residual add with the norms on both sides of
+it, a gate and a multiplier, and the 8-bit quantisation the next integer linear needs) and rotary_embed
+(rotary positions from inv_freq: both pair layouts, part of a head, scaled frequencies).
 """
 import contextlib
+import math
 import sys
 
 import numpy as np
 import torch
 
 from . import _lib as L
+from . import int8_linear
 
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 _checked = {}
@@ -196,3 +203,197 @@ def fused_gated_mlp(mlp):
         yield True
     finally:
         cls.forward = orig
+
+
+# ---- operators of a deployed block ---------------------------------------------------------------
+def _strided_rows(x):
+    """(..., C) as a 2-D view (a copy where there is none) with contiguous rows."""
+    if x.stride(-1) != 1 and x.shape[-1] != 1:
+        x = x.contiguous()
+    return x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+
+
+def _gate_rows(gate, x):
+    """How many rows of gate there are, given that it broadcasts against x (..., C) over trailing tokens: one value
+    per channel (C,), one row per leading index ((B, 1, C), (B, 1, 1, C)) or one per token (x's shape)."""
+    lead = x.shape[:-1]
+    g = tuple(gate.shape[:-1])
+    if gate.shape[-1:] != x.shape[-1:] or len(g) > len(lead):
+        return None
+    g = (1,) * (len(lead) - len(g)) + g
+    n = 0
+    while n < len(lead) and g[n] == lead[n]:
+        n += 1
+    # after the indices it shares with x come ones; a shared 1 may stand on either side
+    if any(v != 1 for v in g[n:]):
+        return None
+    return math.prod(g[:n])
+
+
+def residual_norm(x, residual=None, weight=None, post_weight=None, gate=None, scale=1.0, eps=1e-6, weight_offset=0.0,
+                  quant=False, sym=True):
+    """The residual add of a decoder block and the norms on both sides of it, in one pass:
+
+        t = x                     or  x * rsqrt(mean(x^2) + eps) * (post_weight + weight_offset)
+        h = residual + scale * gate * t
+        y = h * rsqrt(mean(h^2) + eps) * (weight + weight_offset)
+
+    x, residual: (..., C) of one type (bf16, fp16, fp32), any strides; weight, post_weight: (C,); gate: (C,), one row
+    per leading index such as (B, 1, C), or x's shape; all of x's type.  residual, post_weight, gate and weight may each
+    be left out; weight_offset is 1 for norms that store their weight less one.  Statistics and sums are fp32; h is
+    rounded once and y is formed from the rounded h.
+
+    Returns (h, y).  Without weight, y is None.  With quant, y is what int8_linear.act_quant returns for it, (codes,
+    scales) or, with sym=False, (codes, scales, zeros), quantised from fp32.  Where h would equal x, it is x."""
+    name = 'residual_norm'
+    dt = L.lc_dtype(x)
+    L.require_inference(name, x, residual, weight, post_weight, gate)
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError(f'{name}: the last dimension must not be empty')
+    C = x.shape[-1]
+    for key, t in (('residual', residual), ('weight', weight), ('post_weight', post_weight), ('gate', gate)):
+        if t is not None and t.dtype != x.dtype:
+            raise TypeError(f'{name}: {key} is {t.dtype}, x is {x.dtype}')
+        if t is not None and key.endswith('weight') and tuple(t.shape) != (C,):
+            raise ValueError(f'{name}: {key} must have shape ({C},), got {tuple(t.shape)}')
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f'{name}: residual {tuple(residual.shape)} and x {tuple(x.shape)} differ')
+    if quant and weight is None:
+        raise ValueError(f'{name}: quant needs the weight of the norm whose result it quantises')
+    gate_rows = 0
+    if gate is not None:
+        gate_rows = _gate_rows(gate, x)
+        if gate_rows is None:
+            raise ValueError(f'{name}: gate {tuple(gate.shape)} must be ({C},), one row per leading index, or x\'s shape')
+        gate = gate.contiguous()
+    L.require_same_device(name, x, residual=residual, weight=weight, post_weight=post_weight, gate=gate)
+    L.require_cuda(x)
+    x2 = _strided_rows(x)
+    r2 = None if residual is None else _strided_rows(residual)
+    rows = x2.shape[0]
+    kept = residual is None and post_weight is None and gate is None and scale == 1.0
+    if kept and weight is None:
+        return x, None
+    h = x if kept else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = codes = scales = zeros = None
+    pitch = 0
+    if quant:
+        codes, pitch, scales, zeros = int8_linear._codes_like(x2, sym)
+    elif weight is not None:
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if rows:
+        weight = None if weight is None else weight.contiguous()
+        post_weight = None if post_weight is None else post_weight.contiguous()
+        L.launch(x2, 'lc_residual_norm', x2.data_ptr(), _at(r2), _at(post_weight), _at(gate), gate_rows, _at(weight), dt, rows, C,
+                 x2.stride(0), 0 if r2 is None else r2.stride(0), float(scale), float(eps), float(weight_offset),
+                 None if kept else h.data_ptr(), _at(y), _at(codes), pitch, _at(scales), _at(zeros))
+    return h, int8_linear._shaped(codes, scales, zeros, x.shape) if quant else y
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
+
+
+def rotary_embed(q, k, positions, inv_freq, interleaved=False, attention_scale=1.0, inplace=False):
+    """Rotary embedding of q (B, H, T, D) and k (B, G, T, D; may be None) from positions, one launch for both:
+    with angle = positions * inv_freq[i], pair i of the first R = 2 * len(inv_freq) elements of every head becomes
+    attention_scale * (x1 cos - x2 sin, x2 cos + x1 sin); pairs are (i, i + R/2) or, interleaved, (2i, 2i + 1); the
+    other D - R elements are kept.  The angle is formed in 64 bits, the result rounded once.
+
+    q, k: bf16, fp16 or fp32 with contiguous heads (any other strides, e.g. views of one projection's output);
+    positions: int64, (B, T), (1, T) or (T,); inv_freq: (R / 2,) fp32, see rope_frequencies.  Returns (q, k) in new memory,
+    (B, T, H, D) contiguous seen as (B, H, T, D) like the stock projections, or the given tensors if inplace."""
+    name = 'rotary_embed'
+    dt = L.lc_dtype(q)
+    L.require_inference(name, q, k, inv_freq)
+    if q.dim() != 4 or (k is not None and k.dim() != 4):
+        raise ValueError(f'{name}: q and k must be (B, heads, T, D)')
+    B, H, T, D = q.shape
+    if k is not None and (k.dtype != q.dtype or k.shape[0] != B or k.shape[2:] != q.shape[2:]):
+        raise ValueError(f'{name}: k {tuple(k.shape)} {k.dtype} does not go with q {tuple(q.shape)} {q.dtype}')
+    if positions.dtype != torch.int64 or tuple(positions.shape) not in ((B, T), (1, T), (T,)):
+        raise ValueError(f'{name}: positions must be int64 of shape ({B}, {T}), (1, {T}) or ({T},), got {positions.dtype} '
+                         f'{tuple(positions.shape)}')
+    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not 0 < 2 * inv_freq.numel() <= D:
+        raise ValueError(f'{name}: inv_freq must be between 1 and {D // 2} fp32 values, got {inv_freq.dtype} '
+                         f'{tuple(inv_freq.shape)}')
+    if D > 1024:
+        raise NotImplementedError(f'{name}: heads of {D} elements (at most 1024)')
+    L.require_same_device(name, q, k=k, positions=positions, inv_freq=inv_freq)
+    L.require_cuda(q)
+    outs, args = [], []
+    for x in (q, k):
+        if x is None:
+            outs.append(None)
+            args += [None, None, 0, 0, 0, 0]
+            continue
+        if x.stride(-1) != 1 and D != 1:
+            if inplace:
+                raise ValueError(f'{name}: the elements of a head must be contiguous')
+            x = x.contiguous()
+        if inplace and any(n > 1 and s == 0 for n, s in zip(x.shape, x.stride())):
+            raise ValueError(f'{name}: cannot work in place on an expanded tensor')
+        out = x if inplace else torch.empty((B, T, x.shape[1], D), dtype=x.dtype, device=x.device).transpose(1, 2)
+        outs.append(out)
+        sb, sh, st, _ = x.stride()
+        args += [x.data_ptr(), out.data_ptr(), x.shape[1], sb, st, sh]
+    if B and T:
+        positions = positions if positions.stride(-1) == 1 or T == 1 else positions.contiguous()
+        pos_b = positions.stride(0) if positions.dim() == 2 and positions.shape[0] > 1 else 0
+        inv_freq = inv_freq.contiguous()
+        L.launch(q, 'lc_rotary_embed', *args, positions.data_ptr(), pos_b, inv_freq.data_ptr(), dt, B, T, D,
+                 2 * inv_freq.numel(), int(interleaved), float(attention_scale))
+    return outs[0], outs[1]
+
+
+def rope_frequencies(rotary_dim, base=10000.0, scaling=None, seq_len=None, device='cuda'):
+    """(inv_freq fp32 (rotary_dim / 2,), attention_scale) for rotary_embed.  `scaling` is a model configuration's
+    rope_scaling / rope_parameters section: None or type 'default', 'linear' (factor), 'dynamic' (factor,
+    original_max_position_embeddings; uses seq_len), 'llama3' (factor, low_freq_factor, high_freq_factor,
+    original_max_position_embeddings) or 'yarn' (factor, original_max_position_embeddings, optional beta_fast, beta_slow,
+    mscale, mscale_all_dim, attention_factor)."""
+    if rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError(f'rope_frequencies: rotary_dim must be even and positive, got {rotary_dim}')
+    s = dict(scaling or {})
+    kind = s.get('rope_type', s.get('type', 'default'))
+    expo = torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim
+    inv = float(base) ** -expo
+    attention_scale = 1.0
+    if kind == 'linear':
+        inv = inv / s['factor']
+    elif kind == 'dynamic':
+        # the base grows with the sequence once it is longer than what the model was trained on
+        trained = s['original_max_position_embeddings']
+        length = max(seq_len or 0, trained)
+        grown = base * (s['factor'] * length / trained - (s['factor'] - 1)) ** (rotary_dim / (rotary_dim - 2))
+        inv = float(grown) ** -expo
+    elif kind == 'llama3':
+        # wave lengths beyond the trained context are stretched, short ones kept, the ones between blended
+        turns = s['original_max_position_embeddings'] * inv / (2 * math.pi)     # turns within the trained context
+        keep = ((turns - s['low_freq_factor']) / (s['high_freq_factor'] - s['low_freq_factor'])).clamp(0, 1)
+        inv = keep * inv + (1 - keep) * inv / s['factor']
+    elif kind == 'yarn':
+        trained, factor = s['original_max_position_embeddings'], s['factor']
+
+        def pair_with(turns):      # the (fractional) pair that makes so many turns within the trained context
+            return rotary_dim * math.log(trained / (turns * 2 * math.pi)) / (2 * math.log(base))
+        low, high = pair_with(s.get('beta_fast') or 32), pair_with(s.get('beta_slow') or 1)
+        if s.get('truncate', True):
+            low, high = math.floor(low), math.ceil(high)
+        low, high = max(low, 0), min(high, rotary_dim - 1)
+        if low == high:
+            high += 0.001
+        ramp = ((torch.arange(rotary_dim // 2, dtype=torch.float64) - low) / (high - low)).clamp(0, 1)
+        inv = inv / factor * ramp + inv * (1 - ramp)
+
+        def magnitude(m):
+            return 0.1 * m * math.log(factor) + 1 if factor > 1 else 1.0
+        if s.get('attention_factor') is not None:
+            attention_scale = float(s['attention_factor'])
+        elif s.get('mscale') and s.get('mscale_all_dim'):
+            attention_scale = magnitude(s['mscale']) / magnitude(s['mscale_all_dim'])
+        else:
+            attention_scale = magnitude(1.0)
+    elif kind != 'default':
+        raise NotImplementedError(f'rope_frequencies: scaling type {kind!r}')
+    return inv.float().to(device), attention_scale

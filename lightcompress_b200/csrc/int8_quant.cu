@@ -1,0 +1,135 @@
+// Per-token 8-bit quantisation of activations in front of the integer linear (the scaled_int8_quant call of
+// the reference's VllmQuantLinearInt8, llmc/compression/quantization/module_utils.py:145-166), of a tensor or of
+// the gated activation act(gate) * up that feeds an MLP's down projection.  Arithmetic: row_quant.cuh.
+#include "row_quant.cuh"
+
+namespace lc {
+namespace {
+
+constexpr int kThreads = 256;
+
+enum Act { kNone = 0, kSilu = LC_ACT_SILU, kGelu = LC_ACT_GELU, kGeluTanh = LC_ACT_GELU_TANH };
+
+template <int kAct>
+__device__ __forceinline__ float act_of(float x) {
+  if (kAct == kSilu) return __fdividef(x, 1.f + __expf(-x));
+  if (kAct == kGelu) return 0.5f * x * (1.f + erff(x * 0.70710678118654752f));
+  if (kAct == kGeluTanh) return 0.5f * x * (1.f + tanhf(0.79788456080286536f * (x + 0.044715f * x * x * x)));
+  return x;
+}
+
+struct QuantArgs {
+  const void* x;        // gate when an activation is given
+  const void* up;
+  int64_t rows, cols, ldx, ldu, ldc;
+  int8_t* codes;
+  float* scales;
+  int32_t* zeros;       // NULL: symmetric
+};
+
+template <bool kSym>
+__device__ __forceinline__ RowQuant block_row_quant(RowRange<kSym> m, float* red) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  m.warp_reduce();
+  __syncthreads();                       // red may still be read for the previous row
+  if (lane == 0) {
+    red[warp] = m.mx;
+    red[8 + warp] = m.mn;
+  }
+  __syncthreads();
+  float mx = red[0], mn = red[8];
+#pragma unroll
+  for (int w = 1; w < kThreads / 32; ++w) {
+    mx = nan_max(mx, red[w]);
+    mn = nan_min(mn, red[8 + w]);
+  }
+  return row_quant<kSym>(mn, mx);
+}
+
+// Any width and alignment: a CTA per row, the row read twice.
+template <typename T, int kAct, bool kSym>
+__global__ void __launch_bounds__(kThreads) quant_any_kernel(QuantArgs a) {
+  using E = Elem<T>;
+  __shared__ float red[16];
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T* x = static_cast<const T*>(a.x) + row * a.ldx;
+    const T* u = static_cast<const T*>(a.up) + row * a.ldu;
+    auto value = [&](int64_t c) {
+      const float v = E::to_f(x[c]);
+      return kAct == kNone ? v : act_of<kAct>(v) * E::to_f(u[c]);
+    };
+    RowRange<kSym> m;
+    for (int64_t c = threadIdx.x; c < a.cols; c += kThreads) m.add(value(c));
+    const RowQuant q = block_row_quant<kSym>(m, red);
+    int8_t* out = a.codes + row * a.ldc;
+    for (int64_t c = threadIdx.x; c < a.cols; c += kThreads)
+      out[c] = q.bad ? (int8_t)0 : (int8_t)row_code<kSym>(value(c), q);
+    if (threadIdx.x == 0) {
+      a.scales[row] = q.s;
+      if (!kSym) a.zeros[row] = q.z;
+    }
+  }
+}
+
+template <typename T, int kAct, bool kSym>
+int launch(const QuantArgs& a, cudaStream_t st) {
+  const int64_t cap = (int64_t)kNumSMsB200 * 8;
+  quant_any_kernel<T, kAct, kSym><<<(unsigned)(a.rows < cap ? a.rows : cap), kThreads, 0, st>>>(a);
+  LC_LAUNCH_CHECK();
+  return LC_OK;
+}
+
+template <typename T, int kAct>
+int by_sym(const QuantArgs& a, cudaStream_t st) {
+  return a.zeros ? launch<T, kAct, false>(a, st) : launch<T, kAct, true>(a, st);
+}
+
+template <typename T>
+int by_act(const QuantArgs& a, int act, cudaStream_t st) {
+  switch (act) {
+    case kNone: return by_sym<T, kNone>(a, st);
+    case kSilu: return by_sym<T, kSilu>(a, st);
+    case kGelu: return by_sym<T, kGelu>(a, st);
+    case kGeluTanh: return by_sym<T, kGeluTanh>(a, st);
+    default: return LC_ERR_ARG;
+  }
+}
+
+int quant_rows(const QuantArgs& a, int dtype, int act, cudaStream_t st) {
+  switch (dtype) {
+    case LC_F32: return by_act<float>(a, act, st);
+    case LC_BF16: return by_act<__nv_bfloat16>(a, act, st);
+    case LC_F16: return by_act<__half>(a, act, st);
+    default: return LC_ERR_ARG;
+  }
+}
+
+}  // namespace
+
+int int8_quant_rows(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, int8_t* codes, int64_t ldc,
+                    float* scales, int32_t* zeros, cudaStream_t st) {
+  return quant_rows(QuantArgs{x, x, rows, cols, ldx, ldx, ldc, codes, scales, zeros}, dtype, kNone, st);
+}
+
+}  // namespace lc
+
+extern "C" LC_API int lc_int8_act_quant(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, int8_t* codes,
+                                        int64_t ldc, float* scales, int32_t* zeros, lc_stream_t stream) {
+  using namespace lc;
+  if (dtype < LC_F32 || dtype > LC_F16 || rows < 0 || cols <= 0 || ldx < 0 || ldc < cols) return LC_ERR_ARG;
+  if (rows == 0) return LC_OK;
+  if (!x || !codes || !scales) return LC_ERR_ARG;
+  return int8_quant_rows(x, dtype, rows, cols, ldx, codes, ldc, scales, zeros, reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" LC_API int lc_int8_gated_act_quant(const void* gate, const void* up, int dtype, int64_t rows, int64_t cols,
+                                              int64_t ldg, int64_t ldu, int act, int8_t* codes, int64_t ldc,
+                                              float* scales, int32_t* zeros, lc_stream_t stream) {
+  using namespace lc;
+  if (dtype < LC_F32 || dtype > LC_F16 || act < LC_ACT_SILU || act > LC_ACT_GELU_TANH) return LC_ERR_ARG;
+  if (rows < 0 || cols <= 0 || ldg < 0 || ldu < 0 || ldc < cols) return LC_ERR_ARG;
+  if (rows == 0) return LC_OK;
+  if (!gate || !up || !codes || !scales) return LC_ERR_ARG;
+  return quant_rows(QuantArgs{gate, up, rows, cols, ldg, ldu, ldc, codes, scales, zeros}, dtype, act,
+                    reinterpret_cast<cudaStream_t>(stream));
+}

@@ -1,0 +1,250 @@
+"""The 8-bit integer linear: what a W8A8-quantised linear is deployed as.
+
+Counterpart of the reference's VllmQuantLinearInt8 (llmc/compression/quantization/module_utils.py:145-209), which
+hands the per-token quantisation of the activations and the scaled product to third-party kernels, and the integer
+sibling of fp8_linear.  Codes are int8 with an fp32 scale per token (activations) and per output channel (weights);
+activations may carry a zero point per token as well.
+
+Nothing here synchronises or reads device memory on the host, so every call can be captured into a CUDA graph.
+"""
+import torch
+import torch.nn as nn
+
+from . import _lib as L
+
+_ACTS = {'silu': 1, 'gelu': 2, 'gelu_tanh': 3}
+_status = {}
+
+
+def _status_of(t):
+    """The device's status word (a bounded wait that expired in a product), made on first use; None where that
+    first use is inside a capture."""
+    dev = t.get_device()
+    s = _status.get(dev)
+    if s is None:
+        if torch.cuda.is_current_stream_capturing():
+            return None
+        s = torch.zeros(1, dtype=torch.int32, device=t.device)
+        torch.cuda.current_stream(dev).synchronize()      # other streams may use it from here on
+        _status[dev] = s
+    return s
+
+
+def check_status(device=None):
+    """Waits for the device and raises LcError if a product since the last check gave up waiting (its outputs are
+    NaN where that happened)."""
+    dev = torch.device('cuda' if device is None else device)
+    dev = torch.cuda.current_device() if dev.index is None else dev.index
+    torch.cuda.synchronize(dev)
+    s = _status.get(dev)
+    code = int(s.item()) if s is not None else 0
+    if code:
+        s.zero_()
+        raise L.LcError('lc_int8_gemm', code, L.status_string(code))
+
+
+def _float_rows(name, x):
+    """x (..., K) as a 2-D view (or, where no view exists, a copy) whose rows are contiguous."""
+    L.lc_dtype(x)
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError(f'{name}: the last dimension must not be empty')
+    if x.stride(-1) != 1 and x.shape[-1] != 1:
+        x = x.contiguous()
+    return x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+
+
+def _codes_like(x2, sym):
+    """Room for the codes (rows 16 bytes apart or a multiple of that, as the products read them), scales, zeros."""
+    rows, cols = x2.shape
+    pitch = (cols + 15) // 16 * 16
+    codes = torch.empty((rows, pitch), dtype=torch.int8, device=x2.device)
+    scales = torch.empty((rows, 1), dtype=torch.float32, device=x2.device)
+    zeros = None if sym else torch.empty((rows, 1), dtype=torch.int32, device=x2.device)
+    return codes, pitch, scales, zeros
+
+
+def _shaped(codes, scales, zeros, shape):
+    codes = codes[:, :shape[-1]]
+    if len(shape) != 2:
+        codes = codes.unflatten(0, shape[:-1]) if len(shape) > 2 else codes[0]
+        scales = scales.reshape(*shape[:-1], 1)
+        zeros = None if zeros is None else zeros.reshape(*shape[:-1], 1)
+    return (codes, scales) if zeros is None else (codes, scales, zeros)
+
+
+def act_quant(x, sym=True):
+    """(int8 codes of x's shape, fp32 scales (..., 1)), with sym=False also int32 zero points (..., 1): per token
+    s = max(|x|) / 127 and q = rint(x / s), or, with a zero point, 255 steps over the token's range widened to
+    hold zero, x ~ (q - z) s.  x: (..., K) of bf16, fp16 or fp32, any strides.  A token that holds a NaN or an
+    infinity gets scale NaN.  The codes' rows lie a multiple of 16 bytes apart, which the products require."""
+    L.require_inference('act_quant', x)
+    x2 = _float_rows('act_quant', x)
+    L.require_cuda(x)
+    rows, cols = x2.shape
+    codes, pitch, scales, zeros = _codes_like(x2, sym)
+    if rows:
+        L.launch(x2, 'lc_int8_act_quant', x2.data_ptr(), L.lc_dtype(x2), rows, cols, x2.stride(0), codes.data_ptr(), pitch,
+                 scales.data_ptr(), None if sym else zeros.data_ptr())
+    return _shaped(codes, scales, zeros, x.shape)
+
+
+def gated_act_quant(gate, up, act='silu', sym=True):
+    """act_quant(act(gate) * up) in one pass, the product formed in fp32 and not rounded in between: the input of an
+    MLP's down projection.  act: 'silu', 'gelu' or 'gelu_tanh'."""
+    if act not in _ACTS:
+        raise NotImplementedError(f'gated_act_quant: activation {act!r}; there are {sorted(_ACTS)}')
+    if gate.shape != up.shape or gate.dtype != up.dtype:
+        raise ValueError(f'gated_act_quant: gate {tuple(gate.shape)} {gate.dtype} and up {tuple(up.shape)} {up.dtype} differ')
+    L.require_inference('gated_act_quant', gate, up)
+    g2, u2 = _float_rows('gated_act_quant', gate), _float_rows('gated_act_quant', up)
+    L.require_same_device('gated_act_quant', gate, up=up)
+    L.require_cuda(gate)
+    rows, cols = g2.shape
+    codes, pitch, scales, zeros = _codes_like(g2, sym)
+    if rows:
+        L.launch(g2, 'lc_int8_gated_act_quant', g2.data_ptr(), u2.data_ptr(), L.lc_dtype(g2), rows, cols, g2.stride(0),
+                 u2.stride(0), _ACTS[act], codes.data_ptr(), pitch, scales.data_ptr(), None if sym else zeros.data_ptr())
+    return _shaped(codes, scales, zeros, gate.shape)
+
+
+def aligned_rows(codes):
+    """codes (N, K) int8 as the products read them: rows beginning at multiples of 16 bytes.  The tensor itself where
+    it is laid out so already, else a copy (made once, when a weight is loaded)."""
+    if codes.dtype != torch.int8 or codes.dim() != 2:
+        raise TypeError('aligned_rows: int8 codes (N, K) expected')
+    if _rows_aligned(codes):
+        return codes
+    n, k = codes.shape
+    room = torch.zeros((n, (k + 15) // 16 * 16), dtype=torch.int8, device=codes.device)
+    room[:, :k] = codes
+    return room[:, :k]
+
+
+def _rows_aligned(t):
+    return ((t.shape[1] == 1 or t.stride(1) == 1) and t.data_ptr() % 16 == 0
+            and (t.shape[0] <= 1 or (t.stride(0) % 16 == 0 and t.stride(0) >= t.shape[1])))
+
+
+def _pitch(t):
+    """Row pitch of an aligned 2-D code tensor; a single row may carry any stride."""
+    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
+
+
+def _check_weight(name, b, b_s, b_sum, bias, zeros, out_dtype):
+    if b.dtype != torch.int8 or b.dim() != 2:
+        raise TypeError(f'{name}: the weight must be int8 codes (N, K), got {b.dtype} {tuple(b.shape)}')
+    N, K = b.shape
+    if not _rows_aligned(b):
+        raise ValueError(f'{name}: the rows of the weight must begin at multiples of 16 bytes (int8_linear.aligned_rows '
+                         'lays them out once)')
+    if b_s.dtype != torch.float32 or b_s.numel() != N or not b_s.is_contiguous():
+        raise ValueError(f'{name}: the weight needs one fp32 scale per output channel ({N}), contiguous')
+    if zeros:
+        if b_sum is None:
+            raise ValueError(f'{name}: zero points need the sums of the weight\'s rows, w.sum(1, dtype=torch.int32)')
+        if b_sum.dtype != torch.int32 or b_sum.numel() != N or not b_sum.is_contiguous():
+            raise ValueError(f'{name}: the sums of the weight\'s rows must be {N} int32 values, contiguous')
+    if bias is not None and (bias.dtype != out_dtype or bias.numel() != N or not bias.is_contiguous()):
+        raise ValueError(f'{name}: bias must be {N} contiguous values of {out_dtype}')
+    if K > (65793 if zeros else 131071):
+        raise ValueError(f'{name}: {K} products may leave 32 bits (at most 131071, with zero points 65793)')
+
+
+def int8_gemm(a, a_s, b, b_s, bias=None, a_z=None, b_sum=None, out_dtype=torch.bfloat16):
+    """a: (..., K) int8 codes with scales a_s (..., 1) and, if given, zero points a_z (..., 1), as act_quant returns
+    them; b: (N, K) int8 with b_s (N fp32 values) and, with zero points, b_sum (N int32 sums of b's rows).  Returns
+    (..., N) = ((a - a_z) b^T) * a_s * b_s + bias in out_dtype; the sum of products is exact."""
+    name = 'int8_gemm'
+    L.require_inference(name, a_s, b_s, bias)
+    if out_dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise TypeError(f'{name}: unsupported output type {out_dtype}')
+    if a.dtype != torch.int8 or a.dim() == 0:
+        raise TypeError(f'{name}: the activations must be int8 codes (..., K), got {a.dtype}')
+    _check_weight(name, b, b_s, b_sum, bias, a_z is not None, out_dtype)
+    N, K = b.shape
+    if a.shape[-1] != K or K == 0:
+        raise ValueError(f'{name}: activations of {a.shape[-1]} and a weight of {K} input channels')
+    a2 = a if a.dim() == 2 else a.reshape(-1, K)
+    M = a2.shape[0]
+    if not _rows_aligned(a2):
+        raise ValueError(f'{name}: the rows of the activations\' codes must begin at multiples of 16 bytes, as act_quant lays '
+                         'them out')
+    if a_s.dtype != torch.float32 or a_s.numel() != M or not a_s.is_contiguous():
+        raise ValueError(f'{name}: the activations need one fp32 scale per token ({M}), contiguous')
+    if a_z is not None and (a_z.dtype != torch.int32 or a_z.numel() != M or not a_z.is_contiguous()):
+        raise ValueError(f'{name}: zero points must be {M} int32 values, contiguous')
+    L.require_same_device(name, a, a_s=a_s, a_z=a_z, b=b, b_s=b_s, b_sum=b_sum, bias=bias)
+    L.require_cuda(a)
+    c = torch.empty((*a.shape[:-1], N), dtype=out_dtype, device=a.device)
+    if M and N:
+        s = _status_of(a)
+        L.launch(a, 'lc_int8_gemm', a2.data_ptr(), _pitch(a2), a_s.data_ptr(), None if a_z is None else a_z.data_ptr(),
+                 b.data_ptr(), _pitch(b), b_s.data_ptr(), None if a_z is None else b_sum.data_ptr(),
+                 None if bias is None else bias.data_ptr(), M, N, K, c.data_ptr(), L._DTYPES[out_dtype],
+                 None if s is None else s.data_ptr())
+    return c
+
+
+def int8_dynamic_forward_func(x, w, w_scale, bias=None, w_sum=None):
+    """The W8A8 linear's forward: x (..., K) quantised per token and multiplied with w (N, K) int8, scales w_scale (N fp32
+    values), in one call.  With w_sum (N int32 sums of w's rows) the activations get a zero point per token, without it
+    they are quantised symmetrically.  Returns (..., N) of x's type; bias has that type too."""
+    name = 'int8_dynamic_forward_func'
+    L.require_inference(name, x, w_scale, bias)
+    x2 = _float_rows(name, x)
+    sym = w_sum is None
+    _check_weight(name, w, w_scale, w_sum, bias, not sym, x.dtype)
+    N, K = w.shape
+    M = x2.shape[0]
+    if x2.shape[1] != K:
+        raise ValueError(f'{name}: activations of {x2.shape[1]} and a weight of {K} input channels')
+    L.require_same_device(name, x, w=w, w_scale=w_scale, bias=bias, w_sum=w_sum)
+    L.require_cuda(x)
+    c = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=x.device)
+    if M and N:
+        room = M * ((K + 15) // 16 * 16) + 8 * M
+        scratch = torch.empty(room, dtype=torch.int8, device=x.device)
+        s = _status_of(x)
+        L.launch(x2, 'lc_int8_linear', x2.data_ptr(), L.lc_dtype(x2), x2.stride(0), w.data_ptr(), _pitch(w), w_scale.data_ptr(),
+                 None if sym else w_sum.data_ptr(), None if bias is None else bias.data_ptr(), M, N, K, int(sym),
+                 c.data_ptr(), scratch.data_ptr(), room, None if s is None else s.data_ptr())
+    return c
+
+
+class Int8Linear(nn.Module):
+    """Replacement linear with int8 weights and dynamically quantised activations (the role of the reference's
+    VllmQuantLinearInt8).  `new` takes what the algorithms' replacement linears take: the module and its
+    w_q(module, wquantizer) -> (codes, scales, zeros)."""
+
+    def __init__(self, codes, scale, bias=None, sym_act=True):
+        super().__init__()
+        if codes.dtype != torch.int8:
+            raise TypeError('Int8Linear: symmetric int8 weight codes expected')
+        if scale.numel() != codes.shape[0]:
+            raise NotImplementedError('Int8Linear: one scale per output channel (per_channel weights) expected, got '
+                                      f'{scale.numel()} for {codes.shape[0]} channels')
+        self.out_features, self.in_features = codes.shape
+        self.register_buffer('weight', aligned_rows(codes))
+        self.register_buffer('weight_scale', scale.detach().reshape(-1).float().contiguous())
+        self.register_buffer('weight_sum', None if sym_act else codes.sum(1, dtype=torch.int32))
+        self.register_buffer('bias', None if bias is None else bias.detach().contiguous())
+
+    @classmethod
+    @torch.no_grad()
+    def new(cls, module, w_q, wquantizer=None, aquantizer=None):
+        """module: an nn.Linear; w_q: e.g. RTN(wquantizer).w_q, for 8-bit symmetric per_channel weights; aquantizer:
+        the activations' quantizer (8 bits, per_token), whose symmetry is kept; None means symmetric."""
+        if aquantizer is not None and (aquantizer.bit != 8 or aquantizer.granularity != 'per_token'):
+            raise NotImplementedError('Int8Linear: activations are quantised to 8 bits per token')
+        codes, scale, zeros = w_q(module, wquantizer) if wquantizer is not None else w_q(module)
+        if zeros is not None:
+            raise NotImplementedError('Int8Linear: weights with zero points are not supported')
+        bias = getattr(module, 'bias', None)
+        return cls(codes, scale, None if bias is None else bias.data, aquantizer is None or aquantizer.sym)
+
+    @torch.no_grad()
+    def forward(self, x):
+        return int8_dynamic_forward_func(x, self.weight, self.weight_scale, self.bias, self.weight_sum)
+
+    def extra_repr(self):
+        return f'in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}'
