@@ -594,10 +594,10 @@ int lc_rmsnorm(const void* x, const void* weight, int dtype, int64_t rows, int64
  * ------------------------------------------------------------------------------------------ */
 
 /* Per-token 8-bit codes of x (rows x cols of `dtype`, element (r, c) at x[r * ldx + c], any alignment):
- *   zeros NULL   a = max(max|x|, 1e-5), scales = a / 127, codes = rint(x * (127 / a))
- *   zeros given  lo = min(min x, 0), hi = max(max x, 0), d = max(hi - lo, 1e-5), r = 255 / d: scales = d / 255,
- *                zeros = -128 - rint(lo * r), codes = clamp(rint(x * r) + zeros, -128, 127)
- * scales and r are fp32 (one IEEE division each), x * r is rounded once, half to even.  A row that holds a NaN or
+ *   zeros NULL   a = max(max|x|, 1e-5), scales = a / 127, r = 127 * (1 / a), codes = rint(x * r)
+ *   zeros given  lo = min(min x, 0), hi = max(max x, 0), d = max(hi - lo, 1e-5), r = 255 * (1 / d): scales =
+ *                d / 255, zeros = -128 - rint(lo * r), codes = clamp(rint(x * r) + zeros, -128, 127)
+ * scales and r are fp32, every operation rounded to nearest; x * r is rounded once, half to even.  A row that holds a NaN or
  * an infinity (or whose hi - lo overflows fp32) gets scale NaN and codes 0.  codes: row r at codes + r * ldc; the
  * bytes behind a row's `cols` are left as they were.  scales: rows fp32; zeros: rows int32. */
 int lc_int8_act_quant(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, int8_t* codes, int64_t ldc,

@@ -7,7 +7,7 @@
 // how the contraction is split; the zero point enters as -a_z[m] * b_sum[n] in the same 32-bit arithmetic (the
 // bounds on K keep the final sum inside 32 bits; what wraps on the way wraps back).  After that there are two
 // fp32 multiplications and an addition, in this order, and one rounding to the output type.
-#include "lc_common.cuh"
+#include "umma_common.cuh"
 
 namespace lc {
 
@@ -15,6 +15,8 @@ int int8_quant_rows(const void* x, int dtype, int64_t rows, int64_t cols, int64_
                     float* scales, int32_t* zeros, cudaStream_t st);
 
 namespace {
+
+using namespace umma;
 
 struct Int8Args {
   const int8_t* a;
@@ -25,81 +27,280 @@ struct Int8Args {
   const int32_t* b_sum;
   const void* bias;        // out_dtype, or NULL
   void* c;                 // [M][N]
+  int32_t* status;
   int64_t lda, ldb;
   int M, N, K;
 };
 
 // one element of the output; acc is the sum of the products of the codes
-template <typename T>
 __device__ __forceinline__ float finish(int acc, float a_s, int a_z, float b_s, int b_sum, float bias) {
   const int whole = (int)((unsigned)acc - (unsigned)a_z * (unsigned)b_sum);
   return __fadd_rn(__fmul_rn(__fmul_rn(__int2float_rn(whole), a_s), b_s), bias);
 }
 
-constexpr int kTile = 64, kThreads = 256;
+// ---- weights as the 128-row operand, tokens as the columns ---------------------------------------------------
+// One CTA per 128 output channels x NT tokens x one part of K (tcgen05 kind::i8, cta_group::1): the accumulator holds
+// a channel per TMEM lane and a token per column, so a warp's store of one token is 32 neighbouring channels.  Both
+// operands are K-major: a 128-byte swizzled row of a stage is 128 consecutive codes of one channel or token; K's ragged
+// end and the rows behind the last are filled with zeros by the copy.
+//
+// Few tokens leave the weights as the only traffic that matters (N * K bytes), and N / 128 CTAs are too few to draw
+// the HBM's bandwidth: K is split over the CTAs of a cluster, whose partial sums meet through distributed shared
+// memory.  The weights of the first `stages` blocks are requested before the kernel waits for the one that quantises
+// the activations (programmatic dependent launch), which hides it.
+constexpr int kRows = 128, kBlockK = 128, kStreamThreads = 128;
+constexpr int kWeightBytes = kRows * kBlockK;
+constexpr int kSmemMost = 227 * 1024;
 
-// 64 x 64 outputs per CTA, 4 x 4 per thread, four products per DP4A
-template <typename T>
-__global__ void __launch_bounds__(kThreads) dp4a_kernel(Int8Args g) {
-  __shared__ uint32_t sa[kTile][17], sb[kTile][17];
-  const int m0 = blockIdx.y * kTile, n0 = blockIdx.x * kTile;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int lr = threadIdx.x >> 2, lc = (threadIdx.x & 3) * 16;       // row and first byte this thread stages
-  int acc[4][4] = {};
-  auto stage = [&](const int8_t* p, int64_t ld, int row, int rows, int k0, uint32_t* dst) {
-    uint32_t w[4] = {0u, 0u, 0u, 0u};
-    const int k = k0 + lc;
-    if (row < rows && k < g.K) {
-      const int8_t* src = p + (int64_t)row * ld + k;
-      if (k + 16 <= g.K) {
-        const uint4 v = *reinterpret_cast<const uint4*>(src);
-        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-      } else {
-        for (int i = 0; i < g.K - k; ++i) w[i >> 2] |= (uint32_t)(uint8_t)src[i] << (8 * (i & 3));
+// kind::i8: D s32, A and B s8, both K-major
+__host__ __device__ constexpr uint32_t idesc_i8(int m, int n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+
+__device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}"
+      ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+  tmem_wait_ld();
+}
+
+__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ int ld_cluster(uint32_t addr, int rank) {
+  uint32_t a;
+  int v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+
+struct Maps {
+  CUtensorMap w, x;
+};
+
+template <typename T, int NT>
+__global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_constant__ Maps maps, Int8Args g, int splits,
+                                                                int stages) {
+  constexpr int kStage = kWeightBytes + NT * kBlockK;
+  constexpr int kCols = NT < 32 ? 32 : NT;                 // tensor memory is allocated in powers of two from 32 columns
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+  const uint32_t bar0 = base + stages * kStage;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen + stages * kStage + 8 * (2 * stages + 1));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  auto full_bar = [&](int s) { return bar0 + 8u * s; };
+  auto empty_bar = [&](int s) { return bar0 + 8u * (stages + s); };
+  const uint32_t acc_bar = bar0 + 8u * (2 * stages);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = blockIdx.x % splits;
+  const int n0 = (int)(blockIdx.x / splits) * kRows, m0 = (int)blockIdx.y * NT;
+  const int blocks = (g.K + kBlockK - 1) / kBlockK;
+  const int kb0 = (int)((int64_t)blocks * rank / splits), kb1 = (int)((int64_t)blocks * (rank + 1) / splits);
+  const int count = kb1 - kb0;                             // at least 1: splits <= blocks
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < stages; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    mbar_init(acc_bar, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    // the weights do not depend on the kernel before this one
+    for (int i = 0; i < stages && i < count; ++i) {
+      mbar_expect_tx(full_bar(i), kStage);
+      tma_load_2d(base + i * kStage, &maps.w, (kb0 + i) * kBlockK, n0, full_bar(i));
+    }
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"((uint32_t)kCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  grid_dependency_wait();
+
+  int issued = 0;                                          // k blocks requested, known to thread 0
+  if (warp == 0) {
+    if (lane == 0) {
+      for (int i = 0; i < stages && i < count; ++i)
+        tma_load_2d(base + i * kStage + kWeightBytes, &maps.x, (kb0 + i) * kBlockK, m0, full_bar(i));
+      int s = 0;
+      uint32_t ph = 0;
+      issued = min(stages, count);
+      for (int i = stages; i < count; ++i) {
+        if (!mbar_wait(empty_bar(s), ph, abort_flag)) break;
+        mbar_expect_tx(full_bar(s), kStage);
+        tma_load_2d(base + s * kStage, &maps.w, (kb0 + i) * kBlockK, n0, full_bar(s));
+        tma_load_2d(base + s * kStage + kWeightBytes, &maps.x, (kb0 + i) * kBlockK, m0, full_bar(s));
+        issued = i + 1;
+        if (++s == stages) s = 0, ph ^= 1u;
       }
     }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int s = 0;
+      uint32_t ph = 0;
+      for (int i = 0; i < count; ++i) {
+        if (!mbar_wait(full_bar(s), ph, abort_flag)) break;
+        tcgen05_fence_after();
+        const uint32_t sw = base + s * kStage, sx = sw + kWeightBytes;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) dst[i] = w[i];
-  };
-  for (int k0 = 0; k0 < g.K; k0 += 64) {
-    stage(g.a, g.lda, m0 + lr, g.M, k0, &sa[lr][lc >> 2]);
-    stage(g.b, g.ldb, n0 + lr, g.N, k0, &sb[lr][lc >> 2]);
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      int av[4], bv[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) av[i] = (int)sa[ty + 16 * i][k], bv[i] = (int)sb[tx + 16 * i][k];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = __dp4a(av[i], bv[j], acc[i][j]);
-    }
-    __syncthreads();
-  }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int n = n0 + tx + 16 * j;
-    if (n >= g.N) continue;
-    const float bs = g.b_s[n], bias = g.bias ? Elem<T>::to_f(static_cast<const T*>(g.bias)[n]) : 0.f;
-    const int bsum = g.a_z ? g.b_sum[n] : 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int m = m0 + ty + 16 * i;
-      if (m < g.M)
-        static_cast<T*>(g.c)[(int64_t)m * g.N + n] =
-            Elem<T>::from_f(finish<T>(acc[i][j], g.a_s[m], g.a_z ? g.a_z[m] : 0, bs, bsum, bias));
+        for (int j = 0; j < kBlockK / 32; ++j)
+          umma_i8(tmem, make_desc_mn_sw128(sw + j * 32, 16, 1024), make_desc_mn_sw128(sx + j * 32, 16, 1024),
+                  idesc_i8(kRows, NT), (i | j) ? 1u : 0u);
+        umma_commit(empty_bar(s));
+        if (++s == stages) s = 0, ph ^= 1u;
+      }
+      umma_commit(acc_bar);                                // arrives once the MMAs issued so far have retired
     }
   }
+  __syncwarp();
+  // the accumulator (or, after an expired wait, the retirement of what was issued)
+  for (uint32_t it = 0; !mbar_test(acc_bar, 0); ++it) {
+    if (it >= 2 * kSpinLimit) { *abort_flag = 1; break; }
+    if (it >= 64) __nanosleep(50);
+  }
+  tcgen05_fence_after();
+  __syncthreads();
+  bool ok = *abort_flag == 0;
+  if (!ok) {
+    // the copies still in flight land before the CTA's shared memory is used again or released
+    if (threadIdx.x == 0)
+      for (int i = issued > stages ? issued - stages : 0; i < issued; ++i)
+        for (uint32_t it = 0; it < kSpinLimit && !mbar_test(full_bar(i % stages), (uint32_t)(i / stages) & 1u); ++it)
+          __nanosleep(50);
+    __syncthreads();
+  }
+
+  const int c = warp * 32 + lane, n = n0 + c;
+  const bool col_ok = n < g.N;
+  const int tokens = min(NT, g.M - m0);
+  const float b_s = col_ok ? g.b_s[n] : 0.f;
+  const float bias = col_ok && g.bias ? Elem<T>::to_f(static_cast<const T*>(g.bias)[n]) : 0.f;
+  const int b_sum = col_ok && g.a_z ? g.b_sum[n] : 0;
+  T* out = static_cast<T*>(g.c) + (int64_t)m0 * g.N + n;
+  const float lost = __int_as_float(0x7fffffff);
+  const uint32_t taddr = tmem + ((uint32_t)(warp * 32) << 16);
+  if (splits == 1) {
+#pragma unroll 1
+    for (int t0 = 0; t0 < tokens; t0 += 16) {
+      uint32_t v[16];
+      tmem_ld16(taddr + t0, v);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int t = t0 + i;
+        if (t < tokens && col_ok) {
+          const float y = finish((int)v[i], g.a_s[m0 + t], g.a_z ? g.a_z[m0 + t] : 0, b_s, b_sum, bias);
+          out[(int64_t)t * g.N] = Elem<T>::from_f(ok ? y : lost);
+        }
+      }
+    }
+  } else {
+    // [token][channel] partial sums in the stages' memory: every copy into it has landed and every MMA read it
+    int* part = reinterpret_cast<int*>(gen);
+#pragma unroll 1
+    for (int t0 = 0; t0 < tokens; t0 += 16) {
+      uint32_t v[16];
+      tmem_ld16(taddr + t0, v);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) part[(t0 + i) * kRows + c] = (int)v[i];
+    }
+    cluster_sync();
+    for (int r = 0; r < splits; ++r) ok = ok && ld_cluster(smem_u32(const_cast<int*>(abort_flag)), r) == 0;
+    for (int t = rank; t < tokens; t += splits) {
+      unsigned sum = 0;
+      for (int r = 0; r < splits; ++r) sum += (unsigned)ld_cluster(base + (uint32_t)(t * kRows + c) * 4u, r);
+      if (col_ok) {
+        const float y = finish((int)sum, g.a_s[m0 + t], g.a_z ? g.a_z[m0 + t] : 0, b_s, b_sum, bias);
+        out[(int64_t)t * g.N] = Elem<T>::from_f(ok ? y : lost);
+      }
+    }
+    cluster_sync();                                        // nobody leaves while its partial sums are being read
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)kCols) : "memory");
+  if (threadIdx.x == 0 && !ok && g.status) atomicExch(g.status, (int)LC_ERR_TIMEOUT);
+}
+
+int encode_codes(CUtensorMap* m, const int8_t* p, int64_t k, int64_t rows, int64_t ld, int box_rows) {
+  EncodeTiledFn encode = get_encode_fn();
+  if (!encode) return LC_ERR_CUDA;
+  const cuuint64_t dim[2] = {(cuuint64_t)k, (cuuint64_t)rows};
+  const cuuint64_t stride[1] = {(cuuint64_t)ld};
+  const cuuint32_t box[2] = {kBlockK, (cuuint32_t)box_rows};
+  const cuuint32_t step[2] = {1, 1};
+  if (encode(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t*>(p), dim, stride, box, step,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return LC_ERR_CUDA;
+  return LC_OK;
+}
+
+template <typename T, int NT>
+int launch_stream(const Int8Args& g, bool dependent, cudaStream_t st) {
+  constexpr int kStage = kWeightBytes + NT * kBlockK;
+  const int n_tiles = (g.N + kRows - 1) / kRows, m_tiles = (g.M + NT - 1) / NT;
+  if (m_tiles > 65535) return LC_ERR_SHAPE;
+  const int blocks = (g.K + kBlockK - 1) / kBlockK, tiles = n_tiles * m_tiles;
+  int splits = 1;
+  while (splits < 8 && tiles * splits * 2 <= kNumSMsB200 * 2 && splits * 2 <= blocks) splits *= 2;
+  const int per_sm = tiles * splits > kNumSMsB200 ? 2 : 1;
+  int stages = (kSmemMost / per_sm - 2048) / kStage;
+  const int most = (blocks + splits - 1) / splits, least = (NT * kRows * 4 + kStage - 1) / kStage;
+  if (stages > most) stages = most;
+  if (splits > 1 && stages < least) stages = least;
+  const int smem = stages * kStage + 8 * (2 * stages + 1) + 16 + 1024;
+  Maps maps;
+  int rc;
+  if ((rc = encode_codes(&maps.w, g.b, g.K, g.N, g.ldb, kRows)) != LC_OK) return rc;
+  if ((rc = encode_codes(&maps.x, g.a, g.K, g.M, g.lda, NT)) != LC_OK) return rc;
+  // per-device attribute; setting it on every call keeps multi-device processes correct
+  LC_CHECK_CUDA(cudaFuncSetAttribute(stream_kernel<T, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = splits, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(n_tiles * splits), (unsigned)m_tiles);
+  cfg.blockDim = dim3(kStreamThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = dependent ? 2 : 1;
+  LC_CHECK_CUDA(cudaLaunchKernelEx(&cfg, stream_kernel<T, NT>, maps, g, splits, stages));
+  return LC_OK;
 }
 
 template <typename T>
-int launch(const Int8Args& g, cudaStream_t st) {
-  const dim3 grid((unsigned)((g.N + kTile - 1) / kTile), (unsigned)((g.M + kTile - 1) / kTile));
-  if (grid.y > 65535) return LC_ERR_SHAPE;
-  dp4a_kernel<T><<<grid, kThreads, 0, st>>>(g);
-  LC_LAUNCH_CHECK();
-  return LC_OK;
+int launch(const Int8Args& g, bool dependent, cudaStream_t st) {
+  if (g.M <= 16) return launch_stream<T, 16>(g, dependent, st);
+  if (g.M <= 32) return launch_stream<T, 32>(g, dependent, st);
+  if (g.M <= 64) return launch_stream<T, 64>(g, dependent, st);
+  return launch_stream<T, 128>(g, dependent, st);
 }
 
 // sizes, pitches and alignment of the product; the same rules for both entry points
@@ -115,11 +316,24 @@ int check(int64_t M, int64_t N, int64_t K, const void* b, int64_t ldb, const flo
   return LC_OK;
 }
 
-int product(const Int8Args& g, int out_dtype, cudaStream_t st) {
+// kind::i8 exists on sm_100 only
+int check_arch() {
+  int dev = 0, major = 0, minor = 0;
+  LC_CHECK_CUDA(cudaGetDevice(&dev));
+  LC_CHECK_CUDA(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev));
+  LC_CHECK_CUDA(cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev));
+  return major == 10 && minor == 0 ? LC_OK : LC_ERR_ARCH;
+}
+
+// dependent: the kernel before this one on the stream is the quantisation of lc_int8_linear, which writes a, a_s and a_z
+// and nothing else that the product reads
+int product(const Int8Args& g, int out_dtype, bool dependent, cudaStream_t st) {
+  const int rc = check_arch();
+  if (rc != LC_OK) return rc;
   switch (out_dtype) {
-    case LC_F32: return launch<float>(g, st);
-    case LC_BF16: return launch<__nv_bfloat16>(g, st);
-    default: return launch<__half>(g, st);
+    case LC_F32: return launch<float>(g, dependent, st);
+    case LC_BF16: return launch<__nv_bfloat16>(g, dependent, st);
+    default: return launch<__half>(g, dependent, st);
   }
 }
 
@@ -130,12 +344,11 @@ extern "C" LC_API int lc_int8_gemm(const int8_t* a, int64_t lda, const float* a_
                                    int64_t ldb, const float* b_s, const int32_t* b_sum, const void* bias, int64_t M,
                                    int64_t N, int64_t K, void* c, int out_dtype, int32_t* status, lc_stream_t stream) {
   using namespace lc;
-  (void)status;
   const int rc = check(M, N, K, b, ldb, b_s, a_z != nullptr, b_sum, c, out_dtype);
   if (rc != LC_OK || M == 0 || N == 0) return rc;
   if (!a || !a_s || lda < K) return LC_ERR_ARG;
   if (!aligned16(a) || (lda & 15)) return LC_ERR_ALIGN;
-  return product(Int8Args{a, b, a_s, a_z, b_s, b_sum, bias, c, lda, ldb, (int)M, (int)N, (int)K}, out_dtype,
+  return product(Int8Args{a, b, a_s, a_z, b_s, b_sum, bias, c, status, lda, ldb, (int)M, (int)N, (int)K}, out_dtype, false,
                  reinterpret_cast<cudaStream_t>(stream));
 }
 
@@ -148,7 +361,6 @@ extern "C" LC_API int lc_int8_linear(const void* x, int dtype, int64_t ldx, cons
                                      const int32_t* b_sum, const void* bias, int64_t M, int64_t N, int64_t K, int sym,
                                      void* c, void* scratch, int64_t scratch_bytes, int32_t* status, lc_stream_t stream) {
   using namespace lc;
-  (void)status;
   const int rc = check(M, N, K, b, ldb, b_s, !sym, b_sum, c, dtype);
   if (rc != LC_OK || M == 0 || N == 0) return rc;
   if (!x || ldx < 0 || !scratch) return LC_ERR_ARG;
@@ -161,5 +373,6 @@ extern "C" LC_API int lc_int8_linear(const void* x, int dtype, int64_t ldx, cons
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int qrc = int8_quant_rows(x, dtype, M, K, ldx, codes, lda, a_s, a_z, st);
   if (qrc != LC_OK) return qrc;
-  return product(Int8Args{codes, b, a_s, a_z, b_s, b_sum, bias, c, lda, ldb, (int)M, (int)N, (int)K}, dtype, st);
+  return product(Int8Args{codes, b, a_s, a_z, b_s, b_sum, bias, c, status, lda, ldb, (int)M, (int)N, (int)K}, dtype, true,
+                 st);
 }

@@ -1,11 +1,11 @@
 // 8-bit integer quantisation of one row (token), shared by the kernels that produce a row and quantise it.
 //
-//   symmetric   a = max(max |v|, 1e-5);               s = a / 127, r = 127 / a, z = 0,  q = rint(v r)
+//   symmetric   a = max(max |v|, 1e-5);               s = a / 127, r = 127 * (1 / a), z = 0,  q = rint(v r)
 //   asymmetric  lo = min(min v, 0), hi = max(max v, 0), d = max(hi - lo, 1e-5);
-//               s = d / 255, r = 255 / d, z = -128 - rint(lo r),  q = clamp(rint(v r) + z, -128, 127)
+//               s = d / 255, r = 255 * (1 / d), z = -128 - rint(lo r),  q = clamp(rint(v r) + z, -128, 127)
 //
-// s and r are fp32 numbers (one IEEE division each per row); v r is rounded once, to the nearest integer with
-// ties to even: fma(v, r, 1.5 * 2^23) leaves rint(v r) in the low bits of its result, so an element costs one
+// s and r are fp32 numbers, each operation of theirs rounded to nearest; v r is rounded once, to the nearest integer
+// with ties to even: fma(v, r, 1.5 * 2^23) leaves rint(v r) in the low bits of its result, so an element costs one
 // FFMA and its share of a byte pack instead of a division.  |v r| <= 255.0001, far inside the trick's range.
 // A row with a NaN or an infinity (or, asymmetric, one whose hi - lo overflows) gets s = NaN and codes 0.
 #pragma once
@@ -39,7 +39,7 @@ __device__ __forceinline__ RowQuant row_quant(float mn, float mx) {
   q.bad = !(wide <= FLT_MAX);
   constexpr float steps = kSym ? 127.f : 255.f;
   q.s = q.bad ? __int_as_float(0x7fffffff) : __fdiv_rn(wide, steps);
-  q.r = q.bad ? 0.f : __fdiv_rn(steps, wide);
+  q.r = q.bad ? 0.f : __fmul_rn(steps, __frcp_rn(wide));
   q.z = (kSym || q.bad) ? 0 : -128 - (__float_as_int(__fmaf_rn(mn, q.r, kRintMagic)) - kRintBias);
   return q;
 }

@@ -12,13 +12,13 @@ def quant_rows(v, sym=True):
     v32 = v.float()
     if sym:
         wide = v32.abs().amax(1).clamp(min=1e-5)
-        s, r = wide / torch.tensor(127.0), torch.tensor(127.0) / wide
+        s, r = wide / torch.tensor(127.0), torch.tensor(127.0) * (torch.tensor(1.0) / wide)
         z = torch.zeros(v.shape[0], dtype=torch.float64)
         low, high = -127, 127
     else:
         lo, hi = v32.amin(1).clamp(max=0), v32.amax(1).clamp(min=0)
         wide = (hi - lo).clamp(min=1e-5)
-        s, r = wide / torch.tensor(255.0), torch.tensor(255.0) / wide
+        s, r = wide / torch.tensor(255.0), torch.tensor(255.0) * (torch.tensor(1.0) / wide)
         z = -128 - torch.round(lo.double() * r.double())
         low, high = -128, 127
     bad = ~torch.isfinite(wide)
