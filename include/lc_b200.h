@@ -648,6 +648,7 @@ int lc_residual_norm(const void* x, const void* residual, const void* post_weigh
  * formed in fp64, so that far positions (|position| < 2^31) lose nothing; results are rounded once.
  *   q, k        element (b, t, h, d) at [b * q_b + t * q_t + h * q_h + d]; k_heads 0: no k
  *   q_out       (batch, tokens, heads, head_dim) without gaps, or q itself (in place, q's strides); k_out likewise
+ *   at most 1023 heads of q and k together, head_dim at most 1024
  *   positions   int64, (b, t) at [b * pos_b + t] (pos_b 0: one row for all);  inv_freq: rotary_dim / 2 fp32 */
 int lc_rotary_embed(const void* q, void* q_out, int q_heads, int64_t q_b, int64_t q_t, int64_t q_h, const void* k,
                     void* k_out, int k_heads, int64_t k_b, int64_t k_t, int64_t k_h, const int64_t* positions,

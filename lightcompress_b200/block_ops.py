@@ -317,8 +317,9 @@ def rotary_embed(q, k, positions, inv_freq, interleaved=False, attention_scale=1
     if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not 0 < 2 * inv_freq.numel() <= D:
         raise ValueError(f'{name}: inv_freq must be between 1 and {D // 2} fp32 values, got {inv_freq.dtype} '
                          f'{tuple(inv_freq.shape)}')
-    if D > 1024:
-        raise NotImplementedError(f'{name}: heads of {D} elements (at most 1024)')
+    if D > 1024 or H + (0 if k is None else k.shape[1]) > 1023:
+        raise NotImplementedError(f'{name}: heads of at most 1024 elements and at most 1023 of them, got {D} and '
+                                  f'{H + (0 if k is None else k.shape[1])}')
     L.require_same_device(name, q, k=k, positions=positions, inv_freq=inv_freq)
     L.require_cuda(q)
     outs, args = [], []

@@ -74,8 +74,82 @@ __global__ void __launch_bounds__(kThreads) quant_any_kernel(QuantArgs a) {
   }
 }
 
+__device__ __forceinline__ float act_at_run_time(float x, int act) {
+  return act == kSilu ? act_of<kSilu>(x) : act == kGelu ? act_of<kGelu>(x) : act_of<kGeluTanh>(x);
+}
+
+// Rows that registers hold, 16-byte aligned: read once, written once.
+template <typename T, int kWarps, int kVecs, bool kGated>
+__global__ void __launch_bounds__(RowGroup<kWarps>::kThreads) quant_rows_kernel(QuantArgs a, int act) {
+  using G = RowGroup<kWarps>;
+  constexpr int N = Elem<T>::kPerVec;
+  __shared__ float red[2 * kWarps];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // as in quant_any_kernel
+  const int64_t row = (int64_t)blockIdx.x * G::kRows + G::row();
+  if (G::kRows > 1 && row >= a.rows) return;                           // a whole warp, and no barrier follows
+  const int vecs = (int)(a.cols / N);
+  const bool sym = a.zeros == nullptr;
+  const uint4* x = reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + row * a.ldx);
+  const uint4* u = reinterpret_cast<const uint4*>(static_cast<const T*>(a.up) + row * a.ldu);
+  uint4 rx[kVecs], ru[kGated ? kVecs : 1];
+#pragma unroll
+  for (int k = 0; k < kVecs; ++k) {
+    const int i = G::lane() + k * G::kLanes;
+    rx[k] = i < vecs ? __ldcs(x + i) : make_uint4(0u, 0u, 0u, 0u);
+    if (kGated) ru[k] = i < vecs ? __ldcs(u + i) : make_uint4(0u, 0u, 0u, 0u);
+  }
+  float v[kVecs][N];
+  float mn = 0.f, mx = 0.f;
+#pragma unroll
+  for (int k = 0; k < kVecs; ++k) {
+    unpack16<T>(rx[k], v[k]);
+    if (kGated) {
+      float w[N];
+      unpack16<T>(ru[k], w);
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[k][j] = act_at_run_time(v[k][j], act) * w[j];
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      mx = nan_max(mx, v[k][j]);
+      mn = nan_min(mn, v[k][j]);
+    }
+  }
+  G::range(mn, mx, red);
+  const RowQuant q = row_quant_of(mn, mx, sym);
+  int8_t* out = a.codes + row * a.ldc;
+#pragma unroll
+  for (int k = 0; k < kVecs; ++k) {
+    const int i = G::lane() + k * G::kLanes;
+    if (i < vecs) store_row_codes<N>(out + i * N, v[k], q, sym);
+  }
+  if (G::lane() == 0) {
+    a.scales[row] = q.s;
+    if (!sym) a.zeros[row] = q.z;
+  }
+}
+
+// whether quant_rows_kernel took the rows
+template <typename T, bool kGated>
+bool launch_rows(const QuantArgs& a, int act, cudaStream_t st) {
+  constexpr int N = Elem<T>::kPerVec;
+  if (a.cols % N || (a.rows > 1 && (a.ldx % N || a.ldu % N || a.ldc % N)) || !aligned16(a.x) || !aligned16(a.up) ||
+      (reinterpret_cast<uintptr_t>(a.codes) & (N - 1)) || a.rows > 0x7fffffff)
+    return false;
+  return with_row_shape(a.cols / N, [&](auto shape) {
+    using S = decltype(shape);
+    using G = RowGroup<S::kWarps>;
+    quant_rows_kernel<T, S::kWarps, S::kVecs, kGated>
+        <<<(unsigned)((a.rows + G::kRows - 1) / G::kRows), G::kThreads, 0, st>>>(a, act);
+  });
+}
+
 template <typename T, int kAct, bool kSym>
 int launch(const QuantArgs& a, cudaStream_t st) {
+  if (launch_rows<T, kAct != kNone>(a, kAct, st)) {
+    LC_LAUNCH_CHECK();
+    return LC_OK;
+  }
   const int64_t cap = (int64_t)kNumSMsB200 * 8;
   quant_any_kernel<T, kAct, kSym><<<(unsigned)(a.rows < cap ? a.rows : cap), kThreads, 0, st>>>(a);
   LC_LAUNCH_CHECK();

@@ -44,6 +44,7 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads) norm_any_kernel(NormArgs a) {
   using E = Elem<T>;
   __shared__ float red[16];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const float inv_c = 1.f / (float)a.cols;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
@@ -105,8 +106,146 @@ __global__ void __launch_bounds__(kThreads) norm_any_kernel(NormArgs a) {
   }
 }
 
+// Rows that registers hold, 16-byte aligned: x, the residual and the gate are read once, h and y written once; the
+// weights come from the caches.
+template <typename T, int kWarps, int kVecs>
+__global__ void __launch_bounds__(RowGroup<kWarps>::kThreads) norm_rows_kernel(NormArgs a) {
+  using G = RowGroup<kWarps>;
+  using E = Elem<T>;
+  constexpr int N = E::kPerVec;
+  __shared__ float red[4 * kWarps];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // see the integer product
+  const int64_t row = (int64_t)blockIdx.x * G::kRows + G::row();
+  if (G::kRows > 1 && row >= a.rows) return;                           // a whole warp, and no barrier follows
+  const int vecs = (int)(a.cols / N);
+  const float inv_c = 1.f / (float)a.cols;
+  const uint4* x = reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + row * a.ldx);
+  const uint4* res = a.residual ? reinterpret_cast<const uint4*>(static_cast<const T*>(a.residual) + row * a.ldr) : nullptr;
+  const uint4* gate =
+      a.gate ? reinterpret_cast<const uint4*>(static_cast<const T*>(a.gate) + row / a.rows_per_gate * a.cols) : nullptr;
+  const uint4* pw = static_cast<const uint4*>(a.post_weight);
+  const uint4* w = static_cast<const uint4*>(a.weight);
+  uint4 raw[kVecs], rr[kVecs];
+#pragma unroll
+  for (int k = 0; k < kVecs; ++k) {
+    const int i = G::lane() + k * G::kLanes;
+    raw[k] = i < vecs ? __ldcs(x + i) : make_uint4(0u, 0u, 0u, 0u);
+    if (res) rr[k] = i < vecs ? __ldcs(res + i) : make_uint4(0u, 0u, 0u, 0u);
+  }
+  float v[kVecs][N];
+#pragma unroll
+  for (int k = 0; k < kVecs; ++k) unpack16<T>(raw[k], v[k]);
+  if (a.h) {
+    if (pw) {
+      float s = 0.f;
+#pragma unroll
+      for (int k = 0; k < kVecs; ++k)
+#pragma unroll
+        for (int j = 0; j < N; ++j) s = fmaf(v[k][j], v[k][j], s);
+      const float post = rsqrtf(G::sum(s, red) * inv_c + a.eps);
+#pragma unroll
+      for (int k = 0; k < kVecs; ++k) {
+        const int i = G::lane() + k * G::kLanes;
+        if (i < vecs) {
+          float f[N];
+          unpack16<T>(__ldg(pw + i), f);
+#pragma unroll
+          for (int j = 0; j < N; ++j) v[k][j] = v[k][j] * post * (f[j] + a.offset);
+        }
+      }
+    }
+    T* h = static_cast<T*>(a.h) + row * a.cols;
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k) {
+      const int i = G::lane() + k * G::kLanes;
+      if (i < vecs) {
+        if (gate) {
+          float f[N];
+          unpack16<T>(__ldg(gate + i), f);
+#pragma unroll
+          for (int j = 0; j < N; ++j) v[k][j] *= f[j];
+        }
+        float f[N];
+        if (res) unpack16<T>(rr[k], f);
+        uint4 o;
+        T* po = reinterpret_cast<T*>(&o);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          po[j] = E::from_f(res ? v[k][j] * a.scale + f[j] : v[k][j] * a.scale);
+          v[k][j] = E::to_f(po[j]);
+        }
+        reinterpret_cast<uint4*>(h)[i] = o;
+      }
+    }
+  }
+  if (!w) return;
+  float s = 0.f;
+#pragma unroll
+  for (int k = 0; k < kVecs; ++k)
+#pragma unroll
+    for (int j = 0; j < N; ++j) s = fmaf(v[k][j], v[k][j], s);
+  const float pre = rsqrtf(G::sum(s, red + kWarps) * inv_c + a.eps);
+  float mn = 0.f, mx = 0.f;
+#pragma unroll
+  for (int k = 0; k < kVecs; ++k) {
+    const int i = G::lane() + k * G::kLanes;
+    if (i < vecs) {
+      float f[N];
+      unpack16<T>(__ldg(w + i), f);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        v[k][j] = v[k][j] * pre * (f[j] + a.offset);
+        mx = nan_max(mx, v[k][j]);
+        mn = nan_min(mn, v[k][j]);
+      }
+      if (a.y) {
+        uint4 o;
+        T* po = reinterpret_cast<T*>(&o);
+#pragma unroll
+        for (int j = 0; j < N; ++j) po[j] = E::from_f(v[k][j]);
+        reinterpret_cast<uint4*>(static_cast<T*>(a.y) + row * a.cols)[i] = o;
+      }
+    }
+  }
+  if (!a.codes) return;
+  const bool sym = a.zeros == nullptr;
+  G::range(mn, mx, red + 2 * kWarps);
+  const RowQuant q = row_quant_of(mn, mx, sym);
+  int8_t* out = a.codes + row * a.ldc;
+#pragma unroll
+  for (int k = 0; k < kVecs; ++k) {
+    const int i = G::lane() + k * G::kLanes;
+    if (i < vecs) store_row_codes<N>(out + i * N, v[k], q, sym);
+  }
+  if (G::lane() == 0) {
+    a.scales[row] = q.s;
+    if (!sym) a.zeros[row] = q.z;
+  }
+}
+
+// whether norm_rows_kernel took the rows
+template <typename T>
+bool launch_rows(const NormArgs& a, cudaStream_t st) {
+  constexpr int N = Elem<T>::kPerVec;
+  if (a.cols % N || (a.rows > 1 && (a.ldx % N || (a.residual && a.ldr % N) || (a.codes && a.ldc % N))) ||
+      a.rows > 0x7fffffff ||
+      (reinterpret_cast<uintptr_t>(a.codes) & (N - 1)))
+    return false;
+  for (const void* p : {a.x, a.residual, a.post_weight, a.gate, a.weight, (const void*)a.h, (const void*)a.y})
+    if (!aligned16(p)) return false;                                   // NULL counts as aligned
+  return with_row_shape(a.cols / N, [&](auto shape) {
+    using S = decltype(shape);
+    using G = RowGroup<S::kWarps>;
+    norm_rows_kernel<T, S::kWarps, S::kVecs><<<(unsigned)((a.rows + G::kRows - 1) / G::kRows), G::kThreads, 0, st>>>(a);
+  });
+}
+
 template <typename T>
 int launch(const NormArgs& a, cudaStream_t st) {
+  if (launch_rows<T>(a, st)) {
+    LC_LAUNCH_CHECK();
+    return LC_OK;
+  }
   const int64_t cap = (int64_t)kNumSMsB200 * 8;
   norm_any_kernel<T><<<(unsigned)(a.rows < cap ? a.rows : cap), kThreads, 0, st>>>(a);
   LC_LAUNCH_CHECK();

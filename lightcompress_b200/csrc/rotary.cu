@@ -41,49 +41,141 @@ __device__ __forceinline__ float2 turn(int64_t pos, float freq, float scale) {
   return make_float2(c * scale, s * scale);
 }
 
-// One CTA per token: the token's cosines and sines go to shared memory, then every head of q and k is turned.
-template <typename T, bool kInter>
-__global__ void __launch_bounds__(kThreads) rotary_any_kernel(RotaryArgs a) {
+// x / d for x < 2^20 and d <= 1024 as a multiplication: m = ceil(2^32 / d) is off by e < d / 2^32 of itself, and
+// x * e < 2^30
+struct Divider {
+  uint32_t d, m;
+};
+__device__ __forceinline__ uint32_t quotient(uint32_t x, const Divider& v) { return v.d == 1 ? x : __umulhi(x, v.m); }
+
+// V elements move as one access.  A head is R/2/V items that turn two vectors (halves) or R/V that turn the V/2 pairs of
+// one (interleaved), and (D - R)/V items that are copied; a CTA takes `per_cta` tokens, whose cosines and sines it forms
+// in shared memory first.
+template <typename T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
+
+struct Shape {
+  int per_head, turned;      // items of a head, and those among them that turn
+  int heads;                 // q's and k's
+  int per_cta;               // tokens
+  Divider by_head, by_token; // per_head; heads
+};
+
+template <typename T, int V, bool kInter>
+__global__ void __launch_bounds__(kThreads) rotary_kernel(RotaryArgs a, Shape sh) {
   using E = Elem<T>;
+  using P = Pack<T, V>;
   extern __shared__ float2 cs[];
   const int half = a.R / 2;
-  for (int64_t tok = blockIdx.x; tok < a.B * a.T; tok += gridDim.x) {
-    const int64_t b = tok / a.T, t = tok % a.T;
-    __syncthreads();
-    for (int i = threadIdx.x; i < half; i += kThreads)
-      cs[i] = turn(a.positions[b * a.pos_b + t], a.inv_freq[i], a.scale);
-    __syncthreads();
-    const int per_head = half + (a.D - a.R);          // a pair, or an element that is copied
-    for (int idx = threadIdx.x; idx < (a.q.heads + a.k.heads) * per_head; idx += kThreads) {
-      int head = idx / per_head;
-      const int i = idx % per_head;
-      const bool is_k = head >= a.q.heads;
-      const Heads& s = is_k ? a.k : a.q;
-      if (is_k) head -= a.q.heads;
-      const T* in = static_cast<const T*>(s.in) + b * s.in_b + t * s.in_t + head * s.in_h;
-      T* out = static_cast<T*>(s.out) + b * s.out_b + t * s.out_t + head * s.out_h;
-      if (i < half) {
-        const int i1 = kInter ? 2 * i : i, i2 = kInter ? 2 * i + 1 : i + half;
-        const float x1 = E::to_f(in[i1]), x2 = E::to_f(in[i2]);
-        const float2 w = cs[i];
-        out[i1] = E::from_f(x1 * w.x - x2 * w.y);
-        out[i2] = E::from_f(x2 * w.x + x1 * w.y);
+  const int64_t tok0 = (int64_t)blockIdx.x * sh.per_cta;
+  const int tokens = (int)min((int64_t)sh.per_cta, a.B * a.T - tok0);
+  for (int j = threadIdx.x; j < tokens * half; j += kThreads) {
+    const int64_t tok = tok0 + j / half;
+    cs[j] = turn(a.positions[tok / a.T * a.pos_b + tok % a.T], a.inv_freq[j % half], a.scale);
+  }
+  __syncthreads();
+  const uint32_t items = (uint32_t)(tokens * sh.heads * sh.per_head);
+#pragma unroll 2
+  for (uint32_t idx = threadIdx.x; idx < items; idx += kThreads) {
+    const uint32_t th = quotient(idx, sh.by_head), i = idx - th * sh.per_head;
+    const uint32_t tl = quotient(th, sh.by_token);
+    int head = (int)(th - tl * sh.heads);
+    const int64_t tok = tok0 + tl, b = a.B == 1 ? 0 : tok / a.T, t = tok - b * a.T;
+    const bool is_k = head >= a.q.heads;
+    const Heads& s = is_k ? a.k : a.q;
+    if (is_k) head -= a.q.heads;
+    const T* in = static_cast<const T*>(s.in) + b * s.in_b + t * s.in_t + head * s.in_h;
+    T* out = static_cast<T*>(s.out) + b * s.out_b + t * s.out_t + head * s.out_h;
+    const float2* w = cs + tl * half;
+    if ((int)i < sh.turned) {
+      if (kInter) {
+        const int e = (int)i * V;
+        if constexpr (V == 1) {
+          // an item is a pair
+          const float x1 = E::to_f(in[2 * e]), x2 = E::to_f(in[2 * e + 1]);
+          out[2 * e] = E::from_f(x1 * w[e].x - x2 * w[e].y);
+          out[2 * e + 1] = E::from_f(x2 * w[e].x + x1 * w[e].y);
+        } else {
+          const P x = *reinterpret_cast<const P*>(in + e);
+          P o;
+#pragma unroll
+          for (int j = 0; j < V; j += 2) {
+            const float2 c = w[(e + j) / 2];
+            const float x1 = E::to_f(x.v[j]), x2 = E::to_f(x.v[j + 1]);
+            o.v[j] = E::from_f(x1 * c.x - x2 * c.y);
+            o.v[j + 1] = E::from_f(x2 * c.x + x1 * c.y);
+          }
+          *reinterpret_cast<P*>(out + e) = o;
+        }
       } else {
-        out[a.R + i - half] = in[a.R + i - half];
+        const int e = (int)i * V;
+        const P p1 = *reinterpret_cast<const P*>(in + e), p2 = *reinterpret_cast<const P*>(in + half + e);
+        P o1, o2;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const float2 c = w[e + j];
+          const float x1 = E::to_f(p1.v[j]), x2 = E::to_f(p2.v[j]);
+          o1.v[j] = E::from_f(x1 * c.x - x2 * c.y);
+          o2.v[j] = E::from_f(x2 * c.x + x1 * c.y);
+        }
+        *reinterpret_cast<P*>(out + e) = o1;
+        *reinterpret_cast<P*>(out + half + e) = o2;
       }
+    } else {
+      const int e = a.R + ((int)i - sh.turned) * V;
+      *reinterpret_cast<P*>(out + e) = *reinterpret_cast<const P*>(in + e);
     }
   }
 }
 
-template <typename T>
-int launch(const RotaryArgs& a, int interleaved, cudaStream_t st) {
-  const int64_t tokens = a.B * a.T, cap = (int64_t)kNumSMsB200 * 8;
-  const unsigned grid = (unsigned)(tokens < cap ? tokens : cap);
-  const size_t smem = (size_t)a.R / 2 * sizeof(float2);
-  if (interleaved) rotary_any_kernel<T, true><<<grid, kThreads, smem, st>>>(a);
-  else rotary_any_kernel<T, false><<<grid, kThreads, smem, st>>>(a);
+template <typename T, int V, bool kInter>
+int launch_packed(const RotaryArgs& a, cudaStream_t st) {
+  Shape sh;
+  sh.turned = kInter && V > 1 ? a.R / V : a.R / 2 / V;
+  sh.per_head = sh.turned + (a.D - a.R) / V;
+  sh.heads = a.q.heads + a.k.heads;
+  const int per_token = sh.heads * sh.per_head;
+  if (sh.per_head > 1024 || per_token >= 1 << 20) return LC_ERR_SHAPE;
+  // two items a thread at least, so that a token of few heads does not leave a CTA idle; at most 16 KB of angles
+  sh.per_cta = per_token >= 2 * kThreads ? 1 : (2 * kThreads + per_token - 1) / per_token;
+  const int room = 2048 / (a.R / 2) > 0 ? 2048 / (a.R / 2) : 1;
+  if (sh.per_cta > room) sh.per_cta = room;
+  const int64_t tokens = a.B * a.T;
+  if (sh.per_cta > tokens) sh.per_cta = (int)tokens;
+  auto divider = [](int d) { return Divider{(uint32_t)d, (uint32_t)(((1ull << 32) + d - 1) / d)}; };
+  sh.by_head = divider(sh.per_head);
+  sh.by_token = divider(sh.heads);
+  const int64_t grid = (tokens + sh.per_cta - 1) / sh.per_cta;
+  if (grid > 0x7fffffff) return LC_ERR_SHAPE;
+  rotary_kernel<T, V, kInter><<<(unsigned)grid, kThreads, (size_t)sh.per_cta * (a.R / 2) * sizeof(float2), st>>>(a, sh);
   LC_LAUNCH_CHECK();
   return LC_OK;
+}
+
+// whether every vector of V elements that the kernel touches is aligned to its size
+template <typename T>
+bool fits(const RotaryArgs& a, int v, bool inter) {
+  if (a.D % v || a.R % v || (!inter && a.R / 2 % v)) return false;
+  for (const Heads* h : {&a.q, &a.k}) {
+    if (h->heads == 0) continue;
+    const uintptr_t bytes = sizeof(T) * v;
+    if (reinterpret_cast<uintptr_t>(h->in) % bytes || reinterpret_cast<uintptr_t>(h->out) % bytes) return false;
+    for (int64_t s : {h->in_b, h->in_t, h->in_h, h->out_b, h->out_t, h->out_h})
+      if (s % v) return false;
+  }
+  return true;
+}
+
+template <typename T, bool kInter>
+int by_width(const RotaryArgs& a, cudaStream_t st) {
+  constexpr int N = Elem<T>::kPerVec;
+  if (fits<T>(a, N, kInter)) return launch_packed<T, N, kInter>(a, st);
+  if (fits<T>(a, 2, kInter)) return launch_packed<T, 2, kInter>(a, st);
+  return launch_packed<T, 1, kInter>(a, st);
+}
+
+template <typename T>
+int launch(const RotaryArgs& a, int interleaved, cudaStream_t st) {
+  return interleaved ? by_width<T, true>(a, st) : by_width<T, false>(a, st);
 }
 
 }  // namespace
@@ -97,7 +189,7 @@ extern "C" LC_API int lc_rotary_embed(const void* q, void* q_out, int q_heads, i
   using namespace lc;
   if (dtype < LC_F32 || dtype > LC_F16 || batch < 0 || tokens < 0 || q_heads < 0 || k_heads < 0) return LC_ERR_ARG;
   if (head_dim <= 0 || rotary_dim <= 0) return LC_ERR_ARG;
-  if (rotary_dim % 2 != 0 || rotary_dim > head_dim || head_dim > 1024 || q_heads > 65536 || k_heads > 65536)
+  if (rotary_dim % 2 != 0 || rotary_dim > head_dim || head_dim > 1024 || q_heads + (int64_t)k_heads > 1023)
     return LC_ERR_SHAPE;
   if (batch > (1 << 30) || tokens > (1 << 30)) return LC_ERR_SHAPE;
   if (batch == 0 || tokens == 0 || q_heads + k_heads == 0) return LC_OK;

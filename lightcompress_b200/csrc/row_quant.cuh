@@ -77,4 +77,103 @@ struct RowRange {
   }
 };
 
+// ---- rows in registers ---------------------------------------------------------------------------------------
+// kWarps warps hold a row, kVecs 16-byte vectors a lane; one warp to a row needs no barrier, and a CTA then holds
+// eight rows.
+template <int kWarps>
+struct RowGroup {
+  static constexpr int kRows = kWarps == 1 ? 8 : 1;            // rows of a CTA
+  static constexpr int kThreads = kWarps == 1 ? 256 : kWarps * 32;
+  static constexpr int kLanes = kWarps * 32;                   // threads of a row
+  __device__ __forceinline__ static int row() { return kWarps == 1 ? threadIdx.x >> 5 : 0; }
+  __device__ __forceinline__ static int lane() { return kWarps == 1 ? threadIdx.x & 31 : threadIdx.x; }
+
+  // The sum of v over the row's threads, the same in all of them.  red: kWarps floats of shared memory that no other
+  // reduction of this CTA uses (each call site has its own, so that one barrier a call is enough).
+  __device__ __forceinline__ static float sum(float v, float* red) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (kWarps == 1) return v;
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    float s = red[0];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) s += red[w];
+    return s;
+  }
+  // min and max likewise; red: 2 * kWarps floats
+  __device__ __forceinline__ static void range(float& mn, float& mx, float* red) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      mx = nan_max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      mn = nan_min(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+    }
+    if (kWarps == 1) return;
+    if ((threadIdx.x & 31) == 0) {
+      red[threadIdx.x >> 5] = mx;
+      red[kWarps + (threadIdx.x >> 5)] = mn;
+    }
+    __syncthreads();
+    mx = red[0];
+    mn = red[kWarps];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) {
+      mx = nan_max(mx, red[w]);
+      mn = nan_min(mn, red[kWarps + w]);
+    }
+  }
+};
+
+// both forms from a row's minimum and maximum (zero included): max |v| is the larger of the two magnitudes
+__device__ __forceinline__ RowQuant row_quant_of(float mn, float mx, bool sym) {
+  return sym ? row_quant<true>(0.f, nan_max(mx, -mn)) : row_quant<false>(mn, mx);
+}
+
+// the codes of N (4 or 8) neighbouring values, stored at p (N-byte aligned)
+template <int N>
+__device__ __forceinline__ void store_row_codes(int8_t* p, const float (&v)[N], const RowQuant& q, bool sym) {
+  uint32_t w[N / 4];
+#pragma unroll
+  for (int j = 0; j < N / 4; ++j) {
+    if (q.bad) {
+      w[j] = 0u;
+    } else if (sym) {
+      w[j] = pack4(row_code<true>(v[4 * j], q), row_code<true>(v[4 * j + 1], q), row_code<true>(v[4 * j + 2], q),
+                   row_code<true>(v[4 * j + 3], q));
+    } else {
+      w[j] = pack4(row_code<false>(v[4 * j], q), row_code<false>(v[4 * j + 1], q), row_code<false>(v[4 * j + 2], q),
+                   row_code<false>(v[4 * j + 3], q));
+    }
+  }
+  if (N == 4) *reinterpret_cast<uint32_t*>(p) = w[0];
+  else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[N / 4 - 1]);
+}
+
+template <typename T>
+__device__ __forceinline__ void unpack16(const uint4& v, float (&f)[Elem<T>::kPerVec]) {
+  const T* p = reinterpret_cast<const T*>(&v);
+#pragma unroll
+  for (int i = 0; i < Elem<T>::kPerVec; ++i) f[i] = Elem<T>::to_f(p[i]);
+}
+
+// Which kernel holds rows of `vecs` 16-byte vectors: f(kWarps, kVecs) as integral constants; false where none does.
+// One warp to a row up to 2 KB (no barrier); four warps with up to four vectors a lane, which keeps enough CTAs on an
+// SM to cover the barriers; eight warps up to 32 KB.
+template <int W, int V> struct RowShape {
+  static constexpr int kWarps = W, kVecs = V;
+};
+template <typename F>
+bool with_row_shape(int64_t vecs, F&& f) {
+  if (vecs <= 32) f(RowShape<1, 1>{});
+  else if (vecs <= 64) f(RowShape<1, 2>{});
+  else if (vecs <= 128) f(RowShape<1, 4>{});
+  else if (vecs <= 256) f(RowShape<4, 2>{});
+  else if (vecs <= 512) f(RowShape<4, 4>{});
+  else if (vecs <= 1024) f(RowShape<8, 4>{});
+  else if (vecs <= 1536) f(RowShape<8, 6>{});
+  else if (vecs <= 2048) f(RowShape<8, 8>{});
+  else return false;
+  return true;
+}
+
 }  // namespace lc
