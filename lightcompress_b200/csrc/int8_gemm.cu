@@ -245,6 +245,210 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
   if (threadIdx.x == 0 && !ok && g.status) atomicExch(g.status, (int)LC_ERR_TIMEOUT);
 }
 
+// ---- large products: two SMs on one 256 x 256 tile ---------------------------------------------------------------
+// cta_group::2: a pair of CTAs holds 256 channels x 256 tokens, each SM 128 channels (TMEM lanes) of all 256 tokens; a
+// 128-deep k block is 16 KB of weights and 16 KB of tokens per SM, i.e. 128 products per byte that crosses from L2,
+// against 64 for the one-SM tile above.  Persistent, one pair per two SMs; six stages; two accumulators of 256 columns, so
+// that eight warps finish one tile while the tensor cores work on the next.  Warp 0 of each CTA copies its own operands and
+// signals the leader's barrier, warp 1 of the leader issues the MMAs for both, warps 2 - 9 finish.
+// The kernel asks for all of an SM's shared memory: no other CTA that needs tensor memory can then lie beside it and
+// wait for its columns while it waits for theirs.
+constexpr int kPairRows = 256, kPairTokens = 256, kPairStages = 6, kPairBufs = 2;
+constexpr int kHalfBytes = 128 * kBlockK;                   // 128 rows of either operand
+constexpr int kPairStageBytes = 2 * kHalfBytes;
+constexpr int kFinishWarps = 8, kPairThreads = 64 + 32 * kFinishWarps;
+
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void umma_i8_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}"
+      ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc)
+      : "memory");
+}
+// arrives on the same barrier of both CTAs
+__device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+      ::"r"(bar), "h"((uint16_t)3)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
+}
+
+struct PairTiles {
+  int n_tiles, m_tiles, tokens_first;      // tokens_first: consecutive tiles differ in their tokens
+};
+
+template <typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+pair_kernel(const __grid_constant__ Maps maps, Int8Args g, PairTiles pt) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
+  const uint32_t bar0 = base + kPairStages * kPairStageBytes;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen + kPairStages * kPairStageBytes + 8 * (2 * kPairStages + 2 * kPairBufs + 1));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  auto full_bar = [&](int s) { return bar0 + 8u * s; };
+  auto empty_bar = [&](int s) { return bar0 + 8u * (kPairStages + s); };
+  auto acc_full = [&](int b) { return bar0 + 8u * (2 * kPairStages + b); };
+  auto acc_empty = [&](int b) { return bar0 + 8u * (2 * kPairStages + kPairBufs + b); };
+  const uint32_t retired = bar0 + 8u * (2 * kPairStages + 2 * kPairBufs);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = blockIdx.x & 1u;
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int blocks = (g.K + kBlockK - 1) / kBlockK;
+  const int tiles = pt.n_tiles * pt.m_tiles;
+  auto origin = [&](int t, int& n0, int& m0) {
+    const int a = t % (pt.tokens_first ? pt.m_tiles : pt.n_tiles), b = t / (pt.tokens_first ? pt.m_tiles : pt.n_tiles);
+    n0 = (pt.tokens_first ? b : a) * kPairRows;
+    m0 = (pt.tokens_first ? a : b) * kPairTokens;
+  };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kPairStages; ++s) {
+      mbar_init(full_bar(s), 1);                  // the leader's: its producer's arrival and both CTAs' bytes
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int b = 0; b < kPairBufs; ++b) {
+      mbar_init(acc_full(b), 1);
+      mbar_init(acc_empty(b), 2 * kFinishWarps);  // the leader's: the finishing warps of both CTAs
+    }
+    mbar_init(retired, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"((uint32_t)(kPairBufs * kPairTokens))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  cluster_sync();                                 // the peer's barriers exist before anything is sent to them
+  tcgen05_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  grid_dependency_wait();
+
+  uint32_t issued = 0;                            // k blocks requested (thread 0)
+  if (warp == 0) {
+    if (lane == 0) {
+      int s = 0;
+      uint32_t ph = 1;
+      bool ok = true;
+      for (int t = pair; ok && t < tiles; t += pairs) {
+        int n0, m0;
+        origin(t, n0, m0);
+        for (int kb = 0; kb < blocks; ++kb) {
+          if (!mbar_wait(empty_bar(s), ph, abort_flag)) { ok = false; break; }
+          if (rank == 0) mbar_expect_tx(full_bar(s), 2 * kPairStageBytes);
+          const uint32_t bar = in_cta(full_bar(s), 0), sa = base + s * kPairStageBytes;
+          tma_load_pair(sa, &maps.w, kb * kBlockK, n0 + (int)rank * 128, bar);
+          tma_load_pair(sa + kHalfBytes, &maps.x, kb * kBlockK, m0 + (int)rank * 128, bar);
+          ++issued;
+          if (++s == kPairStages) s = 0, ph ^= 1u;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      int s = 0, buf = 0;
+      uint32_t ph = 0, aph = 1;
+      bool ok = true;
+      for (int t = pair; ok && t < tiles; t += pairs) {
+        if (!mbar_wait(acc_empty(buf), aph, abort_flag)) break;
+        tcgen05_fence_after();
+        const uint32_t acc = tmem + (uint32_t)(buf * kPairTokens);
+        for (int kb = 0; kb < blocks; ++kb) {
+          if (!mbar_wait(full_bar(s), ph, abort_flag)) { ok = false; break; }
+          tcgen05_fence_after();
+          const uint32_t sw = base + s * kPairStageBytes, sx = sw + kHalfBytes;
+#pragma unroll
+          for (int j = 0; j < kBlockK / 32; ++j)
+            umma_i8_pair(acc, make_desc_mn_sw128(sw + j * 32, 16, 1024), make_desc_mn_sw128(sx + j * 32, 16, 1024),
+                         idesc_i8(kPairRows, kPairTokens), (kb | j) ? 1u : 0u);
+          umma_commit_pair(empty_bar(s));
+          if (++s == kPairStages) s = 0, ph ^= 1u;
+        }
+        umma_commit_pair(acc_full(buf));
+        if (++buf == kPairBufs) buf = 0, aph ^= 1u;
+      }
+      if (*abort_flag) {
+        // the MMAs already issued retire before the tensor memory is freed
+        umma_commit_pair(retired);
+        for (uint32_t it = 0; it < kSpinLimit && !mbar_test(retired, 0); ++it) __nanosleep(50);
+      }
+    }
+  } else {
+    const int q = warp & 3, h = (warp - 2) >> 2;            // TMEM lane quarter; half of the tile's tokens
+    int buf = 0;
+    uint32_t aph = 0;
+    bool ok = true;
+    for (int t = pair; t < tiles; t += pairs) {
+      int n0, m0;
+      origin(t, n0, m0);
+      const int n = n0 + (int)rank * 128 + q * 32 + lane;
+      const bool col_ok = n < g.N;
+      const float b_s = col_ok ? g.b_s[n] : 0.f;
+      const float bias = col_ok && g.bias ? Elem<T>::to_f(static_cast<const T*>(g.bias)[n]) : 0.f;
+      const int b_sum = col_ok && g.a_z ? g.b_sum[n] : 0;
+      // once a wait has expired, the tiles that remain are written as NaN
+      ok = ok && mbar_wait(acc_full(buf), aph, abort_flag) && *abort_flag == 0;
+      tcgen05_fence_after();
+      const uint32_t taddr = tmem + (uint32_t)(buf * kPairTokens + h * 128) + ((uint32_t)(q * 32) << 16);
+      const int mt = m0 + h * 128, tokens = min(128, g.M - mt);
+      T* out = static_cast<T*>(g.c) + (int64_t)mt * g.N + n;
+#pragma unroll 1
+      for (int t0 = 0; t0 < tokens; t0 += 16) {
+        uint32_t v[16];
+        tmem_ld16(taddr + t0, v);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int m = mt + t0 + i;
+          if (t0 + i < tokens && col_ok) {
+            const float y = finish((int)v[i], g.a_s[m], g.a_z ? g.a_z[m] : 0, b_s, b_sum, bias);
+            out[(int64_t)(t0 + i) * g.N] = Elem<T>::from_f(ok ? y : __int_as_float(0x7fffffff));
+          }
+        }
+      }
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(in_cta(acc_empty(buf), 0));
+      if (++buf == kPairBufs) buf = 0, aph ^= 1u;
+    }
+  }
+
+  __syncwarp();
+  __syncthreads();
+  const bool lost = *abort_flag != 0;
+  if (lost && threadIdx.x == 0 && rank == 0) {
+    // the copies still in flight (both CTAs') land before shared memory is released
+    for (uint32_t i = issued > kPairStages ? issued - kPairStages : 0; i < issued; ++i)
+      for (uint32_t it = 0; it < kSpinLimit && !mbar_test(full_bar(i % kPairStages), (i / kPairStages) & 1u); ++it)
+        __nanosleep(50);
+  }
+  if (lost && threadIdx.x == 0 && g.status) atomicExch(g.status, (int)LC_ERR_TIMEOUT);
+  tcgen05_fence_before();
+  __syncthreads();
+  cluster_sync();                                 // no CTA leaves while the other may still signal it or read its operands
+  tcgen05_fence_after();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)(kPairBufs * kPairTokens))
+                 : "memory");
+}
+
 int encode_codes(CUtensorMap* m, const int8_t* p, int64_t k, int64_t rows, int64_t ld, int box_rows) {
   EncodeTiledFn encode = get_encode_fn();
   if (!encode) return LC_ERR_CUDA;
@@ -296,7 +500,36 @@ int launch_stream(const Int8Args& g, bool dependent, cudaStream_t st) {
 }
 
 template <typename T>
+int launch_pair(const Int8Args& g, bool dependent, cudaStream_t st) {
+  Maps maps;
+  int rc;
+  if ((rc = encode_codes(&maps.w, g.b, g.K, g.N, g.ldb, 128)) != LC_OK) return rc;
+  if ((rc = encode_codes(&maps.x, g.a, g.K, g.M, g.lda, 128)) != LC_OK) return rc;
+  PairTiles pt;
+  pt.n_tiles = (g.N + kPairRows - 1) / kPairRows;
+  pt.m_tiles = (g.M + kPairTokens - 1) / kPairTokens;
+  pt.tokens_first = pt.m_tiles <= pt.n_tiles;
+  const int64_t tiles = (int64_t)pt.n_tiles * pt.m_tiles;
+  if (tiles > 0x3fffffff) return LC_ERR_SHAPE;
+  const int pairs = (int)(tiles < kNumSMsB200 / 2 ? tiles : kNumSMsB200 / 2);
+  LC_CHECK_CUDA(cudaFuncSetAttribute(pair_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost));
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * pairs));
+  cfg.blockDim = dim3(kPairThreads);
+  cfg.dynamicSmemBytes = kSmemMost;
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = dependent ? 1 : 0;
+  LC_CHECK_CUDA(cudaLaunchKernelEx(&cfg, pair_kernel<T>, maps, g, pt));
+  return LC_OK;
+}
+
+template <typename T>
 int launch(const Int8Args& g, bool dependent, cudaStream_t st) {
+  if (g.M > 128 && (int64_t)((g.M + 255) / 256) * ((g.N + 255) / 256) >= 74) return launch_pair<T>(g, dependent, st);
   if (g.M <= 16) return launch_stream<T, 16>(g, dependent, st);
   if (g.M <= 32) return launch_stream<T, 32>(g, dependent, st);
   if (g.M <= 64) return launch_stream<T, 64>(g, dependent, st);
