@@ -161,32 +161,36 @@ def call(name, *args):
     check(name, getattr(lib, name)(*args))
 
 
-def launch(t, name, *args):
-    """call(name, *args, stream) on t's device and torch's current stream there, whichever device is current; the
-    caller's current device is what it was afterwards."""
-    dev, cur = t.get_device(), torch.cuda.current_device()
-    fn = getattr(lib, name)
+# the handle of torch's current stream on a device, without making a Stream object of it
+_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
+
+def launch(dev, name, *args):
+    """call(name, *args, stream) on device `dev` (a tensor's get_device()) and torch's current stream there, whichever
+    device is current; the caller's current device is what it was afterwards.  Tensors without a device end here."""
+    if dev < 0:
+        raise RuntimeError('lightcompress_b200 kernels need CUDA tensors; there is no CPU path')
+    cur = torch.cuda.current_device()
     if dev == cur:
         lib.lc_set_device(dev)
-        code = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+        code = getattr(lib, name)(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
             try:
                 check('lc_set_device', lib.lc_set_device(dev))
-                code = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+                code = getattr(lib, name)(*args, _raw_stream(dev))
             finally:
                 lib.lc_set_device(cur)
     if code != LC_OK:
         check(name, code)
 
 
-def require_inference(name, *tensors):
-    """The kernels have no backward pass: a call that would silently cut a graph is refused."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f'{name} has no backward pass: call it under torch.no_grad(), or on detached tensors')
+def refuse_grad(name):
+    raise RuntimeError(f'{name} has no backward pass: call it under torch.no_grad(), or on detached tensors')
 
 
-def require_same_device(name, t, **others):
+def refuse_devices(name, t, **others):
+    """Says which of the tensors is not where t is."""
     for key, o in others.items():
         if o is not None and o.device != t.device:
             raise ValueError(f'{name}: {key} is on {o.device}, not on {t.device}')

@@ -246,48 +246,70 @@ def residual_norm(x, residual=None, weight=None, post_weight=None, gate=None, sc
     Returns (h, y).  Without weight, y is None.  With quant, y is what int8_linear.act_quant returns for it, (codes,
     scales) or, with sym=False, (codes, scales, zeros), quantised from fp32.  Where h would equal x, it is x."""
     name = 'residual_norm'
-    dt = L.lc_dtype(x)
-    L.require_inference(name, x, residual, weight, post_weight, gate)
-    if x.dim() == 0 or x.shape[-1] == 0:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight, post_weight, gate)):
+        L.refuse_grad(name)
+    dtype, shape, dev = x.dtype, x.shape, x.get_device()
+    dt = L._DTYPES.get(dtype)
+    if dt is None:
+        raise TypeError(f'{name}: unsupported dtype {dtype}')
+    C = shape[-1] if shape else 0
+    if C == 0:
         raise ValueError(f'{name}: the last dimension must not be empty')
-    C = x.shape[-1]
-    for key, t in (('residual', residual), ('weight', weight), ('post_weight', post_weight), ('gate', gate)):
-        if t is not None and t.dtype != x.dtype:
-            raise TypeError(f'{name}: {key} is {t.dtype}, x is {x.dtype}')
-        if t is not None and key.endswith('weight') and tuple(t.shape) != (C,):
-            raise ValueError(f'{name}: {key} must have shape ({C},), got {tuple(t.shape)}')
-    if residual is not None and residual.shape != x.shape:
-        raise ValueError(f'{name}: residual {tuple(residual.shape)} and x {tuple(x.shape)} differ')
-    if quant and weight is None:
+    rows, gate_rows = x.numel() // C, 0
+    contiguous = x.is_contiguous()
+    if contiguous:
+        x2, ldx = x, C
+    else:
+        x2 = _strided_rows(x)
+        ldx = x2.stride(0)
+    r2, ldr = residual, C
+    if residual is not None:
+        if residual.shape != shape or residual.dtype != dtype or residual.get_device() != dev:
+            _refuse_operand(name, 'residual', residual, x, shape)
+        if not residual.is_contiguous():
+            r2 = _strided_rows(residual)
+            ldr = r2.stride(0)
+    if weight is not None:
+        if weight.dtype != dtype or weight.dim() != 1 or weight.numel() != C or weight.get_device() != dev:
+            _refuse_operand(name, 'weight', weight, x, (C,))
+        weight = weight.contiguous()
+    elif quant:
         raise ValueError(f'{name}: quant needs the weight of the norm whose result it quantises')
-    gate_rows = 0
+    if post_weight is not None:
+        if post_weight.dtype != dtype or post_weight.dim() != 1 or post_weight.numel() != C or post_weight.get_device() != dev:
+            _refuse_operand(name, 'post_weight', post_weight, x, (C,))
+        post_weight = post_weight.contiguous()
     if gate is not None:
         gate_rows = _gate_rows(gate, x)
-        if gate_rows is None:
-            raise ValueError(f'{name}: gate {tuple(gate.shape)} must be ({C},), one row per leading index, or x\'s shape')
+        if gate_rows is None or gate.dtype != dtype or gate.get_device() != dev:
+            _refuse_operand(name, 'gate', gate, x, None if gate_rows is None else gate.shape)
         gate = gate.contiguous()
-    L.require_same_device(name, x, residual=residual, weight=weight, post_weight=post_weight, gate=gate)
-    L.require_cuda(x)
-    x2 = _strided_rows(x)
-    r2 = None if residual is None else _strided_rows(residual)
-    rows = x2.shape[0]
     kept = residual is None and post_weight is None and gate is None and scale == 1.0
     if kept and weight is None:
         return x, None
-    h = x if kept else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    h = x if kept else torch.empty_like(x) if contiguous else x.new_empty(shape)
     y = codes = scales = zeros = None
     pitch = 0
     if quant:
-        codes, pitch, scales, zeros = int8_linear._codes_like(x2, sym)
+        codes, pitch, scales, zeros = int8_linear._codes_like(x, rows, C, sym)
     elif weight is not None:
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        y = torch.empty_like(x) if contiguous else x.new_empty(shape)
     if rows:
-        weight = None if weight is None else weight.contiguous()
-        post_weight = None if post_weight is None else post_weight.contiguous()
-        L.launch(x2, 'lc_residual_norm', x2.data_ptr(), _at(r2), _at(post_weight), _at(gate), gate_rows, _at(weight), dt, rows, C,
-                 x2.stride(0), 0 if r2 is None else r2.stride(0), float(scale), float(eps), float(weight_offset),
-                 None if kept else h.data_ptr(), _at(y), _at(codes), pitch, _at(scales), _at(zeros))
-    return h, int8_linear._shaped(codes, scales, zeros, x.shape) if quant else y
+        L.launch(dev, 'lc_residual_norm', x2.data_ptr(), _at(r2), _at(post_weight), _at(gate), gate_rows, _at(weight), dt, rows,
+                 C, ldx, ldr, scale, eps, weight_offset, None if kept else h.data_ptr(), _at(y), _at(codes), pitch, _at(scales),
+                 _at(zeros))
+    return h, int8_linear._shaped(codes, scales, zeros, shape) if quant else y
+
+
+def _refuse_operand(name, key, t, x, shape):
+    """Says what is wrong with an operand that does not go with x."""
+    if t.dtype != x.dtype:
+        raise TypeError(f'{name}: {key} is {t.dtype}, x is {x.dtype}')
+    if shape is None:
+        raise ValueError(f'{name}: gate {tuple(t.shape)} must be ({x.shape[-1]},), one row per leading index, or x\'s shape')
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f'{name}: {key} must have shape {tuple(shape)}, got {tuple(t.shape)}')
+    L.refuse_devices(name, x, **{key: t})
 
 
 def _at(t):
@@ -304,47 +326,60 @@ def rotary_embed(q, k, positions, inv_freq, interleaved=False, attention_scale=1
     positions: int64, (B, T), (1, T) or (T,); inv_freq: (R / 2,) fp32, see rope_frequencies.  Returns (q, k) in new memory,
     (B, T, H, D) contiguous seen as (B, H, T, D) like the stock projections, or the given tensors if inplace."""
     name = 'rotary_embed'
-    dt = L.lc_dtype(q)
-    L.require_inference(name, q, k, inv_freq)
+    if torch.is_grad_enabled() and (q.requires_grad or inv_freq.requires_grad or (k is not None and k.requires_grad)):
+        L.refuse_grad(name)
+    dt = L._DTYPES.get(q.dtype)
+    if dt is None:
+        raise TypeError(f'{name}: unsupported dtype {q.dtype}')
     if q.dim() != 4 or (k is not None and k.dim() != 4):
         raise ValueError(f'{name}: q and k must be (B, heads, T, D)')
     B, H, T, D = q.shape
-    if k is not None and (k.dtype != q.dtype or k.shape[0] != B or k.shape[2:] != q.shape[2:]):
-        raise ValueError(f'{name}: k {tuple(k.shape)} {k.dtype} does not go with q {tuple(q.shape)} {q.dtype}')
-    if positions.dtype != torch.int64 or tuple(positions.shape) not in ((B, T), (1, T), (T,)):
+    G = 0
+    if k is not None:
+        kb, G, kt, kd = k.shape
+        if kb != B or kt != T or kd != D or k.dtype != q.dtype:
+            raise ValueError(f'{name}: k {tuple(k.shape)} {k.dtype} does not go with q {tuple(q.shape)} {q.dtype}')
+    shape = tuple(positions.shape)
+    if positions.dtype != torch.int64 or shape not in ((B, T), (1, T), (T,)):
         raise ValueError(f'{name}: positions must be int64 of shape ({B}, {T}), (1, {T}) or ({T},), got {positions.dtype} '
-                         f'{tuple(positions.shape)}')
-    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not 0 < 2 * inv_freq.numel() <= D:
+                         f'{shape}')
+    half = inv_freq.numel()
+    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or not 0 < 2 * half <= D:
         raise ValueError(f'{name}: inv_freq must be between 1 and {D // 2} fp32 values, got {inv_freq.dtype} '
                          f'{tuple(inv_freq.shape)}')
-    if D > 1024 or H + (0 if k is None else k.shape[1]) > 1023:
-        raise NotImplementedError(f'{name}: heads of at most 1024 elements and at most 1023 of them, got {D} and '
-                                  f'{H + (0 if k is None else k.shape[1])}')
-    L.require_same_device(name, q, k=k, positions=positions, inv_freq=inv_freq)
-    L.require_cuda(q)
-    outs, args = [], []
-    for x in (q, k):
-        if x is None:
-            outs.append(None)
-            args += [None, None, 0, 0, 0, 0]
-            continue
-        if x.stride(-1) != 1 and D != 1:
-            if inplace:
-                raise ValueError(f'{name}: the elements of a head must be contiguous')
-            x = x.contiguous()
-        if inplace and any(n > 1 and s == 0 for n, s in zip(x.shape, x.stride())):
-            raise ValueError(f'{name}: cannot work in place on an expanded tensor')
-        out = x if inplace else torch.empty((B, T, x.shape[1], D), dtype=x.dtype, device=x.device).transpose(1, 2)
-        outs.append(out)
-        sb, sh, st, _ = x.stride()
-        args += [x.data_ptr(), out.data_ptr(), x.shape[1], sb, st, sh]
+    if D > 1024 or H + G > 1023:
+        raise NotImplementedError(f'{name}: heads of at most 1024 elements and at most 1023 of them, got {D} and {H + G}')
+    dev = q.get_device()
+    if not (positions.get_device() == inv_freq.get_device() == dev) or (k is not None and k.get_device() != dev):
+        L.refuse_devices(name, q, k=k, positions=positions, inv_freq=inv_freq)
+    q, q_out, qb, qh, qt = _heads(name, q, inplace)
+    if k is None:
+        k_out, k_at, ko_at, kb, kh, kt = None, None, None, 0, 0, 0
+    else:
+        k, k_out, kb, kh, kt = _heads(name, k, inplace)
+        k_at, ko_at = k.data_ptr(), k_out.data_ptr()
     if B and T:
-        positions = positions if positions.stride(-1) == 1 or T == 1 else positions.contiguous()
-        pos_b = positions.stride(0) if positions.dim() == 2 and positions.shape[0] > 1 else 0
-        inv_freq = inv_freq.contiguous()
-        L.launch(q, 'lc_rotary_embed', *args, positions.data_ptr(), pos_b, inv_freq.data_ptr(), dt, B, T, D,
-                 2 * inv_freq.numel(), int(interleaved), float(attention_scale))
-    return outs[0], outs[1]
+        positions = positions.contiguous()
+        L.launch(dev, 'lc_rotary_embed', q.data_ptr(), q_out.data_ptr(), H, qb, qt, qh, k_at, ko_at, G, kb, kt, kh,
+                 positions.data_ptr(), T if len(shape) == 2 and shape[0] > 1 else 0, inv_freq.contiguous().data_ptr(), dt, B, T, D,
+                 2 * half, interleaved, attention_scale)
+    return q_out, k_out
+
+
+def _heads(name, x, inplace):
+    """(x with contiguous heads, where its result goes, strides of batch, head and token)"""
+    sb, sh, st, sd = x.stride()
+    if sd != 1 and x.shape[3] != 1:
+        if inplace:
+            raise ValueError(f'{name}: the elements of a head must be contiguous')
+        x = x.contiguous()
+        sb, sh, st, _ = x.stride()
+    if inplace:
+        if any(s == 0 and n > 1 for n, s in zip(x.shape, (sb, sh, st))):
+            raise ValueError(f'{name}: cannot work in place on an expanded tensor')
+        return x, x, sb, sh, st
+    B, H, T, D = x.shape
+    return x, x.new_empty((B, T, H, D)).transpose(1, 2), sb, sh, st
 
 
 def rope_frequencies(rotary_dim, base=10000.0, scaling=None, seq_len=None, device='cuda'):

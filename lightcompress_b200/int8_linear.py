@@ -14,20 +14,20 @@ from . import _lib as L
 
 _ACTS = {'silu': 1, 'gelu': 2, 'gelu_tanh': 3}
 _status = {}
+_DTYPES = L._DTYPES
 
 
-def _status_of(t):
-    """The device's status word (a bounded wait that expired in a product), made on first use; None where that
-    first use is inside a capture."""
-    dev = t.get_device()
+def _status_of(t, dev):
+    """Address of the device's status word (a bounded wait that expired in a product), which is made on first use; None
+    where that first use is inside a capture."""
     s = _status.get(dev)
     if s is None:
-        if torch.cuda.is_current_stream_capturing():
+        if dev < 0 or torch.cuda.is_current_stream_capturing():
             return None
         s = torch.zeros(1, dtype=torch.int32, device=t.device)
         torch.cuda.current_stream(dev).synchronize()      # other streams may use it from here on
         _status[dev] = s
-    return s
+    return s.data_ptr()
 
 
 def check_status(device=None):
@@ -44,27 +44,29 @@ def check_status(device=None):
 
 
 def _float_rows(name, x):
-    """x (..., K) as a 2-D view (or, where no view exists, a copy) whose rows are contiguous."""
-    L.lc_dtype(x)
+    """x (..., K) as a 2-D view (or, where no view exists, a copy) whose rows are contiguous, and its type's number."""
+    dt = _DTYPES.get(x.dtype)
+    if dt is None:
+        raise TypeError(f'{name}: unsupported dtype {x.dtype}')
     if x.dim() == 0 or x.shape[-1] == 0:
         raise ValueError(f'{name}: the last dimension must not be empty')
     if x.stride(-1) != 1 and x.shape[-1] != 1:
         x = x.contiguous()
-    return x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    return (x if x.dim() == 2 else x.reshape(-1, x.shape[-1])), dt
 
 
-def _codes_like(x2, sym):
+def _codes_like(x2, rows, cols, sym):
     """Room for the codes (rows 16 bytes apart or a multiple of that, as the products read them), scales, zeros."""
-    rows, cols = x2.shape
     pitch = (cols + 15) // 16 * 16
-    codes = torch.empty((rows, pitch), dtype=torch.int8, device=x2.device)
-    scales = torch.empty((rows, 1), dtype=torch.float32, device=x2.device)
-    zeros = None if sym else torch.empty((rows, 1), dtype=torch.int32, device=x2.device)
-    return codes, pitch, scales, zeros
+    codes = x2.new_empty((rows, pitch), dtype=torch.int8)
+    scales = x2.new_empty((rows, 1), dtype=torch.float32)
+    return codes, pitch, scales, None if sym else x2.new_empty((rows, 1), dtype=torch.int32)
 
 
 def _shaped(codes, scales, zeros, shape):
-    codes = codes[:, :shape[-1]]
+    cols = shape[-1]
+    if codes.shape[1] != cols:
+        codes = codes[:, :cols]
     if len(shape) != 2:
         codes = codes.unflatten(0, shape[:-1]) if len(shape) > 2 else codes[0]
         scales = scales.reshape(*shape[:-1], 1)
@@ -77,13 +79,13 @@ def act_quant(x, sym=True):
     s = max(|x|) / 127 and q = rint(x / s), or, with a zero point, 255 steps over the token's range widened to
     hold zero, x ~ (q - z) s.  x: (..., K) of bf16, fp16 or fp32, any strides.  A token that holds a NaN or an
     infinity gets scale NaN.  The codes' rows lie a multiple of 16 bytes apart, which the products require."""
-    L.require_inference('act_quant', x)
-    x2 = _float_rows('act_quant', x)
-    L.require_cuda(x)
+    if x.requires_grad and torch.is_grad_enabled():
+        L.refuse_grad('act_quant')
+    x2, dt = _float_rows('act_quant', x)
     rows, cols = x2.shape
-    codes, pitch, scales, zeros = _codes_like(x2, sym)
+    codes, pitch, scales, zeros = _codes_like(x2, rows, cols, sym)
     if rows:
-        L.launch(x2, 'lc_int8_act_quant', x2.data_ptr(), L.lc_dtype(x2), rows, cols, x2.stride(0), codes.data_ptr(), pitch,
+        L.launch(x2.get_device(), 'lc_int8_act_quant', x2.data_ptr(), dt, rows, cols, x2.stride(0), codes.data_ptr(), pitch,
                  scales.data_ptr(), None if sym else zeros.data_ptr())
     return _shaped(codes, scales, zeros, x.shape)
 
@@ -91,20 +93,25 @@ def act_quant(x, sym=True):
 def gated_act_quant(gate, up, act='silu', sym=True):
     """act_quant(act(gate) * up) in one pass, the product formed in fp32 and not rounded in between: the input of an
     MLP's down projection.  act: 'silu', 'gelu' or 'gelu_tanh'."""
-    if act not in _ACTS:
+    kind = _ACTS.get(act)
+    if kind is None:
         raise NotImplementedError(f'gated_act_quant: activation {act!r}; there are {sorted(_ACTS)}')
-    if gate.shape != up.shape or gate.dtype != up.dtype:
-        raise ValueError(f'gated_act_quant: gate {tuple(gate.shape)} {gate.dtype} and up {tuple(up.shape)} {up.dtype} differ')
-    L.require_inference('gated_act_quant', gate, up)
-    g2, u2 = _float_rows('gated_act_quant', gate), _float_rows('gated_act_quant', up)
-    L.require_same_device('gated_act_quant', gate, up=up)
-    L.require_cuda(gate)
+    shape = gate.shape
+    if shape != up.shape or gate.dtype != up.dtype:
+        raise ValueError(f'gated_act_quant: gate {tuple(shape)} {gate.dtype} and up {tuple(up.shape)} {up.dtype} differ')
+    if (gate.requires_grad or up.requires_grad) and torch.is_grad_enabled():
+        L.refuse_grad('gated_act_quant')
+    dev = gate.get_device()
+    if up.get_device() != dev:
+        L.refuse_devices('gated_act_quant', gate, up=up)
+    g2, dt = _float_rows('gated_act_quant', gate)
+    u2, _ = _float_rows('gated_act_quant', up)
     rows, cols = g2.shape
-    codes, pitch, scales, zeros = _codes_like(g2, sym)
+    codes, pitch, scales, zeros = _codes_like(g2, rows, cols, sym)
     if rows:
-        L.launch(g2, 'lc_int8_gated_act_quant', g2.data_ptr(), u2.data_ptr(), L.lc_dtype(g2), rows, cols, g2.stride(0),
-                 u2.stride(0), _ACTS[act], codes.data_ptr(), pitch, scales.data_ptr(), None if sym else zeros.data_ptr())
-    return _shaped(codes, scales, zeros, gate.shape)
+        L.launch(dev, 'lc_int8_gated_act_quant', g2.data_ptr(), u2.data_ptr(), dt, rows, cols, g2.stride(0), u2.stride(0), kind,
+                 codes.data_ptr(), pitch, scales.data_ptr(), None if sym else zeros.data_ptr())
+    return _shaped(codes, scales, zeros, shape)
 
 
 def aligned_rows(codes):
@@ -121,16 +128,19 @@ def aligned_rows(codes):
 
 
 def _rows_aligned(t):
-    return ((t.shape[1] == 1 or t.stride(1) == 1) and t.data_ptr() % 16 == 0
-            and (t.shape[0] <= 1 or (t.stride(0) % 16 == 0 and t.stride(0) >= t.shape[1])))
+    rows, cols = t.shape
+    pitch = t.stride(0)
+    return (not t.data_ptr() & 15 and (t.stride(1) == 1 or cols == 1)
+            and ((not pitch & 15 and pitch >= cols) or rows <= 1))
 
 
-def _pitch(t):
+def _pitch(t, rows, cols):
     """Row pitch of an aligned 2-D code tensor; a single row may carry any stride."""
-    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
+    return t.stride(0) if rows > 1 else (cols + 15) // 16 * 16
 
 
 def _check_weight(name, b, b_s, b_sum, bias, zeros, out_dtype):
+    """(N, K) of the weight; refuses what the products do not take."""
     if b.dtype != torch.int8 or b.dim() != 2:
         raise TypeError(f'{name}: the weight must be int8 codes (N, K), got {b.dtype} {tuple(b.shape)}')
     N, K = b.shape
@@ -148,6 +158,7 @@ def _check_weight(name, b, b_s, b_sum, bias, zeros, out_dtype):
         raise ValueError(f'{name}: bias must be {N} contiguous values of {out_dtype}')
     if K > (65793 if zeros else 131071):
         raise ValueError(f'{name}: {K} products may leave 32 bits (at most 131071, with zero points 65793)')
+    return N, K
 
 
 def int8_gemm(a, a_s, b, b_s, bias=None, a_z=None, b_sum=None, out_dtype=torch.bfloat16):
@@ -155,13 +166,14 @@ def int8_gemm(a, a_s, b, b_s, bias=None, a_z=None, b_sum=None, out_dtype=torch.b
     them; b: (N, K) int8 with b_s (N fp32 values) and, with zero points, b_sum (N int32 sums of b's rows).  Returns
     (..., N) = ((a - a_z) b^T) * a_s * b_s + bias in out_dtype; the sum of products is exact."""
     name = 'int8_gemm'
-    L.require_inference(name, a_s, b_s, bias)
-    if out_dtype not in (torch.bfloat16, torch.float16, torch.float32):
+    if torch.is_grad_enabled() and (a_s.requires_grad or b_s.requires_grad or (bias is not None and bias.requires_grad)):
+        L.refuse_grad(name)
+    out = _DTYPES.get(out_dtype)
+    if out is None:
         raise TypeError(f'{name}: unsupported output type {out_dtype}')
     if a.dtype != torch.int8 or a.dim() == 0:
         raise TypeError(f'{name}: the activations must be int8 codes (..., K), got {a.dtype}')
-    _check_weight(name, b, b_s, b_sum, bias, a_z is not None, out_dtype)
-    N, K = b.shape
+    N, K = _check_weight(name, b, b_s, b_sum, bias, a_z is not None, out_dtype)
     if a.shape[-1] != K or K == 0:
         raise ValueError(f'{name}: activations of {a.shape[-1]} and a weight of {K} input channels')
     a2 = a if a.dim() == 2 else a.reshape(-1, K)
@@ -173,16 +185,16 @@ def int8_gemm(a, a_s, b, b_s, bias=None, a_z=None, b_sum=None, out_dtype=torch.b
         raise ValueError(f'{name}: the activations need one fp32 scale per token ({M}), contiguous')
     if a_z is not None and (a_z.dtype != torch.int32 or a_z.numel() != M or not a_z.is_contiguous()):
         raise ValueError(f'{name}: zero points must be {M} int32 values, contiguous')
-    L.require_same_device(name, a, a_s=a_s, a_z=a_z, b=b, b_s=b_s, b_sum=b_sum, bias=bias)
-    L.require_cuda(a)
-    c = torch.empty((*a.shape[:-1], N), dtype=out_dtype, device=a.device)
+    dev = a.get_device()
+    if not (a_s.get_device() == b.get_device() == b_s.get_device() == dev) or (bias is not None and bias.get_device() != dev) \
+            or (a_z is not None and not a_z.get_device() == b_sum.get_device() == dev):
+        L.refuse_devices(name, a, a_s=a_s, a_z=a_z, b=b, b_s=b_s, b_sum=b_sum, bias=bias)
+    c = a2.new_empty((M, N), dtype=out_dtype)
     if M and N:
-        s = _status_of(a)
-        L.launch(a, 'lc_int8_gemm', a2.data_ptr(), _pitch(a2), a_s.data_ptr(), None if a_z is None else a_z.data_ptr(),
-                 b.data_ptr(), _pitch(b), b_s.data_ptr(), None if a_z is None else b_sum.data_ptr(),
-                 None if bias is None else bias.data_ptr(), M, N, K, c.data_ptr(), L._DTYPES[out_dtype],
-                 None if s is None else s.data_ptr())
-    return c
+        L.launch(dev, 'lc_int8_gemm', a2.data_ptr(), _pitch(a2, M, K), a_s.data_ptr(), None if a_z is None else a_z.data_ptr(),
+                 b.data_ptr(), _pitch(b, N, K), b_s.data_ptr(), None if a_z is None else b_sum.data_ptr(),
+                 None if bias is None else bias.data_ptr(), M, N, K, c.data_ptr(), out, _status_of(a, dev))
+    return c if a.dim() == 2 else c.view(*a.shape[:-1], N)
 
 
 def int8_dynamic_forward_func(x, w, w_scale, bias=None, w_sum=None):
@@ -190,25 +202,26 @@ def int8_dynamic_forward_func(x, w, w_scale, bias=None, w_sum=None):
     values), in one call.  With w_sum (N int32 sums of w's rows) the activations get a zero point per token, without it
     they are quantised symmetrically.  Returns (..., N) of x's type; bias has that type too."""
     name = 'int8_dynamic_forward_func'
-    L.require_inference(name, x, w_scale, bias)
-    x2 = _float_rows(name, x)
+    if torch.is_grad_enabled() and (x.requires_grad or w_scale.requires_grad or (bias is not None and bias.requires_grad)):
+        L.refuse_grad(name)
+    x2, dt = _float_rows(name, x)
     sym = w_sum is None
-    _check_weight(name, w, w_scale, w_sum, bias, not sym, x.dtype)
-    N, K = w.shape
-    M = x2.shape[0]
-    if x2.shape[1] != K:
-        raise ValueError(f'{name}: activations of {x2.shape[1]} and a weight of {K} input channels')
-    L.require_same_device(name, x, w=w, w_scale=w_scale, bias=bias, w_sum=w_sum)
-    L.require_cuda(x)
-    c = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=x.device)
+    N, K = _check_weight(name, w, w_scale, w_sum, bias, not sym, x.dtype)
+    M, k = x2.shape
+    if k != K:
+        raise ValueError(f'{name}: activations of {k} and a weight of {K} input channels')
+    dev = x.get_device()
+    if not (w.get_device() == w_scale.get_device() == dev) or (bias is not None and bias.get_device() != dev) \
+            or (not sym and w_sum.get_device() != dev):
+        L.refuse_devices(name, x, w=w, w_scale=w_scale, bias=bias, w_sum=w_sum)
+    c = x2.new_empty((M, N))
     if M and N:
-        room = M * ((K + 15) // 16 * 16) + 8 * M
-        scratch = torch.empty(room, dtype=torch.int8, device=x.device)
-        s = _status_of(x)
-        L.launch(x2, 'lc_int8_linear', x2.data_ptr(), L.lc_dtype(x2), x2.stride(0), w.data_ptr(), _pitch(w), w_scale.data_ptr(),
-                 None if sym else w_sum.data_ptr(), None if bias is None else bias.data_ptr(), M, N, K, int(sym),
-                 c.data_ptr(), scratch.data_ptr(), room, None if s is None else s.data_ptr())
-    return c
+        room = M * ((K + 15) // 16 * 16 + 8)
+        scratch = x2.new_empty(room, dtype=torch.int8)
+        L.launch(dev, 'lc_int8_linear', x2.data_ptr(), dt, x2.stride(0), w.data_ptr(), _pitch(w, N, K), w_scale.data_ptr(),
+                 None if sym else w_sum.data_ptr(), None if bias is None else bias.data_ptr(), M, N, K, sym,
+                 c.data_ptr(), scratch.data_ptr(), room, _status_of(x, dev))
+    return c if x.dim() == 2 else c.view(*x.shape[:-1], N)
 
 
 class Int8Linear(nn.Module):

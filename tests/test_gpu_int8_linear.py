@@ -82,7 +82,7 @@ def test_strided_rows_and_what_lies_behind_them(dtype):
     room = torch.full((8, 320), 55, dtype=torch.int8, device='cuda')
     scales = torch.full((8,), -1.0, device='cuda')
     x = base[:6, :257].contiguous()
-    L.launch(x, 'lc_int8_act_quant', x.data_ptr(), L.lc_dtype(x), 6, 257, 257, room.data_ptr(), 320, scales.data_ptr(), None)
+    L.launch(0, 'lc_int8_act_quant', x.data_ptr(), L.lc_dtype(x), 6, 257, 257, room.data_ptr(), 320, scales.data_ptr(), None)
     q, s, _ = ref.quant_rows(x.cpu())
     assert torch.equal(room[:6, :257].cpu().long(), q) and torch.equal(scales[:6].cpu(), s)
     assert bool((room[:6, 257:] == 55).all()) and bool((room[6:] == 55).all()) and bool((scales[6:] == -1).all())
