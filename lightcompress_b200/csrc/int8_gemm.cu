@@ -38,6 +38,55 @@ __device__ __forceinline__ float finish(int acc, float a_s, int a_z, float b_s, 
   return __fadd_rn(__fmul_rn(__fmul_rn(__int2float_rn(whole), a_s), b_s), bias);
 }
 
+// What a thread knows of its output channel.
+struct Channel {
+  float b_s, bias;
+  int b_sum;
+  bool ok;                 // the channel exists
+};
+template <typename T>
+__device__ __forceinline__ Channel load_channel(const Int8Args& g, int n) {
+  Channel c{0.f, 0.f, 0, n < g.N};
+  if (c.ok) {
+    c.b_s = g.b_s[n];
+    if (g.bias) c.bias = Elem<T>::to_f(static_cast<const T*>(g.bias)[n]);
+    if (g.a_z) c.b_sum = g.b_sum[n];
+  }
+  return c;
+}
+
+// The outputs of C tokens of one channel.  s, z: the tokens' scales and zero points in shared memory (s 16-byte
+// aligned); out: the first token's element, tokens N elements apart; count: how many of the C tokens exist.  All values
+// are formed before the first store: stores may alias anything and would otherwise keep the loads behind them waiting
+// (17 us of a 512-token tile's 22 were that).
+template <typename T, int C>
+__device__ __forceinline__ void finish_tokens(const uint32_t (&v)[C], const float* s, const int* z, bool zeros,
+                                              const Channel& c, T* out, int64_t N, int count, bool lost) {
+  float y[C];
+#pragma unroll
+  for (int i = 0; i < C; i += 4) {
+    const float4 f = *reinterpret_cast<const float4*>(s + i);
+    const int4 w = zeros ? *reinterpret_cast<const int4*>(z + i) : make_int4(0, 0, 0, 0);
+    y[i] = finish((int)v[i], f.x, w.x, c.b_s, c.b_sum, c.bias);
+    y[i + 1] = finish((int)v[i + 1], f.y, w.y, c.b_s, c.b_sum, c.bias);
+    y[i + 2] = finish((int)v[i + 2], f.z, w.z, c.b_s, c.b_sum, c.bias);
+    y[i + 3] = finish((int)v[i + 3], f.w, w.w, c.b_s, c.b_sum, c.bias);
+  }
+  if (lost) {
+#pragma unroll
+    for (int i = 0; i < C; ++i) y[i] = __int_as_float(0x7fffffff);
+  }
+  if (!c.ok) return;
+  if (count >= C) {
+#pragma unroll
+    for (int i = 0; i < C; ++i) out[i * N] = Elem<T>::from_f(y[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+      if (i < count) out[i * N] = Elem<T>::from_f(y[i]);
+  }
+}
+
 // ---- weights as the 128-row operand, tokens as the columns ---------------------------------------------------
 // One CTA per 128 output channels x NT tokens x one part of K (tcgen05 kind::i8, cta_group::1): the accumulator holds
 // a channel per TMEM lane and a token per column, so a warp's store of one token is 32 neighbouring channels.  Both
@@ -45,8 +94,8 @@ __device__ __forceinline__ float finish(int acc, float a_s, int a_z, float b_s, 
 // end and the rows behind the last are filled with zeros by the copy.
 //
 // Few tokens leave the weights as the only traffic that matters (N * K bytes), and N / 128 CTAs are too few to draw
-// the HBM's bandwidth: K is split over the CTAs of a cluster, whose partial sums meet through distributed shared
-// memory.  The weights of the first `stages` blocks are requested before the kernel waits for the one that quantises
+// the HBM's bandwidth: K is split over the CTAs of a cluster.  Token t belongs to CTA t mod splits; every CTA writes its
+// partial sums into the owners' shared memory, and after one cluster barrier each owner adds and finishes its tokens.  The weights of the first `stages` blocks are requested before the kernel waits for the one that quantises
 // the activations (programmatic dependent launch), which hides it.
 constexpr int kRows = 128, kBlockK = 128, kStreamThreads = 128;
 constexpr int kWeightBytes = kRows * kBlockK;
@@ -77,31 +126,48 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
 }
 
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ int ld_cluster(uint32_t addr, int rank) {
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {
   uint32_t a;
-  int v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
-  return v;
+  return a;
+}
+__device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 
 struct Maps {
   CUtensorMap w, x;
 };
 
+// Shared memory of a CTA: stages, barriers, the tokens' scales and zero points, and the partial sums it owns, which lie in
+// the stages' memory where they are large (all CTAs of the cluster have to be done with their products then).
+template <int NT> struct StreamSmem {
+  static constexpr int kStage = kWeightBytes + NT * kBlockK;
+  static constexpr int kParts = (NT + 7) * kRows * 4;
+  static constexpr bool kOwnParts = NT <= 32;
+  __host__ __device__ static int bars(int stages) { return stages * kStage; }
+  __host__ __device__ static int scales(int stages) { return bars(stages) + (8 * (2 * stages + 1) + 8 + 15) / 16 * 16; }
+  __host__ __device__ static int parts(int stages) { return kOwnParts ? scales(stages) + NT * 8 : 0; }
+  __host__ __device__ static int bytes(int stages, bool split) {
+    return 1024 + scales(stages) + NT * 8 + (kOwnParts && split ? kParts : 0);
+  }
+};
+
 template <typename T, int NT>
 __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_constant__ Maps maps, Int8Args g, int splits,
                                                                 int stages) {
-  constexpr int kStage = kWeightBytes + NT * kBlockK;
+  using Smem = StreamSmem<NT>;
+  constexpr int kStage = Smem::kStage;
   constexpr int kCols = NT < 32 ? 32 : NT;                 // tensor memory is allocated in powers of two from 32 columns
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
-  const uint32_t bar0 = base + stages * kStage;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen + stages * kStage + 8 * (2 * stages + 1));
+  const uint32_t bar0 = base + Smem::bars(stages);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen + Smem::bars(stages) + 8 * (2 * stages + 1));
+  float* s_scale = reinterpret_cast<float*>(gen + Smem::scales(stages));
+  int* s_zero = reinterpret_cast<int*>(s_scale + NT);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
   auto empty_bar = [&](int s) { return bar0 + 8u * (stages + s); };
@@ -137,7 +203,15 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
   __syncthreads();
   tcgen05_fence_after();
   const uint32_t tmem = *tmem_slot;
+  if (splits > 1) cluster_arrive();                        // waited for before anything is sent to another CTA
+  const int tokens = min(NT, g.M - m0);
+  const int c = warp * 32 + lane, n = n0 + c;
+  const Channel ch = load_channel<T>(g, n);                // weights' side: nothing the kernel before this one writes
   grid_dependency_wait();
+  for (int t = threadIdx.x - 64; t >= 0 && t < NT; t += 64) {
+    s_scale[t] = t < tokens ? g.a_s[m0 + t] : 0.f;
+    s_zero[t] = t < tokens && g.a_z ? g.a_z[m0 + t] : 0;
+  }
 
   int issued = 0;                                          // k blocks requested, known to thread 0
   if (warp == 0) {
@@ -192,50 +266,57 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
     __syncthreads();
   }
 
-  const int c = warp * 32 + lane, n = n0 + c;
-  const bool col_ok = n < g.N;
-  const int tokens = min(NT, g.M - m0);
-  const float b_s = col_ok ? g.b_s[n] : 0.f;
-  const float bias = col_ok && g.bias ? Elem<T>::to_f(static_cast<const T*>(g.bias)[n]) : 0.f;
-  const int b_sum = col_ok && g.a_z ? g.b_sum[n] : 0;
   T* out = static_cast<T*>(g.c) + (int64_t)m0 * g.N + n;
-  const float lost = __int_as_float(0x7fffffff);
   const uint32_t taddr = tmem + ((uint32_t)(warp * 32) << 16);
+  constexpr int kChunk = NT < 32 ? 16 : 32;
+  auto accumulators = [&](int t0, uint32_t (&v)[kChunk]) {
+    if constexpr (kChunk == 16) {
+      tmem_ld16(taddr + t0, v);
+    } else {
+      tmem_ld32_nowait(taddr + t0, v);
+      tmem_wait_ld();
+    }
+  };
   if (splits == 1) {
 #pragma unroll 1
-    for (int t0 = 0; t0 < tokens; t0 += 16) {
-      uint32_t v[16];
-      tmem_ld16(taddr + t0, v);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int t = t0 + i;
-        if (t < tokens && col_ok) {
-          const float y = finish((int)v[i], g.a_s[m0 + t], g.a_z ? g.a_z[m0 + t] : 0, b_s, b_sum, bias);
-          out[(int64_t)t * g.N] = Elem<T>::from_f(ok ? y : lost);
-        }
-      }
+    for (int t0 = 0; t0 < tokens; t0 += kChunk) {
+      uint32_t v[kChunk];
+      accumulators(t0, v);
+      finish_tokens<T, kChunk>(v, s_scale + t0, s_zero + t0, g.a_z != nullptr, ch, out + (int64_t)t0 * g.N, g.N, tokens - t0,
+                               !ok);
     }
   } else {
-    // [token][channel] partial sums in the stages' memory: every copy into it has landed and every MMA read it
-    int* part = reinterpret_cast<int*>(gen);
-#pragma unroll 1
-    for (int t0 = 0; t0 < tokens; t0 += 16) {
-      uint32_t v[16];
-      tmem_ld16(taddr + t0, v);
-#pragma unroll
-      for (int i = 0; i < 16; ++i) part[(t0 + i) * kRows + c] = (int)v[i];
+    // part [t / splits][rank][channel] of token t's owner
+    const uint32_t parts = base + Smem::parts(stages);
+    cluster_wait();                                        // every CTA of the cluster runs
+    if (!Smem::kOwnParts) {
+      cluster_arrive();                                    // and has no products to form any more
+      cluster_wait();
     }
-    cluster_sync();
-    for (int r = 0; r < splits; ++r) ok = ok && ld_cluster(smem_u32(const_cast<int*>(abort_flag)), r) == 0;
-    for (int t = rank; t < tokens; t += splits) {
-      unsigned sum = 0;
-      for (int r = 0; r < splits; ++r) sum += (unsigned)ld_cluster(base + (uint32_t)(t * kRows + c) * 4u, r);
-      if (col_ok) {
-        const float y = finish((int)sum, g.a_s[m0 + t], g.a_z ? g.a_z[m0 + t] : 0, b_s, b_sum, bias);
-        out[(int64_t)t * g.N] = Elem<T>::from_f(ok ? y : lost);
+    if (!ok && threadIdx.x < (unsigned)splits)             // tell every CTA that a part is missing
+      st_cluster(in_cta(smem_u32(const_cast<int*>(abort_flag)), threadIdx.x), 1u);
+#pragma unroll 1
+    for (int t0 = 0; t0 < tokens; t0 += kChunk) {
+      uint32_t v[kChunk];
+      accumulators(t0, v);
+      int owner = t0 % splits, slot = t0 / splits * splits + rank;
+#pragma unroll
+      for (int i = 0; i < kChunk; ++i) {
+        if (t0 + i < tokens) st_cluster(in_cta(parts + (uint32_t)(slot * kRows + c) * 4u, owner), v[i]);
+        if (++owner == splits) owner = 0, slot += splits;
       }
     }
-    cluster_sync();                                        // nobody leaves while its partial sums are being read
+    cluster_arrive();
+    cluster_wait();
+    ok = *abort_flag == 0;
+    const uint32_t* mine = reinterpret_cast<const uint32_t*>(gen + Smem::parts(stages)) + c;
+#pragma unroll 4
+    for (int t = rank, k = 0; t < tokens; t += splits, k += splits) {
+      uint32_t sum = 0;
+      for (int r = 0; r < splits; ++r) sum += mine[(k + r) * kRows];
+      const float y = finish((int)sum, s_scale[t], s_zero[t], ch.b_s, ch.b_sum, ch.bias);
+      if (ch.ok) out[(int64_t)t * g.N] = Elem<T>::from_f(ok ? y : __int_as_float(0x7fffffff));
+    }
   }
   tcgen05_fence_before();
   __syncthreads();
@@ -257,6 +338,8 @@ constexpr int kPairRows = 256, kPairTokens = 256, kPairStages = 6, kPairBufs = 2
 constexpr int kHalfBytes = 128 * kBlockK;                   // 128 rows of either operand
 constexpr int kPairStageBytes = 2 * kHalfBytes;
 constexpr int kFinishWarps = 8, kPairThreads = 64 + 32 * kFinishWarps;
+constexpr int kPairScales = kPairStages * kPairStageBytes + 256;      // behind the stages and barriers: 1 KB a warp
+static_assert(1024 + kPairScales + kFinishWarps * 1024 <= kSmemMost, "");
 
 __device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
   asm volatile(
@@ -277,11 +360,6 @@ __device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
       "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
       ::"r"(bar), "h"((uint16_t)3)
       : "memory");
-}
-__device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {
-  uint32_t a;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
-  return a;
 }
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(addr) : "memory");
@@ -337,7 +415,8 @@ pair_kernel(const __grid_constant__ Maps maps, Int8Args g, PairTiles pt) {
   }
   tcgen05_fence_before();
   __syncthreads();
-  cluster_sync();                                 // the peer's barriers exist before anything is sent to them
+  cluster_arrive();                               // the peer's barriers exist before anything is sent to them
+  cluster_wait();
   tcgen05_fence_after();
   const uint32_t tmem = *tmem_slot;
   grid_dependency_wait();
@@ -393,6 +472,9 @@ pair_kernel(const __grid_constant__ Maps maps, Int8Args g, PairTiles pt) {
     }
   } else {
     const int q = warp & 3, h = (warp - 2) >> 2;            // TMEM lane quarter; half of the tile's tokens
+    // each warp keeps the scales and zero points of its 128 tokens to itself
+    float* s_scale = reinterpret_cast<float*>(gen + kPairScales) + (warp - 2) * 256;
+    int* s_zero = reinterpret_cast<int*>(s_scale + 128);
     int buf = 0;
     uint32_t aph = 0;
     bool ok = true;
@@ -400,28 +482,25 @@ pair_kernel(const __grid_constant__ Maps maps, Int8Args g, PairTiles pt) {
       int n0, m0;
       origin(t, n0, m0);
       const int n = n0 + (int)rank * 128 + q * 32 + lane;
-      const bool col_ok = n < g.N;
-      const float b_s = col_ok ? g.b_s[n] : 0.f;
-      const float bias = col_ok && g.bias ? Elem<T>::to_f(static_cast<const T*>(g.bias)[n]) : 0.f;
-      const int b_sum = col_ok && g.a_z ? g.b_sum[n] : 0;
+      const Channel ch = load_channel<T>(g, n);
+      const int mt = m0 + h * 128, tokens = min(128, g.M - mt);
+#pragma unroll
+      for (int i = lane; i < 128; i += 32) {
+        s_scale[i] = i < tokens ? g.a_s[mt + i] : 0.f;
+        if (g.a_z) s_zero[i] = i < tokens ? g.a_z[mt + i] : 0;
+      }
+      __syncwarp();
       // once a wait has expired, the tiles that remain are written as NaN
       ok = ok && mbar_wait(acc_full(buf), aph, abort_flag) && *abort_flag == 0;
       tcgen05_fence_after();
       const uint32_t taddr = tmem + (uint32_t)(buf * kPairTokens + h * 128) + ((uint32_t)(q * 32) << 16);
-      const int mt = m0 + h * 128, tokens = min(128, g.M - mt);
       T* out = static_cast<T*>(g.c) + (int64_t)mt * g.N + n;
 #pragma unroll 1
-      for (int t0 = 0; t0 < tokens; t0 += 16) {
-        uint32_t v[16];
-        tmem_ld16(taddr + t0, v);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int m = mt + t0 + i;
-          if (t0 + i < tokens && col_ok) {
-            const float y = finish((int)v[i], g.a_s[m], g.a_z ? g.a_z[m] : 0, b_s, b_sum, bias);
-            out[(int64_t)(t0 + i) * g.N] = Elem<T>::from_f(ok ? y : __int_as_float(0x7fffffff));
-          }
-        }
+      for (int t0 = 0; t0 < tokens; t0 += 32) {
+        uint32_t v[32];
+        tmem_ld32_nowait(taddr + t0, v);
+        tmem_wait_ld();
+        finish_tokens<T, 32>(v, s_scale + t0, s_zero + t0, g.a_z != nullptr, ch, out + (int64_t)t0 * g.N, g.N, tokens - t0, !ok);
       }
       tcgen05_fence_before();
       __syncwarp();
@@ -442,7 +521,8 @@ pair_kernel(const __grid_constant__ Maps maps, Int8Args g, PairTiles pt) {
   if (lost && threadIdx.x == 0 && g.status) atomicExch(g.status, (int)LC_ERR_TIMEOUT);
   tcgen05_fence_before();
   __syncthreads();
-  cluster_sync();                                 // no CTA leaves while the other may still signal it or read its operands
+  cluster_arrive();
+  cluster_wait();                                 // no CTA leaves while the other may still signal it or read its operands
   tcgen05_fence_after();
   if (warp == 1)
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)(kPairBufs * kPairTokens))
@@ -472,11 +552,12 @@ int launch_stream(const Int8Args& g, bool dependent, cudaStream_t st) {
   int splits = 1;
   while (splits < 8 && tiles * splits * 2 <= kNumSMsB200 * 2 && splits * 2 <= blocks) splits *= 2;
   const int per_sm = tiles * splits > kNumSMsB200 ? 2 : 1;
-  int stages = (kSmemMost / per_sm - 2048) / kStage;
-  const int most = (blocks + splits - 1) / splits, least = (NT * kRows * 4 + kStage - 1) / kStage;
-  if (stages > most) stages = most;
-  if (splits > 1 && stages < least) stages = least;
-  const int smem = stages * kStage + 8 * (2 * stages + 1) + 16 + 1024;
+  using Smem = StreamSmem<NT>;
+  int stages = (blocks + splits - 1) / splits;             // more than a CTA's blocks are of no use
+  while (stages > 1 && Smem::bytes(stages, splits > 1) > kSmemMost / per_sm - 1024) --stages;
+  if (splits > 1 && !Smem::kOwnParts)
+    while (stages * kStage < Smem::kParts) ++stages;       // the partial sums take the stages' place
+  const int smem = Smem::bytes(stages, splits > 1);
   Maps maps;
   int rc;
   if ((rc = encode_codes(&maps.w, g.b, g.K, g.N, g.ldb, kRows)) != LC_OK) return rc;
