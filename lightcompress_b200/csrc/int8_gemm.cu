@@ -94,10 +94,11 @@ __device__ __forceinline__ void finish_tokens(const uint32_t (&v)[C], const floa
 // end and the rows behind the last are filled with zeros by the copy.
 //
 // Few tokens leave the weights as the only traffic that matters (N * K bytes), and N / 128 CTAs are too few to draw
-// the HBM's bandwidth: K is split over the CTAs of a cluster.  Token t belongs to CTA t mod splits; every CTA writes its
-// partial sums into the owners' shared memory, and after one cluster barrier each owner adds and finishes its tokens.  The weights of the first `stages` blocks are requested before the kernel waits for the one that quantises
+// the HBM's bandwidth: K is split over the CTAs of a cluster.  Each CTA owns a run of the tile's tokens; every CTA lays its
+// partial sums out by token in shared memory, one bulk copy takes an owner's run there, and the owner adds and finishes
+// it (stores of 4 bytes to the other CTAs cost 40 ns a token: 4 us for 128 of them).  The weights of the first `stages` blocks are requested before the kernel waits for the one that quantises
 // the activations (programmatic dependent launch), which hides it.
-constexpr int kRows = 128, kBlockK = 128, kStreamThreads = 128;
+constexpr int kRows = 128, kBlockK = 128, kStreamThreads = 256;
 constexpr int kWeightBytes = kRows * kBlockK;
 constexpr int kSmemMost = 227 * 1024;
 
@@ -114,15 +115,30 @@ __device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t adesc, uint64_
       : "memory");
 }
 
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr)
-      : "memory");
+template <int C>
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[C]) {
+  static_assert(C == 8 || C == 16, "");
+  if constexpr (C == 8)
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr)
+                 : "memory");
+  else
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
   tmem_wait_ld();
+}
+
+// true in one lane of a converged warp
+__device__ __forceinline__ bool elect_one() {
+  uint32_t is;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(is));
+  return is != 0;
 }
 
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
@@ -133,25 +149,31 @@ __device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
   return a;
 }
-__device__ __forceinline__ void st_cluster(uint32_t addr, uint32_t v) {
-  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+// shared memory of this CTA -> that of a CTA of its cluster (dst and bar are addresses there)
+__device__ __forceinline__ void copy_to_cta(uint32_t dst, uint32_t src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(dst), "r"(src), "r"(bytes), "r"(bar)
+               : "memory");
 }
 
 struct Maps {
   CUtensorMap w, x;
 };
 
-// Shared memory of a CTA: stages, barriers, the tokens' scales and zero points, and the partial sums it owns, which lie in
-// the stages' memory where they are large (all CTAs of the cluster have to be done with their products then).
+// Shared memory of a CTA: stages, barriers, the tokens' scales and zero points.  The CTA's own partial sums take the
+// stages' place once its products are formed; those of the others land behind everything else where they are small, else
+// behind its own (no CTA of the cluster may have products to form any more then).
 template <int NT> struct StreamSmem {
   static constexpr int kStage = kWeightBytes + NT * kBlockK;
   static constexpr int kParts = (NT + 7) * kRows * 4;
-  static constexpr bool kOwnParts = NT <= 32;
+  static constexpr bool kLandApart = NT <= 32;
+  // stages that the partial sums need
+  static constexpr int kLeast = ((kLandApart ? 1 : 2) * kParts + kStage - 1) / kStage;
   __host__ __device__ static int bars(int stages) { return stages * kStage; }
-  __host__ __device__ static int scales(int stages) { return bars(stages) + (8 * (2 * stages + 1) + 8 + 15) / 16 * 16; }
-  __host__ __device__ static int parts(int stages) { return kOwnParts ? scales(stages) + NT * 8 : 0; }
+  __host__ __device__ static int scales(int stages) { return bars(stages) + (8 * (2 * stages + 2) + 8 + 15) / 16 * 16; }
+  __host__ __device__ static int landing(int stages) { return kLandApart ? scales(stages) + NT * 8 : kParts; }
   __host__ __device__ static int bytes(int stages, bool split) {
-    return 1024 + scales(stages) + NT * 8 + (kOwnParts && split ? kParts : 0);
+    return 1024 + scales(stages) + NT * 8 + (kLandApart && split ? kParts : 0);
   }
 };
 
@@ -165,19 +187,22 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
   const uint32_t bar0 = base + Smem::bars(stages);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen + Smem::bars(stages) + 8 * (2 * stages + 1));
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen + Smem::bars(stages) + 8 * (2 * stages + 2));
   float* s_scale = reinterpret_cast<float*>(gen + Smem::scales(stages));
   int* s_zero = reinterpret_cast<int*>(s_scale + NT);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
   auto empty_bar = [&](int s) { return bar0 + 8u * (stages + s); };
-  const uint32_t acc_bar = bar0 + 8u * (2 * stages);
+  const uint32_t acc_bar = bar0 + 8u * (2 * stages), land_bar = acc_bar + 8u;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = blockIdx.x % splits;
   const int n0 = (int)(blockIdx.x / splits) * kRows, m0 = (int)blockIdx.y * NT;
   const int blocks = (g.K + kBlockK - 1) / kBlockK;
   const int kb0 = (int)((int64_t)blocks * rank / splits), kb1 = (int)((int64_t)blocks * (rank + 1) / splits);
   const int count = kb1 - kb0;                             // at least 1: splits <= blocks
+  const int tokens = min(NT, g.M - m0);
+  // with splits: tokens [first, first + mine) of the tile are this CTA's to finish
+  const int run = (tokens + splits - 1) / splits, first = rank * run, mine = max(0, min(run, tokens - first));
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) {
@@ -185,8 +210,10 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
       mbar_init(empty_bar(s), 1);
     }
     mbar_init(acc_bar, 1);
+    mbar_init(land_bar, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    if (splits > 1 && mine > 0) mbar_expect_tx(land_bar, (uint32_t)((splits - 1) * mine * kRows * 4));
     // the weights do not depend on the kernel before this one
     for (int i = 0; i < stages && i < count; ++i) {
       mbar_expect_tx(full_bar(i), kStage);
@@ -204,11 +231,11 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
   tcgen05_fence_after();
   const uint32_t tmem = *tmem_slot;
   if (splits > 1) cluster_arrive();                        // waited for before anything is sent to another CTA
-  const int tokens = min(NT, g.M - m0);
-  const int c = warp * 32 + lane, n = n0 + c;
+  const int group = warp >> 2;                             // of the two that share a channel
+  const int c = (warp & 3) * 32 + lane, n = n0 + c;
   const Channel ch = load_channel<T>(g, n);                // weights' side: nothing the kernel before this one writes
   grid_dependency_wait();
-  for (int t = threadIdx.x - 64; t >= 0 && t < NT; t += 64) {
+  for (int t = (int)threadIdx.x - 64; t >= 0 && t < NT; t += kStreamThreads - 64) {
     s_scale[t] = t < tokens ? g.a_s[m0 + t] : 0.f;
     s_zero[t] = t < tokens && g.a_z ? g.a_z[m0 + t] : 0;
   }
@@ -231,22 +258,26 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      int s = 0;
-      uint32_t ph = 0;
-      for (int i = 0; i < count; ++i) {
-        if (!mbar_wait(full_bar(s), ph, abort_flag)) break;
-        tcgen05_fence_after();
-        const uint32_t sw = base + s * kStage, sx = sw + kWeightBytes;
+    // The whole warp walks the stages and one lane issues, so that descriptors are formed in uniform registers; in a loop
+    // of one lane alone they are moved there for every MMA, and the issue bound the kernel (64 x 128 tiles, 86 blocks: 0.28
+    // us a block and 28.4 us in all; 0.20 and 22.4 this way; the pairs below gained 8 %).
+    int s = 0;
+    uint32_t ph = 0;
+    const uint64_t dw0 = make_desc_mn_sw128(base, 16, 1024), dx0 = make_desc_mn_sw128(base + kWeightBytes, 16, 1024);
+    for (int i = 0; i < count; ++i) {
+      if (!mbar_wait(full_bar(s), ph, abort_flag)) break;
+      tcgen05_fence_after();
+      const uint64_t at = (uint64_t)(s * (kStage >> 4));
+      if (elect_one()) {
 #pragma unroll
         for (int j = 0; j < kBlockK / 32; ++j)
-          umma_i8(tmem, make_desc_mn_sw128(sw + j * 32, 16, 1024), make_desc_mn_sw128(sx + j * 32, 16, 1024),
-                  idesc_i8(kRows, NT), (i | j) ? 1u : 0u);
+          umma_i8(tmem, dw0 + at + j * 2, dx0 + at + j * 2, idesc_i8(kRows, NT), (i | j) ? 1u : 0u);
         umma_commit(empty_bar(s));
-        if (++s == stages) s = 0, ph ^= 1u;
       }
-      umma_commit(acc_bar);                                // arrives once the MMAs issued so far have retired
+      __syncwarp();
+      if (++s == stages) s = 0, ph ^= 1u;
     }
+    if (elect_one()) umma_commit(acc_bar);                 // arrives once the MMAs issued so far have retired
   }
   __syncwarp();
   // the accumulator (or, after an expired wait, the retirement of what was issued)
@@ -266,57 +297,78 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
     __syncthreads();
   }
 
+  // Two warps to a lane quarter: they take chunks of tokens in turn (one warp a scheduler leaves it waiting for its own
+  // results; 33 clocks a token).
   T* out = static_cast<T*>(g.c) + (int64_t)m0 * g.N + n;
-  const uint32_t taddr = tmem + ((uint32_t)(warp * 32) << 16);
-  constexpr int kChunk = NT < 32 ? 16 : 32;
-  auto accumulators = [&](int t0, uint32_t (&v)[kChunk]) {
-    if constexpr (kChunk == 16) {
-      tmem_ld16(taddr + t0, v);
-    } else {
-      tmem_ld32_nowait(taddr + t0, v);
-      tmem_wait_ld();
-    }
-  };
+  const uint32_t taddr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+  constexpr int kChunk = NT < 32 ? 8 : 16;
   if (splits == 1) {
 #pragma unroll 1
-    for (int t0 = 0; t0 < tokens; t0 += kChunk) {
+    for (int t0 = group * kChunk; t0 < tokens; t0 += 2 * kChunk) {
       uint32_t v[kChunk];
-      accumulators(t0, v);
+      tmem_ld<kChunk>(taddr + t0, v);
       finish_tokens<T, kChunk>(v, s_scale + t0, s_zero + t0, g.a_z != nullptr, ch, out + (int64_t)t0 * g.N, g.N, tokens - t0,
                                !ok);
     }
   } else {
-    // part [t / splits][rank][channel] of token t's owner
-    const uint32_t parts = base + Smem::parts(stages);
+    uint32_t* part = reinterpret_cast<uint32_t*>(gen);     // [token][channel]
+#pragma unroll 1
+    for (int t0 = group * kChunk; t0 < tokens; t0 += 2 * kChunk) {
+      uint32_t v[kChunk];
+      tmem_ld<kChunk>(taddr + t0, v);
+#pragma unroll
+      for (int i = 0; i < kChunk; ++i) part[(t0 + i) * kRows + c] = v[i];
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");         // the bulk copies read what was just written
+    __syncthreads();
     cluster_wait();                                        // every CTA of the cluster runs
-    if (!Smem::kOwnParts) {
+    if (!Smem::kLandApart) {
       cluster_arrive();                                    // and has no products to form any more
       cluster_wait();
     }
-    if (!ok && threadIdx.x < (unsigned)splits)             // tell every CTA that a part is missing
-      st_cluster(in_cta(smem_u32(const_cast<int*>(abort_flag)), threadIdx.x), 1u);
+    // lane r sends to CTA r; a CTA whose sums are not whole sends nothing, and the owners' waits expire
+    if (warp == 0 && lane < splits && lane != rank && ok) {
+      const int from = lane * run, many = min(run, tokens - from);
+      if (many > 0)
+        copy_to_cta(in_cta(base + Smem::landing(stages) + (uint32_t)((rank < lane ? rank : rank - 1) * many * kRows * 4), lane),
+                    base + (uint32_t)(from * kRows * 4), (uint32_t)(many * kRows * 4), in_cta(land_bar, lane));
+    }
+    __syncwarp();
+    if (mine > 0) ok = mbar_wait(land_bar, 0, abort_flag) && ok;
+    __syncwarp();
+    cluster_arrive();                                      // what was sent here is here
+    const uint32_t* own = part + first * kRows + c;
+    const uint32_t* landed = reinterpret_cast<const uint32_t*>(gen + Smem::landing(stages)) + c;
+    const int step = mine * kRows;
 #pragma unroll 1
-    for (int t0 = 0; t0 < tokens; t0 += kChunk) {
-      uint32_t v[kChunk];
-      accumulators(t0, v);
-      int owner = t0 % splits, slot = t0 / splits * splits + rank;
+    for (int t0 = group * 4; t0 < mine; t0 += 8) {
+      // Four tokens at a time, formed before the first store (see finish_tokens).  Behind the run's last token the sums
+      // are of whatever lies there, inside shared memory, and are not stored.
+      uint32_t sum[4];
 #pragma unroll
-      for (int i = 0; i < kChunk; ++i) {
-        if (t0 + i < tokens) st_cluster(in_cta(parts + (uint32_t)(slot * kRows + c) * 4u, owner), v[i]);
-        if (++owner == splits) owner = 0, slot += splits;
+      for (int i = 0; i < 4; ++i) sum[i] = own[(t0 + i) * kRows];
+      const uint32_t* p = landed + t0 * kRows;
+#pragma unroll 3
+      for (int r = 1; r < splits; ++r, p += step) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] += p[i * kRows];
+      }
+      float y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = min(first + t0 + i, NT - 1);
+        y[i] = finish((int)sum[i], s_scale[t], s_zero[t], ch.b_s, ch.b_sum, ch.bias);
+        if (!ok) y[i] = __int_as_float(0x7fffffff);
+      }
+      if (ch.ok) {
+        T* to = out + (int64_t)(first + t0) * g.N;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (t0 + i < mine) to[i * (int64_t)g.N] = Elem<T>::from_f(y[i]);
       }
     }
-    cluster_arrive();
-    cluster_wait();
-    ok = *abort_flag == 0;
-    const uint32_t* mine = reinterpret_cast<const uint32_t*>(gen + Smem::parts(stages)) + c;
-#pragma unroll 4
-    for (int t = rank, k = 0; t < tokens; t += splits, k += splits) {
-      uint32_t sum = 0;
-      for (int r = 0; r < splits; ++r) sum += mine[(k + r) * kRows];
-      const float y = finish((int)sum, s_scale[t], s_zero[t], ch.b_s, ch.b_sum, ch.bias);
-      if (ch.ok) out[(int64_t)t * g.N] = Elem<T>::from_f(ok ? y : __int_as_float(0x7fffffff));
-    }
+    __syncwarp();
+    cluster_wait();                                        // nobody leaves while its sums are on their way
   }
   tcgen05_fence_before();
   __syncthreads();
@@ -331,7 +383,8 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
 // 128-deep k block is 16 KB of weights and 16 KB of tokens per SM, i.e. 128 products per byte that crosses from L2,
 // against 64 for the one-SM tile above.  Persistent, one pair per two SMs; six stages; two accumulators of 256 columns, so
 // that eight warps finish one tile while the tensor cores work on the next.  Warp 0 of each CTA copies its own operands and
-// signals the leader's barrier, warp 1 of the leader issues the MMAs for both, warps 2 - 9 finish.
+// signals the leader's barrier, warp 1 of the leader issues the MMAs for both, the others finish 128 tokens of 32
+// channels each (sixteen warps with 64 each were 3 % slower: they take issue slots and power from the product).
 // The kernel asks for all of an SM's shared memory: no other CTA that needs tensor memory can then lie beside it and
 // wait for its columns while it waits for theirs.
 constexpr int kPairRows = 256, kPairTokens = 256, kPairStages = 6, kPairBufs = 2;
@@ -427,25 +480,29 @@ pair_kernel(const __grid_constant__ Maps maps, Int8Args g, PairTiles pt) {
       int s = 0;
       uint32_t ph = 1;
       bool ok = true;
+      const uint32_t full0 = in_cta(full_bar(0), 0);
       for (int t = pair; ok && t < tiles; t += pairs) {
         int n0, m0;
         origin(t, n0, m0);
+        n0 += (int)rank * 128, m0 += (int)rank * 128;
         for (int kb = 0; kb < blocks; ++kb) {
           if (!mbar_wait(empty_bar(s), ph, abort_flag)) { ok = false; break; }
+          const uint32_t sa = base + s * kPairStageBytes;
           if (rank == 0) mbar_expect_tx(full_bar(s), 2 * kPairStageBytes);
-          const uint32_t bar = in_cta(full_bar(s), 0), sa = base + s * kPairStageBytes;
-          tma_load_pair(sa, &maps.w, kb * kBlockK, n0 + (int)rank * 128, bar);
-          tma_load_pair(sa + kHalfBytes, &maps.x, kb * kBlockK, m0 + (int)rank * 128, bar);
+          tma_load_pair(sa, &maps.w, kb * kBlockK, n0, full0 + 8u * s);
+          tma_load_pair(sa + kHalfBytes, &maps.x, kb * kBlockK, m0, full0 + 8u * s);
           ++issued;
           if (++s == kPairStages) s = 0, ph ^= 1u;
         }
       }
     }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
+      // the whole warp walks, one lane issues (see stream_kernel)
       int s = 0, buf = 0;
       uint32_t ph = 0, aph = 1;
       bool ok = true;
+      const uint64_t dw0 = make_desc_mn_sw128(base, 16, 1024), dx0 = make_desc_mn_sw128(base + kHalfBytes, 16, 1024);
       for (int t = pair; ok && t < tiles; t += pairs) {
         if (!mbar_wait(acc_empty(buf), aph, abort_flag)) break;
         tcgen05_fence_after();
@@ -453,20 +510,23 @@ pair_kernel(const __grid_constant__ Maps maps, Int8Args g, PairTiles pt) {
         for (int kb = 0; kb < blocks; ++kb) {
           if (!mbar_wait(full_bar(s), ph, abort_flag)) { ok = false; break; }
           tcgen05_fence_after();
-          const uint32_t sw = base + s * kPairStageBytes, sx = sw + kHalfBytes;
+          const uint64_t at = (uint64_t)(s * (kPairStageBytes >> 4));
+          if (elect_one()) {
 #pragma unroll
-          for (int j = 0; j < kBlockK / 32; ++j)
-            umma_i8_pair(acc, make_desc_mn_sw128(sw + j * 32, 16, 1024), make_desc_mn_sw128(sx + j * 32, 16, 1024),
-                         idesc_i8(kPairRows, kPairTokens), (kb | j) ? 1u : 0u);
-          umma_commit_pair(empty_bar(s));
+            for (int j = 0; j < kBlockK / 32; ++j)
+              umma_i8_pair(acc, dw0 + at + j * 2, dx0 + at + j * 2, idesc_i8(kPairRows, kPairTokens), (kb | j) ? 1u : 0u);
+            umma_commit_pair(empty_bar(s));
+          }
+          __syncwarp();
           if (++s == kPairStages) s = 0, ph ^= 1u;
         }
-        umma_commit_pair(acc_full(buf));
+        if (elect_one()) umma_commit_pair(acc_full(buf));
+        __syncwarp();
         if (++buf == kPairBufs) buf = 0, aph ^= 1u;
       }
       if (*abort_flag) {
         // the MMAs already issued retire before the tensor memory is freed
-        umma_commit_pair(retired);
+        if (elect_one()) umma_commit_pair(retired);
         for (uint32_t it = 0; it < kSpinLimit && !mbar_test(retired, 0); ++it) __nanosleep(50);
       }
     }
@@ -543,20 +603,64 @@ int encode_codes(CUtensorMap* m, const int8_t* p, int64_t k, int64_t rows, int64
   return LC_OK;
 }
 
+// ---- which tile, which split ---------------------------------------------------------------------------------------
+// The product of every choice is the same to the bit, so the choice is the one whose estimated time is least.  Measured
+// (us): a CTA of the first kernel takes `base` for its launch, its first copies and its finishing, and c1 for a k block
+// when it has an SM to itself, c2 when two share one; each further round of CTAs costs their finishing again; splitting K
+// adds the exchange of partial sums, and clusters do not fill every SM.  A wave of pairs takes 0.30 a block, or what its
+// finishing takes.  No choice is faster than the weights arrive from HBM.  Against the best of all choices, over M 1 -
+// 2600 and N, K 64 - 11008, the one taken was within 5 % in most cases and within 20 % in all but a few of under 8 us
+// (e.g. 256 x 4096 x 4096: 11.9 us on 64-token tiles, 16.2 on pairs; 1024 x 11008 x 4096: 36 on pairs, 50 on 128-token
+// tiles; 1 x 4096 x 11008: 12.3 with K split six ways, 21.2 without).
+struct Choice {
+  int tokens;      // of a tile: 16, 32, 64, 128; 256 for the pair kernel
+  int splits;
+};
+// CTAs that run at once, one to an SM; clusters leave SMs of a GPC over
+constexpr int ctas_at_once(int splits) { return splits > 1 ? kNumSMsB200 - 16 : kNumSMsB200; }
+
+Choice choose(int64_t M, int64_t N, int64_t K) {
+  constexpr int kNT[4] = {16, 32, 64, 128};
+  constexpr float kBase[4] = {3.3f, 3.5f, 3.9f, 4.7f}, kC1[4] = {0.225f, 0.225f, 0.23f, 0.235f},
+                  kC2[4] = {0.32f, 0.31f, 0.33f, 0.39f}, kExchange[4] = {1.9f, 2.0f, 2.9f, 4.0f},
+                  kRound[4] = {2.0f, 2.5f, 3.0f, 4.0f};
+  constexpr int kSplits[6] = {1, 2, 3, 4, 6, 8};
+  const int64_t blocks = (K + kBlockK - 1) / kBlockK, n_tiles = (N + kRows - 1) / kRows;
+  const float arrive = 4.5f + (float)(N * K) / 6.0e6f;
+  Choice best{256, 1};
+  const int64_t pair_tiles = ((N + 255) / 256) * ((M + 255) / 256), halves = kNumSMsB200 / 2;
+  const float wave = (float)blocks * 0.30f;
+  float least = 6.5f + (float)((pair_tiles + halves - 1) / halves) * (wave > 3.3f ? wave : 3.3f);
+  if (M <= 128) least = 1e30f;
+  for (int i = 0; i < 4; ++i) {
+    if (i > 0 && kNT[i - 1] >= M) break;                   // half of the tile's tokens would not exist
+    const int64_t tiles = n_tiles * ((M + kNT[i] - 1) / kNT[i]);
+    for (int sp : kSplits) {
+      const int64_t ctas = tiles * sp, count = (blocks + sp - 1) / sp;
+      if (sp > 1 && (sp > blocks || ctas > (kNT[i] == 128 ? 1 : 2) * ctas_at_once(sp))) break;
+      const int64_t rounds = (ctas + 2 * kNumSMsB200 - 1) / (2 * kNumSMsB200);
+      float t = kBase[i] + (ctas <= ctas_at_once(sp) ? (float)count * kC1[i] : (float)(rounds * count) * kC2[i]) +
+                (float)(rounds - 1) * kRound[i] + (sp > 1 ? kExchange[i] : 0.f);
+      if (t < arrive && N * K > (4 << 20)) t = arrive + (sp > 1 ? 0.3f * kExchange[i] : 0.f) + 1e-3f * t;
+      if (t < least) {
+        least = t;
+        best = Choice{kNT[i], sp};
+      }
+    }
+  }
+  return best;
+}
+
 template <typename T, int NT>
-int launch_stream(const Int8Args& g, bool dependent, cudaStream_t st) {
-  constexpr int kStage = kWeightBytes + NT * kBlockK;
+int launch_stream(const Int8Args& g, int splits, bool dependent, cudaStream_t st) {
   const int n_tiles = (g.N + kRows - 1) / kRows, m_tiles = (g.M + NT - 1) / NT;
   if (m_tiles > 65535) return LC_ERR_SHAPE;
-  const int blocks = (g.K + kBlockK - 1) / kBlockK, tiles = n_tiles * m_tiles;
-  int splits = 1;
-  while (splits < 8 && tiles * splits * 2 <= kNumSMsB200 * 2 && splits * 2 <= blocks) splits *= 2;
-  const int per_sm = tiles * splits > kNumSMsB200 ? 2 : 1;
+  const int blocks = (g.K + kBlockK - 1) / kBlockK;
+  const int per_sm = (int64_t)n_tiles * m_tiles * splits > ctas_at_once(splits) ? 2 : 1;
   using Smem = StreamSmem<NT>;
   int stages = (blocks + splits - 1) / splits;             // more than a CTA's blocks are of no use
   while (stages > 1 && Smem::bytes(stages, splits > 1) > kSmemMost / per_sm - 1024) --stages;
-  if (splits > 1 && !Smem::kOwnParts)
-    while (stages * kStage < Smem::kParts) ++stages;       // the partial sums take the stages' place
+  if (splits > 1 && stages < Smem::kLeast) stages = Smem::kLeast;
   const int smem = Smem::bytes(stages, splits > 1);
   Maps maps;
   int rc;
@@ -610,11 +714,14 @@ int launch_pair(const Int8Args& g, bool dependent, cudaStream_t st) {
 
 template <typename T>
 int launch(const Int8Args& g, bool dependent, cudaStream_t st) {
-  if (g.M > 128 && (int64_t)((g.M + 255) / 256) * ((g.N + 255) / 256) >= 74) return launch_pair<T>(g, dependent, st);
-  if (g.M <= 16) return launch_stream<T, 16>(g, dependent, st);
-  if (g.M <= 32) return launch_stream<T, 32>(g, dependent, st);
-  if (g.M <= 64) return launch_stream<T, 64>(g, dependent, st);
-  return launch_stream<T, 128>(g, dependent, st);
+  const Choice c = choose(g.M, g.N, g.K);
+  switch (c.tokens) {
+    case 16: return launch_stream<T, 16>(g, c.splits, dependent, st);
+    case 32: return launch_stream<T, 32>(g, c.splits, dependent, st);
+    case 64: return launch_stream<T, 64>(g, c.splits, dependent, st);
+    case 128: return launch_stream<T, 128>(g, c.splits, dependent, st);
+    default: return launch_pair<T>(g, dependent, st);
+  }
 }
 
 // sizes, pitches and alignment of the product; the same rules for both entry points
