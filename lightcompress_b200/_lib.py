@@ -84,7 +84,7 @@ SIGNATURES = {
     'lc_int8_act_quant': [_p, _i, _i64, _i64, _i64, _p, _i64, _p, _p, _p],
     'lc_int8_gated_act_quant': [_p, _p, _i, _i64, _i64, _i64, _i64, _i, _p, _i64, _p, _p, _p],
     'lc_int8_gemm': [_p, _i64, _p, _p, _p, _i64, _p, _p, _p, _i64, _i64, _i64, _p, _i, _p, _p],
-    'lc_int8_linear_scratch': [_i64, _i64],
+    'lc_int8_linear_scratch': [_i64, _i64, _i64],
     'lc_int8_linear': [_p, _i, _i64, _p, _i64, _p, _p, _p, _i64, _i64, _i64, _i, _p, _p, _i64, _p, _p],
     'lc_residual_norm': [_p, _p, _p, _p, _i64, _p, _i, _i64, _i64, _i64, _i64, _f, _f, _f, _p, _p, _p, _i64, _p, _p, _p],
     'lc_rotary_embed': [_p, _p, _i, _i64, _i64, _i64, _p, _p, _i, _i64, _i64, _i64, _p, _i64, _p, _i, _i64, _i64, _i, _i,

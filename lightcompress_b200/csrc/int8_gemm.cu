@@ -7,6 +7,7 @@
 // how the contraction is split; the zero point enters as -a_z[m] * b_sum[n] in the same 32-bit arithmetic (the
 // bounds on K keep the final sum inside 32 bits; what wraps on the way wraps back).  After that there are two
 // fp32 multiplications and an addition, in this order, and one rounding to the output type.
+#include "row_quant.cuh"
 #include "umma_common.cuh"
 
 namespace lc {
@@ -19,6 +20,9 @@ namespace {
 using namespace umma;
 
 struct Int8Args {
+  const void* x;           // activations that the kernel quantises itself (then a, a_s and a_z are not read)
+  int64_t ldx;
+  int sym, wide;           // wide: x's rows are 16-byte aligned
   const int8_t* a;
   const int8_t* b;
   const float* a_s;
@@ -50,7 +54,7 @@ __device__ __forceinline__ Channel load_channel(const Int8Args& g, int n) {
   if (c.ok) {
     c.b_s = g.b_s[n];
     if (g.bias) c.bias = Elem<T>::to_f(static_cast<const T*>(g.bias)[n]);
-    if (g.a_z) c.b_sum = g.b_sum[n];
+    if (g.b_sum) c.b_sum = g.b_sum[n];
   }
   return c;
 }
@@ -160,35 +164,115 @@ struct Maps {
   CUtensorMap w, x;
 };
 
+// A few tokens are quantised by the product itself (kQuant): every CTA reads all of x for the rows' ranges and lays the
+// codes of its own part of K out as the copies would (8-row, 128-byte swizzled atoms).  That is M * K values from L2 per CTA
+// against a launch and a scratch buffer less, while the CTA's first weights are on their way.
+//
 // Shared memory of a CTA: stages, barriers, the tokens' scales and zero points.  The CTA's own partial sums take the
 // stages' place once its products are formed; those of the others land behind everything else where they are small, else
 // behind its own (no CTA of the cluster may have products to form any more then).
-template <int NT> struct StreamSmem {
-  static constexpr int kStage = kWeightBytes + NT * kBlockK;
+constexpr int kRangeBytes = 2 * 8 * 8 * 4;                  // [min / max][part of a row][row]
+template <int NT, bool kQuant> struct StreamSmem {
+  static constexpr int kStage = kWeightBytes + (kQuant ? 0 : NT * kBlockK);
   static constexpr int kParts = (NT + 7) * kRows * 4;
   static constexpr bool kLandApart = NT <= 32;
   // stages that the partial sums need
   static constexpr int kLeast = ((kLandApart ? 1 : 2) * kParts + kStage - 1) / kStage;
-  __host__ __device__ static int bars(int stages) { return stages * kStage; }
-  __host__ __device__ static int scales(int stages) { return bars(stages) + (8 * (2 * stages + 2) + 8 + 15) / 16 * 16; }
-  __host__ __device__ static int landing(int stages) { return kLandApart ? scales(stages) + NT * 8 : kParts; }
-  __host__ __device__ static int bytes(int stages, bool split) {
-    return 1024 + scales(stages) + NT * 8 + (kLandApart && split ? kParts : 0);
+  // codes: k blocks of codes that the CTA lays out itself
+  __host__ __device__ static int codes(int stages) { return stages * kStage; }
+  __host__ __device__ static int bars(int stages, int count) { return codes(stages) + (kQuant ? count * NT * kBlockK : 0); }
+  __host__ __device__ static int scales(int stages, int count) {
+    return bars(stages, count) + (8 * (2 * stages + 2) + 8 + 15) / 16 * 16;
+  }
+  __host__ __device__ static int ranges(int stages, int count) { return scales(stages, count) + NT * 8; }
+  __host__ __device__ static int landing(int stages, int count) {
+    return kLandApart ? ranges(stages, count) + (kQuant ? kRangeBytes : 0) : kParts;
+  }
+  __host__ __device__ static int bytes(int stages, int count, bool split) {
+    return 1024 + ranges(stages, count) + (kQuant ? kRangeBytes : 0) + (kLandApart && split ? kParts : 0);
   }
 };
 
-template <typename T, int NT>
+// 16 neighbouring values of a row from k on; zeros behind the row's end
+template <typename T>
+__device__ __forceinline__ void load_values(const T* row, int k, int K, bool wide, float (&v)[16]) {
+  constexpr int N = Elem<T>::kPerVec;
+  if (wide && k + 16 <= K) {
+#pragma unroll
+    for (int i = 0; i < 16 / N; ++i) {
+      float f[N];
+      unpack16<T>(*reinterpret_cast<const uint4*>(row + k + i * N), f);
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[i * N + j] = f[j];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = k + i < K ? Elem<T>::to_f(row[k + i]) : 0.f;
+  }
+}
+
+// All of the CTA's threads: the tokens' scales and zero points, and the codes of k blocks [kb0, kb0 + count).
+template <typename T>
+__device__ __forceinline__ void quantise_tokens(const Int8Args& g, int kb0, int count, uint8_t* codes, float* s_scale,
+                                                int* s_zero, float* range) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rows = g.M <= 1 ? 1 : g.M <= 2 ? 2 : g.M <= 4 ? 4 : 8, parts = 8 / rows;
+  const int chunks = (g.K + 15) / 16;
+  if (const int r = warp % rows; r < g.M) {
+    const T* row = static_cast<const T*>(g.x) + r * g.ldx;
+    float mn = 0.f, mx = 0.f;
+    for (int c = warp / rows * 32 + lane; c < chunks; c += parts * 32) {
+      float v[16];
+      load_values<T>(row, c * 16, g.K, g.wide, v);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mn = nan_min(mn, v[i]), mx = nan_max(mx, v[i]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      mx = nan_max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      mn = nan_min(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+    }
+    if (lane == 0) range[warp / rows * 8 + r] = mn, range[64 + warp / rows * 8 + r] = mx;
+  }
+  __syncthreads();
+  auto of_row = [&](int r) {
+    float mn = range[r], mx = range[64 + r];
+    for (int p = 1; p < parts; ++p) mn = nan_min(mn, range[p * 8 + r]), mx = nan_max(mx, range[64 + p * 8 + r]);
+    return row_quant_of(mn, mx, g.sym);
+  };
+  if ((int)threadIdx.x < g.M) {
+    const RowQuant q = of_row(threadIdx.x);
+    s_scale[threadIdx.x] = q.s;
+    s_zero[threadIdx.x] = q.z;
+  }
+  for (int i = threadIdx.x; i < g.M * count * 8; i += kStreamThreads) {
+    const int r = i / (count * 8), at = i - r * (count * 8), kb = at >> 3, c = at & 7;
+    const RowQuant q = of_row(r);
+    float v[16];
+    load_values<T>(static_cast<const T*>(g.x) + r * g.ldx, (kb0 + kb) * kBlockK + c * 16, g.K, g.wide, v);
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float u[4] = {v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]};
+      store_row_codes<4>(reinterpret_cast<int8_t*>(w + j), u, q, g.sym);
+    }
+    *reinterpret_cast<uint4*>(codes + kb * (16 * kBlockK) + r * kBlockK + ((c ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+template <typename T, int NT, bool kQuant>
 __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_constant__ Maps maps, Int8Args g, int splits,
                                                                 int stages) {
-  using Smem = StreamSmem<NT>;
+  using Smem = StreamSmem<NT, kQuant>;
   constexpr int kStage = Smem::kStage;
   constexpr int kCols = NT < 32 ? 32 : NT;                 // tensor memory is allocated in powers of two from 32 columns
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* gen = smem_raw + (base - smem_u32(smem_raw));
-  const uint32_t bar0 = base + Smem::bars(stages);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen + Smem::bars(stages) + 8 * (2 * stages + 2));
-  float* s_scale = reinterpret_cast<float*>(gen + Smem::scales(stages));
+  const int blocks = (g.K + kBlockK - 1) / kBlockK, most = (blocks + splits - 1) / splits;
+  const uint32_t bar0 = base + Smem::bars(stages, most);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(gen + Smem::bars(stages, most) + 8 * (2 * stages + 2));
+  float* s_scale = reinterpret_cast<float*>(gen + Smem::scales(stages, most));
   int* s_zero = reinterpret_cast<int*>(s_scale + NT);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
@@ -197,7 +281,6 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = blockIdx.x % splits;
   const int n0 = (int)(blockIdx.x / splits) * kRows, m0 = (int)blockIdx.y * NT;
-  const int blocks = (g.K + kBlockK - 1) / kBlockK;
   const int kb0 = (int)((int64_t)blocks * rank / splits), kb1 = (int)((int64_t)blocks * (rank + 1) / splits);
   const int count = kb1 - kb0;                             // at least 1: splits <= blocks
   const int tokens = min(NT, g.M - m0);
@@ -234,17 +317,26 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
   const int group = warp >> 2;                             // of the two that share a channel
   const int c = (warp & 3) * 32 + lane, n = n0 + c;
   const Channel ch = load_channel<T>(g, n);                // weights' side: nothing the kernel before this one writes
-  grid_dependency_wait();
-  for (int t = (int)threadIdx.x - 64; t >= 0 && t < NT; t += kStreamThreads - 64) {
-    s_scale[t] = t < tokens ? g.a_s[m0 + t] : 0.f;
-    s_zero[t] = t < tokens && g.a_z ? g.a_z[m0 + t] : 0;
+  const bool zeros = kQuant ? !g.sym : g.a_z != nullptr;
+  if constexpr (kQuant) {
+    quantise_tokens<T>(g, kb0, count, gen + Smem::codes(stages), s_scale, s_zero,
+                       reinterpret_cast<float*>(gen + Smem::ranges(stages, most)));
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");         // the MMAs read what was just written
+    __syncthreads();
+  } else {
+    grid_dependency_wait();
+    for (int t = (int)threadIdx.x - 64; t >= 0 && t < NT; t += kStreamThreads - 64) {
+      s_scale[t] = t < tokens ? g.a_s[m0 + t] : 0.f;
+      s_zero[t] = t < tokens && g.a_z ? g.a_z[m0 + t] : 0;
+    }
   }
 
   int issued = 0;                                          // k blocks requested, known to thread 0
   if (warp == 0) {
     if (lane == 0) {
-      for (int i = 0; i < stages && i < count; ++i)
-        tma_load_2d(base + i * kStage + kWeightBytes, &maps.x, (kb0 + i) * kBlockK, m0, full_bar(i));
+      if (!kQuant)
+        for (int i = 0; i < stages && i < count; ++i)
+          tma_load_2d(base + i * kStage + kWeightBytes, &maps.x, (kb0 + i) * kBlockK, m0, full_bar(i));
       int s = 0;
       uint32_t ph = 0;
       issued = min(stages, count);
@@ -252,7 +344,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
         if (!mbar_wait(empty_bar(s), ph, abort_flag)) break;
         mbar_expect_tx(full_bar(s), kStage);
         tma_load_2d(base + s * kStage, &maps.w, (kb0 + i) * kBlockK, n0, full_bar(s));
-        tma_load_2d(base + s * kStage + kWeightBytes, &maps.x, (kb0 + i) * kBlockK, m0, full_bar(s));
+        if (!kQuant) tma_load_2d(base + s * kStage + kWeightBytes, &maps.x, (kb0 + i) * kBlockK, m0, full_bar(s));
         issued = i + 1;
         if (++s == stages) s = 0, ph ^= 1u;
       }
@@ -263,15 +355,16 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
     // us a block and 28.4 us in all; 0.20 and 22.4 this way; the pairs below gained 8 %).
     int s = 0;
     uint32_t ph = 0;
-    const uint64_t dw0 = make_desc_mn_sw128(base, 16, 1024), dx0 = make_desc_mn_sw128(base + kWeightBytes, 16, 1024);
+    const uint64_t dw0 = make_desc_mn_sw128(base, 16, 1024);
+    const uint64_t dx0 = make_desc_mn_sw128(base + (kQuant ? Smem::codes(stages) : kWeightBytes), 16, 1024);
     for (int i = 0; i < count; ++i) {
       if (!mbar_wait(full_bar(s), ph, abort_flag)) break;
       tcgen05_fence_after();
-      const uint64_t at = (uint64_t)(s * (kStage >> 4));
+      const uint64_t at = (uint64_t)(s * (kStage >> 4)), xat = kQuant ? (uint64_t)(i * (NT * kBlockK >> 4)) : at;
       if (elect_one()) {
 #pragma unroll
         for (int j = 0; j < kBlockK / 32; ++j)
-          umma_i8(tmem, dw0 + at + j * 2, dx0 + at + j * 2, idesc_i8(kRows, NT), (i | j) ? 1u : 0u);
+          umma_i8(tmem, dw0 + at + j * 2, dx0 + xat + j * 2, idesc_i8(kRows, NT), (i | j) ? 1u : 0u);
         umma_commit(empty_bar(s));
       }
       __syncwarp();
@@ -307,7 +400,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
     for (int t0 = group * kChunk; t0 < tokens; t0 += 2 * kChunk) {
       uint32_t v[kChunk];
       tmem_ld<kChunk>(taddr + t0, v);
-      finish_tokens<T, kChunk>(v, s_scale + t0, s_zero + t0, g.a_z != nullptr, ch, out + (int64_t)t0 * g.N, g.N, tokens - t0,
+      finish_tokens<T, kChunk>(v, s_scale + t0, s_zero + t0, zeros, ch, out + (int64_t)t0 * g.N, g.N, tokens - t0,
                                !ok);
     }
   } else {
@@ -330,7 +423,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
     if (warp == 0 && lane < splits && lane != rank && ok) {
       const int from = lane * run, many = min(run, tokens - from);
       if (many > 0)
-        copy_to_cta(in_cta(base + Smem::landing(stages) + (uint32_t)((rank < lane ? rank : rank - 1) * many * kRows * 4), lane),
+        copy_to_cta(in_cta(base + Smem::landing(stages, most) + (uint32_t)((rank < lane ? rank : rank - 1) * many * kRows * 4), lane),
                     base + (uint32_t)(from * kRows * 4), (uint32_t)(many * kRows * 4), in_cta(land_bar, lane));
     }
     __syncwarp();
@@ -338,7 +431,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
     __syncwarp();
     cluster_arrive();                                      // what was sent here is here
     const uint32_t* own = part + first * kRows + c;
-    const uint32_t* landed = reinterpret_cast<const uint32_t*>(gen + Smem::landing(stages)) + c;
+    const uint32_t* landed = reinterpret_cast<const uint32_t*>(gen + Smem::landing(stages, most)) + c;
     const int step = mine * kRows;
 #pragma unroll 1
     for (int t0 = group * 4; t0 < mine; t0 += 8) {
@@ -641,7 +734,8 @@ Choice choose(int64_t M, int64_t N, int64_t K) {
       const int64_t rounds = (ctas + 2 * kNumSMsB200 - 1) / (2 * kNumSMsB200);
       float t = kBase[i] + (ctas <= ctas_at_once(sp) ? (float)count * kC1[i] : (float)(rounds * count) * kC2[i]) +
                 (float)(rounds - 1) * kRound[i] + (sp > 1 ? kExchange[i] : 0.f);
-      if (t < arrive && N * K > (4 << 20)) t = arrive + (sp > 1 ? 0.3f * kExchange[i] : 0.f) + 1e-3f * t;
+      const float floor = arrive + (sp > 1 ? 0.3f * kExchange[i] : 0.f);
+      if (t < floor && N * K > (4 << 20)) t = floor + 1e-3f * t;
       if (t < least) {
         least = t;
         best = Choice{kNT[i], sp};
@@ -651,23 +745,37 @@ Choice choose(int64_t M, int64_t N, int64_t K) {
   return best;
 }
 
-template <typename T, int NT>
+// Whether lc_int8_linear's product quantises the activations itself: one tile of 16 tokens, at most 32768 values for every
+// CTA to read, and codes of a CTA's part of K that leave room for the weights.
+bool quantises_itself(int64_t M, int64_t N, int64_t K) {
+  if (M > 8 || M * K > 32768) return false;
+  const Choice c = choose(M, N, K);
+  return c.tokens == 16 && (K + kBlockK - 1) / kBlockK <= (int64_t)32 * c.splits;
+}
+
+// What a kernel may ask for; the same for every launch, so that calls from two threads do not take it from one another.
+template <typename F>
+cudaError_t allow_smem(F* kernel) {
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost);
+}
+
+template <typename T, int NT, bool kQuant = false>
 int launch_stream(const Int8Args& g, int splits, bool dependent, cudaStream_t st) {
   const int n_tiles = (g.N + kRows - 1) / kRows, m_tiles = (g.M + NT - 1) / NT;
   if (m_tiles > 65535) return LC_ERR_SHAPE;
   const int blocks = (g.K + kBlockK - 1) / kBlockK;
   const int per_sm = (int64_t)n_tiles * m_tiles * splits > ctas_at_once(splits) ? 2 : 1;
-  using Smem = StreamSmem<NT>;
-  int stages = (blocks + splits - 1) / splits;             // more than a CTA's blocks are of no use
-  while (stages > 1 && Smem::bytes(stages, splits > 1) > kSmemMost / per_sm - 1024) --stages;
+  using Smem = StreamSmem<NT, kQuant>;
+  const int most = (blocks + splits - 1) / splits;         // a CTA's blocks: more stages than that are of no use
+  int stages = most;
+  while (stages > 1 && Smem::bytes(stages, most, splits > 1) > kSmemMost / per_sm - 1024) --stages;
   if (splits > 1 && stages < Smem::kLeast) stages = Smem::kLeast;
-  const int smem = Smem::bytes(stages, splits > 1);
+  const int smem = Smem::bytes(stages, most, splits > 1);
   Maps maps;
   int rc;
   if ((rc = encode_codes(&maps.w, g.b, g.K, g.N, g.ldb, kRows)) != LC_OK) return rc;
-  if ((rc = encode_codes(&maps.x, g.a, g.K, g.M, g.lda, NT)) != LC_OK) return rc;
-  // per-device attribute; setting it on every call keeps multi-device processes correct
-  LC_CHECK_CUDA(cudaFuncSetAttribute(stream_kernel<T, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  if (!kQuant && (rc = encode_codes(&maps.x, g.a, g.K, g.M, g.lda, NT)) != LC_OK) return rc;
+  LC_CHECK_CUDA(allow_smem(stream_kernel<T, NT, kQuant>));
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = splits, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
@@ -680,7 +788,7 @@ int launch_stream(const Int8Args& g, int splits, bool dependent, cudaStream_t st
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = dependent ? 2 : 1;
-  LC_CHECK_CUDA(cudaLaunchKernelEx(&cfg, stream_kernel<T, NT>, maps, g, splits, stages));
+  LC_CHECK_CUDA(cudaLaunchKernelEx(&cfg, stream_kernel<T, NT, kQuant>, maps, g, splits, stages));
   return LC_OK;
 }
 
@@ -697,7 +805,7 @@ int launch_pair(const Int8Args& g, bool dependent, cudaStream_t st) {
   const int64_t tiles = (int64_t)pt.n_tiles * pt.m_tiles;
   if (tiles > 0x3fffffff) return LC_ERR_SHAPE;
   const int pairs = (int)(tiles < kNumSMsB200 / 2 ? tiles : kNumSMsB200 / 2);
-  LC_CHECK_CUDA(cudaFuncSetAttribute(pair_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMost));
+  LC_CHECK_CUDA(allow_smem(pair_kernel<T>));
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
@@ -769,31 +877,45 @@ extern "C" LC_API int lc_int8_gemm(const int8_t* a, int64_t lda, const float* a_
   if (rc != LC_OK || M == 0 || N == 0) return rc;
   if (!a || !a_s || lda < K) return LC_ERR_ARG;
   if (!aligned16(a) || (lda & 15)) return LC_ERR_ALIGN;
-  return product(Int8Args{a, b, a_s, a_z, b_s, b_sum, bias, c, status, lda, ldb, (int)M, (int)N, (int)K}, out_dtype, false,
+  return product(Int8Args{nullptr, 0, 0, 0, a, b, a_s, a_z, b_s, b_sum, bias, c, status, lda, ldb, (int)M, (int)N, (int)K}, out_dtype, false,
                  reinterpret_cast<cudaStream_t>(stream));
 }
 
-extern "C" LC_API int64_t lc_int8_linear_scratch(int64_t M, int64_t K) {
-  if (M < 0 || K < 0) return 0;
-  return M * ((K + 15) / 16 * 16) + 8 * M;
+extern "C" LC_API int64_t lc_int8_linear_scratch(int64_t M, int64_t N, int64_t K) {
+  using namespace lc;
+  if (M <= 0 || N <= 0 || K <= 0 || quantises_itself(M, N, K)) return 0;
+  return M * ((K + 15) / 16 * 16 + 8);
 }
 
 extern "C" LC_API int lc_int8_linear(const void* x, int dtype, int64_t ldx, const int8_t* b, int64_t ldb, const float* b_s,
                                      const int32_t* b_sum, const void* bias, int64_t M, int64_t N, int64_t K, int sym,
                                      void* c, void* scratch, int64_t scratch_bytes, int32_t* status, lc_stream_t stream) {
   using namespace lc;
-  const int rc = check(M, N, K, b, ldb, b_s, !sym, b_sum, c, dtype);
+  int rc = check(M, N, K, b, ldb, b_s, !sym, b_sum, c, dtype);
   if (rc != LC_OK || M == 0 || N == 0) return rc;
-  if (!x || ldx < 0 || !scratch) return LC_ERR_ARG;
-  if (scratch_bytes < lc_int8_linear_scratch(M, K)) return LC_ERR_WORKSPACE;
+  if (!x || ldx < 0) return LC_ERR_ARG;
+  const int64_t room = lc_int8_linear_scratch(M, N, K);
+  if (room > 0 && !scratch) return LC_ERR_ARG;
+  if (scratch_bytes < room) return LC_ERR_WORKSPACE;
   if (!aligned16(scratch)) return LC_ERR_ALIGN;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const int64_t per_vec = dtype == LC_F32 ? 4 : 8;
+  Int8Args g{x, ldx, sym != 0, aligned16(x) && (M == 1 || ldx % per_vec == 0), nullptr, b, nullptr, nullptr, b_s,
+             sym ? nullptr : b_sum, bias, c, status, 0, ldb, (int)M, (int)N, (int)K};
+  if (room == 0) {
+    if ((rc = check_arch()) != LC_OK) return rc;
+    const int splits = choose(M, N, K).splits;
+    switch (dtype) {
+      case LC_F32: return launch_stream<float, 16, true>(g, splits, false, st);
+      case LC_BF16: return launch_stream<__nv_bfloat16, 16, true>(g, splits, false, st);
+      default: return launch_stream<__half, 16, true>(g, splits, false, st);
+    }
+  }
   const int64_t lda = (K + 15) / 16 * 16;
   int8_t* codes = static_cast<int8_t*>(scratch);
   float* a_s = reinterpret_cast<float*>(codes + M * lda);
   int32_t* a_z = sym ? nullptr : reinterpret_cast<int32_t*>(a_s + M);
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const int qrc = int8_quant_rows(x, dtype, M, K, ldx, codes, lda, a_s, a_z, st);
-  if (qrc != LC_OK) return qrc;
-  return product(Int8Args{codes, b, a_s, a_z, b_s, b_sum, bias, c, status, lda, ldb, (int)M, (int)N, (int)K}, dtype, true,
-                 st);
+  if ((rc = int8_quant_rows(x, dtype, M, K, ldx, codes, lda, a_s, a_z, st)) != LC_OK) return rc;
+  g.a = codes, g.lda = lda, g.a_s = a_s, g.a_z = a_z;
+  return product(g, dtype, true, st);
 }

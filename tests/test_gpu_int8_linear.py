@@ -167,7 +167,9 @@ def test_largest_sums(m):
 
 
 @pytest.mark.parametrize('dtype', TYPES)
-@pytest.mark.parametrize('m,n,k', [(1, 64, 64), (1, 4096, 4096), (4, 1000, 11008), (9, 130, 1399), (40, 256, 512), (300, 520, 1040)])
+@pytest.mark.parametrize('m,n,k', [(1, 1, 1), (1, 64, 64), (1, 4096, 4096), (1, 4096, 4099), (2, 333, 11008), (3, 1000, 9000), (8, 520, 4096),
+                                   (5, 11008, 4096), (7, 130, 130), (8, 40, 17), (4, 1000, 11008), (9, 130, 1399), (40, 256, 512),
+                                   (300, 520, 1040)])
 def test_linear_is_quantisation_and_product(dtype, m, n, k):
     from lightcompress_b200.int8_linear import act_quant, check_status, int8_dynamic_forward_func, int8_gemm
     b, bd, bs = _weight(n, k)

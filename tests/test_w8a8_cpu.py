@@ -43,10 +43,11 @@ def test_product_refusals_at_the_c_boundary():
     assert gemm(K=65794, lda=65808, ldb=65808, a_z=P, b_sum=P) == L.LC_ERR_SHAPE
     assert gemm(M=0, a=None, c=None) == L.LC_OK and gemm(N=0, b=None, c=None) == L.LC_OK
 
-    def linear(M=4, K=64, ldb=64, sym=1, scratch=P, room=1 << 20, dtype=1, b_sum=None, x=P):
+    def linear(M=40, K=64, ldb=64, sym=1, scratch=P, room=1 << 20, dtype=1, b_sum=None, x=P):
         return lib.lc_int8_linear(x, dtype, 64, P, ldb, P, b_sum, None, M, 4, K, sym, P, scratch, room, None, None)
-    assert lib.lc_int8_linear_scratch(4, 65) == 4 * 80 + 32
-    assert linear(room=4 * 64 + 31) == L.LC_ERR_WORKSPACE
+    assert lib.lc_int8_linear_scratch(40, 4, 65) == 40 * 80 + 320
+    assert lib.lc_int8_linear_scratch(1, 4096, 4096) == 0 and lib.lc_int8_linear_scratch(0, 4, 65) == 0
+    assert linear(room=40 * 64 + 319) == L.LC_ERR_WORKSPACE
     assert linear(scratch=None) == L.LC_ERR_ARG and linear(x=None) == L.LC_ERR_ARG
     assert linear(scratch=ctypes.c_void_p(4104)) == L.LC_ERR_ALIGN
     assert linear(sym=0) == L.LC_ERR_ARG and linear(dtype=5) == L.LC_ERR_ARG
