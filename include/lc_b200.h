@@ -623,7 +623,7 @@ int lc_int8_gemm(const int8_t* a, int64_t lda, const float* a_s, const int32_t* 
 
 /* lc_int8_act_quant and lc_int8_gemm as one call: c = x b^T with x M x K of `dtype` quantised on the way (sym != 0:
  * without zero points), c and bias of the same dtype.  scratch: lc_int8_linear_scratch(M, N, K) bytes, 16-byte aligned
- * (0 for a few tokens, which the product quantises itself: scratch may be NULL); its contents are not kept from one call
+ * (0 for a single token that the product quantises itself: scratch may be NULL); its contents are not kept from one call
  * to the next. */
 int64_t lc_int8_linear_scratch(int64_t M, int64_t N, int64_t K);
 int lc_int8_linear(const void* x, int dtype, int64_t ldx, const int8_t* b, int64_t ldb, const float* b_s,

@@ -20,9 +20,8 @@ namespace {
 using namespace umma;
 
 struct Int8Args {
-  const void* x;           // activations that the kernel quantises itself (then a, a_s and a_z are not read)
-  int64_t ldx;
-  int sym, wide;           // wide: x's rows are 16-byte aligned
+  const void* x;           // a token that the kernel quantises itself (then a, a_s and a_z are not read)
+  int sym, wide;           // wide: x is 16-byte aligned
   const int8_t* a;
   const int8_t* b;
   const float* a_s;
@@ -164,14 +163,15 @@ struct Maps {
   CUtensorMap w, x;
 };
 
-// A few tokens are quantised by the product itself (kQuant): every CTA reads all of x for the rows' ranges and lays the
-// codes of its own part of K out as the copies would (8-row, 128-byte swizzled atoms).  That is M * K values from L2 per CTA
-// against a launch and a scratch buffer less, while the CTA's first weights are on their way.
+// A single token is quantised by the product itself (kQuant): every CTA reads all of it for the range, before it asks for
+// its weights (behind them a load took up to 2.5 us to come), keeps it in registers and lays the codes of its own part
+// of K out as the copies would, while its first weights are on their way.  That saves a launch and a scratch buffer (3.5 us
+// of a call); for more values than one a thread's 16 the separate kernel, which the product overlaps, is faster.
 //
 // Shared memory of a CTA: stages, barriers, the tokens' scales and zero points.  The CTA's own partial sums take the
 // stages' place once its products are formed; those of the others land behind everything else where they are small, else
 // behind its own (no CTA of the cluster may have products to form any more then).
-constexpr int kRangeBytes = 2 * 8 * 8 * 4;                  // [min / max][part of a row][row]
+constexpr int kRangeBytes = 2 * (kStreamThreads / 32) * 4;
 template <int NT, bool kQuant> struct StreamSmem {
   static constexpr int kStage = kWeightBytes + (kQuant ? 0 : NT * kBlockK);
   static constexpr int kParts = (NT + 7) * kRows * 4;
@@ -193,70 +193,53 @@ template <int NT, bool kQuant> struct StreamSmem {
   }
 };
 
-// 16 neighbouring values of a row from k on; zeros behind the row's end
+// 16 neighbouring values of the token, as they lie in memory: chunk threadIdx.x of it
+constexpr int kMostToken = kStreamThreads * 16;
+template <typename T> struct Values {
+  uint4 raw[sizeof(T)];
+};
+
 template <typename T>
-__device__ __forceinline__ void load_values(const T* row, int k, int K, bool wide, float (&v)[16]) {
-  constexpr int N = Elem<T>::kPerVec;
-  if (wide && k + 16 <= K) {
+__device__ __forceinline__ Values<T> load_token(const Int8Args& g) {
+  Values<T> v;
+  const int k = (int)threadIdx.x * 16;
+  const T* x = static_cast<const T*>(g.x) + k;
+  if (g.wide && k + 16 <= g.K) {
 #pragma unroll
-    for (int i = 0; i < 16 / N; ++i) {
-      float f[N];
-      unpack16<T>(*reinterpret_cast<const uint4*>(row + k + i * N), f);
-#pragma unroll
-      for (int j = 0; j < N; ++j) v[i * N + j] = f[j];
-    }
+    for (int i = 0; i < (int)sizeof(T); ++i) v.raw[i] = reinterpret_cast<const uint4*>(x)[i];
   } else {
+    T* p = reinterpret_cast<T*>(v.raw);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = k + i < K ? Elem<T>::to_f(row[k + i]) : 0.f;
+    for (int i = 0; i < 16; ++i) p[i] = k + i < g.K ? x[i] : Elem<T>::from_f(0.f);
   }
+  return v;
 }
 
-// All of the CTA's threads: the tokens' scales and zero points, and the codes of k blocks [kb0, kb0 + count).
+// The token's scale and zero point, and its codes in k blocks [kb0, kb0 + count) as row 0 of their atoms.
 template <typename T>
-__device__ __forceinline__ void quantise_tokens(const Int8Args& g, int kb0, int count, uint8_t* codes, float* s_scale,
-                                                int* s_zero, float* range) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rows = g.M <= 1 ? 1 : g.M <= 2 ? 2 : g.M <= 4 ? 4 : 8, parts = 8 / rows;
-  const int chunks = (g.K + 15) / 16;
-  if (const int r = warp % rows; r < g.M) {
-    const T* row = static_cast<const T*>(g.x) + r * g.ldx;
-    float mn = 0.f, mx = 0.f;
-    for (int c = warp / rows * 32 + lane; c < chunks; c += parts * 32) {
-      float v[16];
-      load_values<T>(row, c * 16, g.K, g.wide, v);
+__device__ __forceinline__ void quantise_token(const Int8Args& g, const Values<T>& values, int kb0, int count, uint8_t* codes,
+                                               int block_bytes, float* s_scale, int* s_zero, float* range) {
+  float v[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) mn = nan_min(mn, v[i]), mx = nan_max(mx, v[i]);
-    }
+  for (int i = 0; i < 16; ++i) v[i] = Elem<T>::to_f(reinterpret_cast<const T*>(values.raw)[i]);
+  float mn = 0.f, mx = 0.f;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      mx = nan_max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-      mn = nan_min(mn, __shfl_xor_sync(0xffffffffu, mn, o));
-    }
-    if (lane == 0) range[warp / rows * 8 + r] = mn, range[64 + warp / rows * 8 + r] = mx;
+  for (int i = 0; i < 16; ++i) mn = nan_min(mn, v[i]), mx = nan_max(mx, v[i]);
+  RowGroup<kStreamThreads / 32>::range(mn, mx, range);
+  const RowQuant q = row_quant_of(mn, mx, g.sym);
+  if (threadIdx.x == 0) {
+    *s_scale = q.s;
+    *s_zero = q.z;
   }
-  __syncthreads();
-  auto of_row = [&](int r) {
-    float mn = range[r], mx = range[64 + r];
-    for (int p = 1; p < parts; ++p) mn = nan_min(mn, range[p * 8 + r]), mx = nan_max(mx, range[64 + p * 8 + r]);
-    return row_quant_of(mn, mx, g.sym);
-  };
-  if ((int)threadIdx.x < g.M) {
-    const RowQuant q = of_row(threadIdx.x);
-    s_scale[threadIdx.x] = q.s;
-    s_zero[threadIdx.x] = q.z;
-  }
-  for (int i = threadIdx.x; i < g.M * count * 8; i += kStreamThreads) {
-    const int r = i / (count * 8), at = i - r * (count * 8), kb = at >> 3, c = at & 7;
-    const RowQuant q = of_row(r);
-    float v[16];
-    load_values<T>(static_cast<const T*>(g.x) + r * g.ldx, (kb0 + kb) * kBlockK + c * 16, g.K, g.wide, v);
+  const int kb = ((int)threadIdx.x >> 3) - kb0;
+  if (kb >= 0 && kb < count) {
     uint32_t w[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float u[4] = {v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]};
-      store_row_codes<4>(reinterpret_cast<int8_t*>(w + j), u, q, g.sym);
+    for (int i = 0; i < 4; ++i) {
+      const float u[4] = {v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
+      store_row_codes<4>(reinterpret_cast<int8_t*>(w + i), u, q, g.sym);
     }
-    *reinterpret_cast<uint4*>(codes + kb * (16 * kBlockK) + r * kBlockK + ((c ^ (r & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+    *reinterpret_cast<uint4*>(codes + kb * block_bytes + ((threadIdx.x & 7) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
@@ -287,6 +270,8 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
   // with splits: tokens [first, first + mine) of the tile are this CTA's to finish
   const int run = (tokens + splits - 1) / splits, first = rank * run, mine = max(0, min(run, tokens - first));
 
+  Values<T> token;
+  if constexpr (kQuant) token = load_token<T>(g);
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) {
       mbar_init(full_bar(s), 1);
@@ -319,8 +304,8 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
   const Channel ch = load_channel<T>(g, n);                // weights' side: nothing the kernel before this one writes
   const bool zeros = kQuant ? !g.sym : g.a_z != nullptr;
   if constexpr (kQuant) {
-    quantise_tokens<T>(g, kb0, count, gen + Smem::codes(stages), s_scale, s_zero,
-                       reinterpret_cast<float*>(gen + Smem::ranges(stages, most)));
+    quantise_token<T>(g, token, kb0, count, gen + Smem::codes(stages), NT * kBlockK, s_scale, s_zero,
+                   reinterpret_cast<float*>(gen + Smem::ranges(stages, most)));
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");         // the MMAs read what was just written
     __syncthreads();
   } else {
@@ -745,12 +730,10 @@ Choice choose(int64_t M, int64_t N, int64_t K) {
   return best;
 }
 
-// Whether lc_int8_linear's product quantises the activations itself: one tile of 16 tokens, at most 32768 values for every
-// CTA to read, and codes of a CTA's part of K that leave room for the weights.
+// Whether lc_int8_linear's product quantises the activations itself: one token that a CTA's registers hold, and codes of a
+// CTA's part of K that leave room for the weights.
 bool quantises_itself(int64_t M, int64_t N, int64_t K) {
-  if (M > 8 || M * K > 32768) return false;
-  const Choice c = choose(M, N, K);
-  return c.tokens == 16 && (K + kBlockK - 1) / kBlockK <= (int64_t)32 * c.splits;
+  return M == 1 && K <= kMostToken && (K + kBlockK - 1) / kBlockK <= (int64_t)32 * choose(M, N, K).splits;
 }
 
 // What a kernel may ask for; the same for every launch, so that calls from two threads do not take it from one another.
@@ -877,7 +860,7 @@ extern "C" LC_API int lc_int8_gemm(const int8_t* a, int64_t lda, const float* a_
   if (rc != LC_OK || M == 0 || N == 0) return rc;
   if (!a || !a_s || lda < K) return LC_ERR_ARG;
   if (!aligned16(a) || (lda & 15)) return LC_ERR_ALIGN;
-  return product(Int8Args{nullptr, 0, 0, 0, a, b, a_s, a_z, b_s, b_sum, bias, c, status, lda, ldb, (int)M, (int)N, (int)K}, out_dtype, false,
+  return product(Int8Args{nullptr, 0, 0, a, b, a_s, a_z, b_s, b_sum, bias, c, status, lda, ldb, (int)M, (int)N, (int)K}, out_dtype, false,
                  reinterpret_cast<cudaStream_t>(stream));
 }
 
@@ -899,8 +882,7 @@ extern "C" LC_API int lc_int8_linear(const void* x, int dtype, int64_t ldx, cons
   if (scratch_bytes < room) return LC_ERR_WORKSPACE;
   if (!aligned16(scratch)) return LC_ERR_ALIGN;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  const int64_t per_vec = dtype == LC_F32 ? 4 : 8;
-  Int8Args g{x, ldx, sym != 0, aligned16(x) && (M == 1 || ldx % per_vec == 0), nullptr, b, nullptr, nullptr, b_s,
+  Int8Args g{x, sym != 0, aligned16(x), nullptr, b, nullptr, nullptr, b_s,
              sym ? nullptr : b_sum, bias, c, status, 0, ldb, (int)M, (int)N, (int)K};
   if (room == 0) {
     if ((rc = check_arch()) != LC_OK) return rc;

@@ -216,7 +216,7 @@ def int8_dynamic_forward_func(x, w, w_scale, bias=None, w_sum=None):
         L.refuse_devices(name, x, w=w, w_scale=w_scale, bias=bias, w_sum=w_sum)
     c = x2.new_empty((M, N))
     if M and N:
-        room = L.lib.lc_int8_linear_scratch(M, N, K) if M <= 8 else M * ((K + 15) // 16 * 16 + 8)
+        room = L.lib.lc_int8_linear_scratch(M, N, K) if M == 1 else M * ((K + 15) // 16 * 16 + 8)
         scratch = x2.new_empty(room, dtype=torch.int8) if room else None
         L.launch(dev, 'lc_int8_linear', x2.data_ptr(), dt, x2.stride(0), w.data_ptr(), _pitch(w, N, K), w_scale.data_ptr(),
                  None if sym else w_sum.data_ptr(), None if bias is None else bias.data_ptr(), M, N, K, sym,

@@ -167,7 +167,8 @@ def test_largest_sums(m):
 
 
 @pytest.mark.parametrize('dtype', TYPES)
-@pytest.mark.parametrize('m,n,k', [(1, 1, 1), (1, 64, 64), (1, 4096, 4096), (1, 4096, 4099), (2, 333, 11008), (3, 1000, 9000), (8, 520, 4096),
+@pytest.mark.parametrize('m,n,k', [(1, 1, 1), (1, 64, 64), (1, 4096, 4096), (1, 4096, 4099), (1, 300, 11008), (1, 50, 4080), (1, 50, 4100),
+                                   (1, 20000, 16000), (2, 333, 11008), (3, 1000, 9000), (8, 520, 4096),
                                    (5, 11008, 4096), (7, 130, 130), (8, 40, 17), (4, 1000, 11008), (9, 130, 1399), (40, 256, 512),
                                    (300, 520, 1040)])
 def test_linear_is_quantisation_and_product(dtype, m, n, k):
