@@ -611,24 +611,51 @@ int lc_int8_gated_act_quant(const void* gate, const void* up, int dtype, int64_t
                             int64_t ldu, int act, int8_t* codes, int64_t ldc, float* scales, int32_t* zeros,
                             lc_stream_t stream);
 
+/* Calls with many arguments take them as a struct in host memory; all of its members are 8 bytes wide. */
+
 /* c[m][n] = float(sum_k (a[m][k] - a_z[m]) b[n][k]) * a_s[m] * b_s[n] (+ bias[n]): a M x K and b N x K int8, rows lda /
  * ldb bytes apart; a_s M and b_s N fp32; a_z (M int32) may be NULL, and with it b_sum, the N int32 sums of b's rows;
  * bias N values of out_dtype or NULL; c M x N of out_dtype, contiguous.  The sum is exact in 32 bits, then come two fp32
  * multiplications and an addition, in that order, and one rounding.  a, b and c are 16-byte aligned, lda and ldb multiples
  * of 16 (LC_ERR_ALIGN); K at most 131071, with zero points 65793 (LC_ERR_SHAPE).  *status (may be NULL) receives
  * LC_ERR_TIMEOUT if a bounded pipeline wait expires; outputs that could then not be formed are NaN. */
-int lc_int8_gemm(const int8_t* a, int64_t lda, const float* a_s, const int32_t* a_z, const int8_t* b, int64_t ldb,
-                 const float* b_s, const int32_t* b_sum, const void* bias, int64_t M, int64_t N, int64_t K, void* c,
-                 int out_dtype, int32_t* status, lc_stream_t stream);
+typedef struct {
+  const int8_t* a;
+  int64_t lda;
+  const float* a_s;
+  const int32_t* a_z;
+  const int8_t* b;
+  int64_t ldb;
+  const float* b_s;
+  const int32_t* b_sum;
+  const void* bias;
+  int64_t M, N, K;
+  void* c;
+  int64_t out_dtype;
+  int32_t* status;
+} lc_int8_gemm_args;
+int lc_int8_gemm(const lc_int8_gemm_args* args_host, lc_stream_t stream);
 
-/* lc_int8_act_quant and lc_int8_gemm as one call: c = x b^T with x M x K of `dtype` quantised on the way (sym != 0:
- * without zero points), c and bias of the same dtype.  scratch: lc_int8_linear_scratch(M, N, K) bytes, 16-byte aligned
- * (0 for a single token that the product quantises itself: scratch may be NULL); its contents are not kept from one call
- * to the next. */
-int64_t lc_int8_linear_scratch(int64_t M, int64_t N, int64_t K);
-int lc_int8_linear(const void* x, int dtype, int64_t ldx, const int8_t* b, int64_t ldb, const float* b_s,
-                   const int32_t* b_sum, const void* bias, int64_t M, int64_t N, int64_t K, int sym, void* c,
-                   void* scratch, int64_t scratch_bytes, int32_t* status, lc_stream_t stream);
+/* lc_int8_act_quant and lc_int8_gemm as one call: c = x b^T with x M x K of `dtype` (rows ldx elements apart) quantised on
+ * the way (sym != 0: without zero points, else b_sum is needed), c and bias of the same dtype.  scratch:
+ * lc_int8_linear_scratch(M, K) bytes, 16-byte aligned (0 for a single token of at most 4096 values, which the product
+ * quantises itself: scratch may be NULL); its contents are not kept from one call to the next. */
+int64_t lc_int8_linear_scratch(int64_t M, int64_t K);
+typedef struct {
+  const void* x;
+  int64_t dtype, ldx;
+  const int8_t* b;
+  int64_t ldb;
+  const float* b_s;
+  const int32_t* b_sum;
+  const void* bias;
+  int64_t M, N, K, sym;
+  void* c;
+  void* scratch;
+  int64_t scratch_bytes;
+  int32_t* status;
+} lc_int8_linear_args;
+int lc_int8_linear(const lc_int8_linear_args* args_host, lc_stream_t stream);
 
 /* The residual add of a decoder block with the norms on both sides of it:
  *   t = x, or x * rsqrt(mean(x^2) + eps) * (post_weight + weight_offset) when post_weight is given
@@ -636,12 +663,22 @@ int lc_int8_linear(const void* x, int dtype, int64_t ldx, const int8_t* b, int64
  *   y = h * rsqrt(mean(h^2) + eps) * (weight + weight_offset)      (weight NULL: no y)
  * in fp32 between the loads and the roundings; y is formed from the rounded h.  y is written as `dtype` (y), or
  * quantised from fp32 like lc_int8_act_quant (codes / scales / zeros), or both.  x and residual: rows x cols, rows ldx /
- * ldr elements apart; gate: gate_rows x cols contiguous, row r using gate row r / (rows / gate_rows); h, y contiguous.
- * h may be NULL when x itself is the stream (no residual, post_weight or gate, scale 1): then y is x's norm. */
-int lc_residual_norm(const void* x, const void* residual, const void* post_weight, const void* gate, int64_t gate_rows,
-                     const void* weight, int dtype, int64_t rows, int64_t cols, int64_t ldx, int64_t ldr, float scale,
-                     float eps, float weight_offset, void* h, void* y, int8_t* codes, int64_t ldc, float* scales,
-                     int32_t* zeros, lc_stream_t stream);
+ * ldr elements apart; gate: gate_rows x cols contiguous, row r using gate row r / (rows / gate_rows); h, y contiguous; the
+ * rows of codes lie ldc bytes apart.  h may be NULL when x itself is the stream (no residual, post_weight or gate, scale
+ * 1): then y is x's norm. */
+typedef struct {
+  const void *x, *residual, *post_weight, *gate;
+  int64_t gate_rows;
+  const void* weight;
+  int64_t dtype, rows, cols, ldx, ldr;
+  double scale, eps, weight_offset;
+  void *h, *y;
+  int8_t* codes;
+  int64_t ldc;
+  float* scales;
+  int32_t* zeros;
+} lc_residual_norm_args;
+int lc_residual_norm(const lc_residual_norm_args* args_host, lc_stream_t stream);
 
 /* Rotary embedding of q and k from positions: with angle = positions[b][t] * inv_freq[i], the pair (x1, x2) number i of
  * the first rotary_dim elements of a head becomes scale * (x1 cos - x2 sin, x2 cos + x1 sin); pairs are
@@ -649,12 +686,22 @@ int lc_residual_norm(const void* x, const void* residual, const void* post_weigh
  * formed in fp64, so that far positions (|position| < 2^31) lose nothing; results are rounded once.
  *   q, k        element (b, t, h, d) at [b * q_b + t * q_t + h * q_h + d]; k_heads 0: no k
  *   q_out       (batch, tokens, heads, head_dim) without gaps, or q itself (in place, q's strides); k_out likewise
- *   at most 1023 heads of q and k together, head_dim at most 1024
- *   positions   int64, (b, t) at [b * pos_b + t] (pos_b 0: one row for all);  inv_freq: rotary_dim / 2 fp32 */
-int lc_rotary_embed(const void* q, void* q_out, int q_heads, int64_t q_b, int64_t q_t, int64_t q_h, const void* k,
-                    void* k_out, int k_heads, int64_t k_b, int64_t k_t, int64_t k_h, const int64_t* positions,
-                    int64_t pos_b, const float* inv_freq, int dtype, int64_t batch, int64_t tokens, int head_dim,
-                    int rotary_dim, int interleaved, float scale, lc_stream_t stream);
+ *   positions   int64, (b, t) at [b * pos_b + t] (pos_b 0: one row for all);  inv_freq: rotary_dim / 2 fp32
+ * at most 1023 heads of q and k together, head_dim at most 1024. */
+typedef struct {
+  const void* q;
+  void* q_out;
+  int64_t q_heads, q_b, q_t, q_h;
+  const void* k;
+  void* k_out;
+  int64_t k_heads, k_b, k_t, k_h;
+  const int64_t* positions;
+  int64_t pos_b;
+  const float* inv_freq;
+  int64_t dtype, batch, tokens, head_dim, rotary_dim, interleaved;
+  double scale;
+} lc_rotary_embed_args;
+int lc_rotary_embed(const lc_rotary_embed_args* args_host, lc_stream_t stream);
 
 #ifdef __cplusplus
 }

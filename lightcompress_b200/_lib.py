@@ -6,6 +6,7 @@ no CPU or pure-torch fallback.  torch is used only to own device memory and stre
 """
 import ctypes
 import os
+import struct
 
 import torch
 
@@ -23,6 +24,7 @@ LC_H_REVERSE, LC_H_UPPER, LC_H_LATE_DEAD = 1, 2, 4
 _DTYPES = {torch.float32: LC_F32, torch.bfloat16: LC_BF16, torch.float16: LC_F16}
 
 _p, _i, _i64, _f, _d = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_double
+_s = ctypes.c_char_p     # a packed host struct
 
 # name -> argtypes; every function returns int except those given another restype in _load
 SIGNATURES = {
@@ -83,15 +85,22 @@ SIGNATURES = {
     'lc_rmsnorm': [_p, _p, _i, _i64, _i64, _f, _f, _p, _p],
     'lc_int8_act_quant': [_p, _i, _i64, _i64, _i64, _p, _i64, _p, _p, _p],
     'lc_int8_gated_act_quant': [_p, _p, _i, _i64, _i64, _i64, _i64, _i, _p, _i64, _p, _p, _p],
-    'lc_int8_gemm': [_p, _i64, _p, _p, _p, _i64, _p, _p, _p, _i64, _i64, _i64, _p, _i, _p, _p],
-    'lc_int8_linear_scratch': [_i64, _i64, _i64],
-    'lc_int8_linear': [_p, _i, _i64, _p, _i64, _p, _p, _p, _i64, _i64, _i64, _i, _p, _p, _i64, _p, _p],
-    'lc_residual_norm': [_p, _p, _p, _p, _i64, _p, _i, _i64, _i64, _i64, _i64, _f, _f, _f, _p, _p, _p, _i64, _p, _p, _p],
-    'lc_rotary_embed': [_p, _p, _i, _i64, _i64, _i64, _p, _p, _i, _i64, _i64, _i64, _p, _i64, _p, _i, _i64, _i64, _i, _i,
-                        _i, _f, _p],
+    'lc_int8_gemm': [_s, _p],
+    'lc_int8_linear_scratch': [_i64, _i64],
+    'lc_int8_linear': [_s, _p],
+    'lc_residual_norm': [_s, _p],
+    'lc_rotary_embed': [_s, _p],
     'lc_awq_clip_search': [_p, _p, _i, _i64, _i64, _i64, _i64, _i64, _i, _i, _i, _i, _d, _p, _p, _p, _p],
     'lc_awq_clip_search_cuda_cores': [_p, _p, _i, _i64, _i64, _i64, _i64, _i64, _i, _i, _i, _i, _d, _p, _p, _p, _p],
 }
+
+
+# Host structs of calls with many arguments (include/lc_b200.h), in the order of their members: pointers (0 for none),
+# int64 and double.  Packing one and passing its address costs a third of what as many ctypes arguments do.
+INT8_GEMM = struct.Struct('@PqPPPqPPPqqqPqP')
+INT8_LINEAR = struct.Struct('@PqqPqPPPqqqqPPqP')
+RESIDUAL_NORM = struct.Struct('@PPPPqPqqqqqdddPPPqPP')
+ROTARY_EMBED = struct.Struct('@PPqqqqPPqqqqPqPqqqqqqd')
 
 
 class LcError(RuntimeError):

@@ -246,7 +246,9 @@ def residual_norm(x, residual=None, weight=None, post_weight=None, gate=None, sc
     Returns (h, y).  Without weight, y is None.  With quant, y is what int8_linear.act_quant returns for it, (codes,
     scales) or, with sym=False, (codes, scales, zeros), quantised from fp32.  Where h would equal x, it is x."""
     name = 'residual_norm'
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight, post_weight, gate)):
+    if torch.is_grad_enabled() and (
+            x.requires_grad or (weight is not None and weight.requires_grad) or (residual is not None and residual.requires_grad)
+            or (post_weight is not None and post_weight.requires_grad) or (gate is not None and gate.requires_grad)):
         L.refuse_grad(name)
     dtype, shape, dev = x.dtype, x.shape, x.get_device()
     dt = L._DTYPES.get(dtype)
@@ -261,14 +263,14 @@ def residual_norm(x, residual=None, weight=None, post_weight=None, gate=None, sc
         x2, ldx = x, C
     else:
         x2 = _strided_rows(x)
-        ldx = x2.stride(0)
+        ldx = x2.stride()[0]
     r2, ldr = residual, C
     if residual is not None:
         if residual.shape != shape or residual.dtype != dtype or residual.get_device() != dev:
             _refuse_operand(name, 'residual', residual, x, shape)
         if not residual.is_contiguous():
             r2 = _strided_rows(residual)
-            ldr = r2.stride(0)
+            ldr = r2.stride()[0]
     if weight is not None:
         if weight.dtype != dtype or weight.dim() != 1 or weight.numel() != C or weight.get_device() != dev:
             _refuse_operand(name, 'weight', weight, x, (C,))
@@ -295,9 +297,9 @@ def residual_norm(x, residual=None, weight=None, post_weight=None, gate=None, sc
     elif weight is not None:
         y = torch.empty_like(x) if contiguous else x.new_empty(shape)
     if rows:
-        L.launch(dev, 'lc_residual_norm', x2.data_ptr(), _at(r2), _at(post_weight), _at(gate), gate_rows, _at(weight), dt, rows,
-                 C, ldx, ldr, scale, eps, weight_offset, None if kept else h.data_ptr(), _at(y), _at(codes), pitch, _at(scales),
-                 _at(zeros))
+        L.launch(dev, 'lc_residual_norm', L.RESIDUAL_NORM.pack(
+            x2.data_ptr(), _at(r2), _at(post_weight), _at(gate), gate_rows, _at(weight), dt, rows, C, ldx, ldr, scale, eps,
+            weight_offset, 0 if kept else h.data_ptr(), _at(y), _at(codes), pitch, _at(scales), _at(zeros)))
     return h, int8_linear._shaped(codes, scales, zeros, shape) if quant else y
 
 
@@ -313,7 +315,7 @@ def _refuse_operand(name, key, t, x, shape):
 
 
 def _at(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
 
 
 def rotary_embed(q, k, positions, inv_freq, interleaved=False, attention_scale=1.0, inplace=False):
@@ -352,33 +354,35 @@ def rotary_embed(q, k, positions, inv_freq, interleaved=False, attention_scale=1
     dev = q.get_device()
     if not (positions.get_device() == inv_freq.get_device() == dev) or (k is not None and k.get_device() != dev):
         L.refuse_devices(name, q, k=k, positions=positions, inv_freq=inv_freq)
-    q, q_out, qb, qh, qt = _heads(name, q, inplace)
+    q, q_out, qb, qh, qt = _heads(name, q, B, H, T, D, inplace)
     if k is None:
-        k_out, k_at, ko_at, kb, kh, kt = None, None, None, 0, 0, 0
+        k_out, k_at, ko_at, kb, kh, kt = None, 0, 0, 0, 0, 0
     else:
-        k, k_out, kb, kh, kt = _heads(name, k, inplace)
+        k, k_out, kb, kh, kt = _heads(name, k, B, G, T, D, inplace)
         k_at, ko_at = k.data_ptr(), k_out.data_ptr()
     if B and T:
-        positions = positions.contiguous()
-        L.launch(dev, 'lc_rotary_embed', q.data_ptr(), q_out.data_ptr(), H, qb, qt, qh, k_at, ko_at, G, kb, kt, kh,
-                 positions.data_ptr(), T if len(shape) == 2 and shape[0] > 1 else 0, inv_freq.contiguous().data_ptr(), dt, B, T, D,
-                 2 * half, interleaved, attention_scale)
+        positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
+        L.launch(dev, 'lc_rotary_embed', L.ROTARY_EMBED.pack(
+            q.data_ptr(), q_out.data_ptr(), H, qb, qt, qh, k_at, ko_at, G, kb, kt, kh, positions.data_ptr(),
+            T if len(shape) == 2 and shape[0] > 1 else 0, inv_freq.data_ptr(), dt, B, T, D, 2 * half, interleaved,
+            attention_scale))
     return q_out, k_out
 
 
-def _heads(name, x, inplace):
+def _heads(name, x, B, H, T, D, inplace):
     """(x with contiguous heads, where its result goes, strides of batch, head and token)"""
     sb, sh, st, sd = x.stride()
-    if sd != 1 and x.shape[3] != 1:
+    if sd != 1 and D != 1:
         if inplace:
             raise ValueError(f'{name}: the elements of a head must be contiguous')
         x = x.contiguous()
-        sb, sh, st, _ = x.stride()
+        sb, sh, st, sd = x.stride()
     if inplace:
-        if any(s == 0 and n > 1 for n, s in zip(x.shape, (sb, sh, st))):
+        if (sb == 0 and B > 1) or (sh == 0 and H > 1) or (st == 0 and T > 1):
             raise ValueError(f'{name}: cannot work in place on an expanded tensor')
         return x, x, sb, sh, st
-    B, H, T, D = x.shape
+    if sd == 1 and sh == D and st == H * D and sb == T * H * D:
+        return x, torch.empty_like(x), sb, sh, st           # x lies as the result does, and so will a tensor like it
     return x, x.new_empty((B, T, H, D)).transpose(1, 2), sb, sh, st
 
 

@@ -730,11 +730,9 @@ Choice choose(int64_t M, int64_t N, int64_t K) {
   return best;
 }
 
-// Whether lc_int8_linear's product quantises the activations itself: one token that a CTA's registers hold, and codes of a
-// CTA's part of K that leave room for the weights.
-bool quantises_itself(int64_t M, int64_t N, int64_t K) {
-  return M == 1 && K <= kMostToken && (K + kBlockK - 1) / kBlockK <= (int64_t)32 * choose(M, N, K).splits;
-}
+// Whether lc_int8_linear's product quantises the activations itself: one token that a CTA's registers hold.  Its codes are
+// 2 KB a k block, 64 KB at most, and leave room for the weights.  (One token of any length gets the 16-token tile.)
+bool quantises_itself(int64_t M, int64_t K) { return M == 1 && K <= kMostToken; }
 
 // What a kernel may ask for; the same for every launch, so that calls from two threads do not take it from one another.
 template <typename F>
@@ -817,7 +815,7 @@ int launch(const Int8Args& g, bool dependent, cudaStream_t st) {
 
 // sizes, pitches and alignment of the product; the same rules for both entry points
 int check(int64_t M, int64_t N, int64_t K, const void* b, int64_t ldb, const float* b_s, bool zeros,
-          const int32_t* b_sum, const void* c, int out_dtype) {
+          const int32_t* b_sum, const void* c, int64_t out_dtype) {
   if (out_dtype < LC_F32 || out_dtype > LC_F16 || M < 0 || N < 0 || K <= 0) return LC_ERR_ARG;
   if (zeros && N > 0 && !b_sum) return LC_ERR_ARG;
   // |sum| <= 128 * 128 * K without and 255 * 128 * K with zero points must fit 32 bits
@@ -852,52 +850,53 @@ int product(const Int8Args& g, int out_dtype, bool dependent, cudaStream_t st) {
 }  // namespace
 }  // namespace lc
 
-extern "C" LC_API int lc_int8_gemm(const int8_t* a, int64_t lda, const float* a_s, const int32_t* a_z, const int8_t* b,
-                                   int64_t ldb, const float* b_s, const int32_t* b_sum, const void* bias, int64_t M,
-                                   int64_t N, int64_t K, void* c, int out_dtype, int32_t* status, lc_stream_t stream) {
+extern "C" LC_API int lc_int8_gemm(const lc_int8_gemm_args* args_host, lc_stream_t stream) {
   using namespace lc;
-  const int rc = check(M, N, K, b, ldb, b_s, a_z != nullptr, b_sum, c, out_dtype);
-  if (rc != LC_OK || M == 0 || N == 0) return rc;
-  if (!a || !a_s || lda < K) return LC_ERR_ARG;
-  if (!aligned16(a) || (lda & 15)) return LC_ERR_ALIGN;
-  return product(Int8Args{nullptr, 0, 0, a, b, a_s, a_z, b_s, b_sum, bias, c, status, lda, ldb, (int)M, (int)N, (int)K}, out_dtype, false,
-                 reinterpret_cast<cudaStream_t>(stream));
+  if (!args_host) return LC_ERR_ARG;
+  const lc_int8_gemm_args& p = *args_host;
+  const int rc = check(p.M, p.N, p.K, p.b, p.ldb, p.b_s, p.a_z != nullptr, p.b_sum, p.c, p.out_dtype);
+  if (rc != LC_OK || p.M == 0 || p.N == 0) return rc;
+  if (!p.a || !p.a_s || p.lda < p.K) return LC_ERR_ARG;
+  if (!aligned16(p.a) || (p.lda & 15)) return LC_ERR_ALIGN;
+  return product(Int8Args{nullptr, 0, 0, p.a, p.b, p.a_s, p.a_z, p.b_s, p.b_sum, p.bias, p.c, p.status, p.lda, p.ldb, (int)p.M,
+                          (int)p.N, (int)p.K},
+                 (int)p.out_dtype, false, reinterpret_cast<cudaStream_t>(stream));
 }
 
-extern "C" LC_API int64_t lc_int8_linear_scratch(int64_t M, int64_t N, int64_t K) {
-  using namespace lc;
-  if (M <= 0 || N <= 0 || K <= 0 || quantises_itself(M, N, K)) return 0;
+extern "C" LC_API int64_t lc_int8_linear_scratch(int64_t M, int64_t K) {
+  if (M <= 0 || K <= 0 || lc::quantises_itself(M, K)) return 0;
   return M * ((K + 15) / 16 * 16 + 8);
 }
 
-extern "C" LC_API int lc_int8_linear(const void* x, int dtype, int64_t ldx, const int8_t* b, int64_t ldb, const float* b_s,
-                                     const int32_t* b_sum, const void* bias, int64_t M, int64_t N, int64_t K, int sym,
-                                     void* c, void* scratch, int64_t scratch_bytes, int32_t* status, lc_stream_t stream) {
+extern "C" LC_API int lc_int8_linear(const lc_int8_linear_args* args_host, lc_stream_t stream) {
   using namespace lc;
-  int rc = check(M, N, K, b, ldb, b_s, !sym, b_sum, c, dtype);
-  if (rc != LC_OK || M == 0 || N == 0) return rc;
-  if (!x || ldx < 0) return LC_ERR_ARG;
-  const int64_t room = lc_int8_linear_scratch(M, N, K);
-  if (room > 0 && !scratch) return LC_ERR_ARG;
-  if (scratch_bytes < room) return LC_ERR_WORKSPACE;
-  if (!aligned16(scratch)) return LC_ERR_ALIGN;
+  if (!args_host) return LC_ERR_ARG;
+  const lc_int8_linear_args& p = *args_host;
+  int rc = check(p.M, p.N, p.K, p.b, p.ldb, p.b_s, !p.sym, p.b_sum, p.c, p.dtype);
+  if (rc != LC_OK || p.M == 0 || p.N == 0) return rc;
+  if (!p.x || p.ldx < 0) return LC_ERR_ARG;
+  const int64_t room = lc_int8_linear_scratch(p.M, p.K);
+  if (room > 0 && !p.scratch) return LC_ERR_ARG;
+  if (p.scratch_bytes < room) return LC_ERR_WORKSPACE;
+  if (!aligned16(p.scratch)) return LC_ERR_ALIGN;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  Int8Args g{x, sym != 0, aligned16(x), nullptr, b, nullptr, nullptr, b_s,
-             sym ? nullptr : b_sum, bias, c, status, 0, ldb, (int)M, (int)N, (int)K};
+  const int dtype = (int)p.dtype;
+  Int8Args g{p.x, p.sym != 0, aligned16(p.x), nullptr, p.b, nullptr, nullptr, p.b_s, p.sym ? nullptr : p.b_sum, p.bias, p.c,
+             p.status, 0, p.ldb, (int)p.M, (int)p.N, (int)p.K};
   if (room == 0) {
     if ((rc = check_arch()) != LC_OK) return rc;
-    const int splits = choose(M, N, K).splits;
+    const int splits = choose(1, p.N, p.K).splits;
     switch (dtype) {
       case LC_F32: return launch_stream<float, 16, true>(g, splits, false, st);
       case LC_BF16: return launch_stream<__nv_bfloat16, 16, true>(g, splits, false, st);
       default: return launch_stream<__half, 16, true>(g, splits, false, st);
     }
   }
-  const int64_t lda = (K + 15) / 16 * 16;
-  int8_t* codes = static_cast<int8_t*>(scratch);
-  float* a_s = reinterpret_cast<float*>(codes + M * lda);
-  int32_t* a_z = sym ? nullptr : reinterpret_cast<int32_t*>(a_s + M);
-  if ((rc = int8_quant_rows(x, dtype, M, K, ldx, codes, lda, a_s, a_z, st)) != LC_OK) return rc;
+  const int64_t lda = (p.K + 15) / 16 * 16;
+  int8_t* codes = static_cast<int8_t*>(p.scratch);
+  float* a_s = reinterpret_cast<float*>(codes + p.M * lda);
+  int32_t* a_z = p.sym ? nullptr : reinterpret_cast<int32_t*>(a_s + p.M);
+  if ((rc = int8_quant_rows(p.x, dtype, p.M, p.K, p.ldx, codes, lda, a_s, a_z, st)) != LC_OK) return rc;
   g.a = codes, g.lda = lda, g.a_s = a_s, g.a_z = a_z;
   return product(g, dtype, true, st);
 }

@@ -255,25 +255,23 @@ int launch(const NormArgs& a, cudaStream_t st) {
 }  // namespace
 }  // namespace lc
 
-extern "C" LC_API int lc_residual_norm(const void* x, const void* residual, const void* post_weight, const void* gate,
-                                       int64_t gate_rows, const void* weight, int dtype, int64_t rows, int64_t cols,
-                                       int64_t ldx, int64_t ldr, float scale, float eps, float weight_offset, void* h,
-                                       void* y, int8_t* codes, int64_t ldc, float* scales, int32_t* zeros,
-                                       lc_stream_t stream) {
+extern "C" LC_API int lc_residual_norm(const lc_residual_norm_args* args_host, lc_stream_t stream) {
   using namespace lc;
-  if (dtype < LC_F32 || dtype > LC_F16 || rows < 0 || cols <= 0 || ldx < 0 || ldr < 0) return LC_ERR_ARG;
-  if (gate && (gate_rows <= 0 || rows % gate_rows != 0)) return LC_ERR_SHAPE;
-  if (rows == 0) return LC_OK;
-  if (!x) return LC_ERR_ARG;
+  if (!args_host) return LC_ERR_ARG;
+  const lc_residual_norm_args& p = *args_host;
+  if (p.dtype < LC_F32 || p.dtype > LC_F16 || p.rows < 0 || p.cols <= 0 || p.ldx < 0 || p.ldr < 0) return LC_ERR_ARG;
+  if (p.gate && (p.gate_rows <= 0 || p.rows % p.gate_rows != 0)) return LC_ERR_SHAPE;
+  if (p.rows == 0) return LC_OK;
+  if (!p.x) return LC_ERR_ARG;
   // without h the norm is x's own: nothing may change x first
-  if (!h && (residual || post_weight || gate || scale != 1.f)) return LC_ERR_ARG;
-  if (!h && !weight) return LC_ERR_ARG;
-  if ((weight != nullptr) != (y != nullptr || codes != nullptr)) return LC_ERR_ARG;
-  if (codes && (!scales || ldc < cols)) return LC_ERR_ARG;
-  NormArgs a{x, residual, post_weight, gate, weight, rows, cols, ldx, ldr, gate ? rows / gate_rows : rows, ldc,
-             scale, eps, weight_offset, h, y, codes, scales, zeros};
+  if (!p.h && (p.residual || p.post_weight || p.gate || p.scale != 1.0 || !p.weight)) return LC_ERR_ARG;
+  if ((p.weight != nullptr) != (p.y != nullptr || p.codes != nullptr)) return LC_ERR_ARG;
+  if (p.codes && (!p.scales || p.ldc < p.cols)) return LC_ERR_ARG;
+  NormArgs a{p.x, p.residual, p.post_weight, p.gate, p.weight, p.rows, p.cols, p.ldx, p.ldr,
+             p.gate ? p.rows / p.gate_rows : p.rows, p.ldc, (float)p.scale, (float)p.eps, (float)p.weight_offset,
+             p.h, p.y, p.codes, p.scales, p.zeros};
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  switch (dtype) {
+  switch (p.dtype) {
     case LC_F32: return launch<float>(a, st);
     case LC_BF16: return launch<__nv_bfloat16>(a, st);
     default: return launch<__half>(a, st);

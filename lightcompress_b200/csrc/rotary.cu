@@ -181,29 +181,28 @@ int launch(const RotaryArgs& a, int interleaved, cudaStream_t st) {
 }  // namespace
 }  // namespace lc
 
-extern "C" LC_API int lc_rotary_embed(const void* q, void* q_out, int q_heads, int64_t q_b, int64_t q_t, int64_t q_h,
-                                      const void* k, void* k_out, int k_heads, int64_t k_b, int64_t k_t, int64_t k_h,
-                                      const int64_t* positions, int64_t pos_b, const float* inv_freq, int dtype,
-                                      int64_t batch, int64_t tokens, int head_dim, int rotary_dim, int interleaved,
-                                      float scale, lc_stream_t stream) {
+extern "C" LC_API int lc_rotary_embed(const lc_rotary_embed_args* args_host, lc_stream_t stream) {
   using namespace lc;
-  if (dtype < LC_F32 || dtype > LC_F16 || batch < 0 || tokens < 0 || q_heads < 0 || k_heads < 0) return LC_ERR_ARG;
-  if (head_dim <= 0 || rotary_dim <= 0) return LC_ERR_ARG;
-  if (rotary_dim % 2 != 0 || rotary_dim > head_dim || head_dim > 1024 || q_heads + (int64_t)k_heads > 1023)
-    return LC_ERR_SHAPE;
-  if (batch > (1 << 30) || tokens > (1 << 30)) return LC_ERR_SHAPE;
-  if (batch == 0 || tokens == 0 || q_heads + k_heads == 0) return LC_OK;
-  if (!positions || !inv_freq || (q_heads && (!q || !q_out)) || (k_heads && (!k || !k_out))) return LC_ERR_ARG;
+  if (!args_host) return LC_ERR_ARG;
+  const lc_rotary_embed_args& p = *args_host;
+  if (p.dtype < LC_F32 || p.dtype > LC_F16 || p.batch < 0 || p.tokens < 0 || p.q_heads < 0 || p.k_heads < 0) return LC_ERR_ARG;
+  if (p.head_dim <= 0 || p.rotary_dim <= 0) return LC_ERR_ARG;
+  if (p.rotary_dim % 2 != 0 || p.rotary_dim > p.head_dim || p.head_dim > 1024) return LC_ERR_SHAPE;
+  if (p.q_heads > 1023 || p.k_heads > 1023 || p.q_heads + p.k_heads > 1023) return LC_ERR_SHAPE;
+  if (p.batch > (1 << 30) || p.tokens > (1 << 30)) return LC_ERR_SHAPE;
+  if (p.batch == 0 || p.tokens == 0 || p.q_heads + p.k_heads == 0) return LC_OK;
+  if (!p.positions || !p.inv_freq || (p.q_heads && (!p.q || !p.q_out)) || (p.k_heads && (!p.k || !p.k_out))) return LC_ERR_ARG;
   // outputs lie as (batch, tokens, heads, head_dim) without gaps, unless they are the inputs themselves
-  auto heads = [&](const void* in, void* out, int n, int64_t sb, int64_t st, int64_t sh) {
-    const int64_t row = (int64_t)n * head_dim;
-    return in == out ? Heads{in, out, n, sb, st, sh, sb, st, sh}
-                     : Heads{in, out, n, sb, st, sh, row * tokens, row, head_dim};
+  auto heads = [&](const void* in, void* out, int64_t n, int64_t sb, int64_t st, int64_t sh) {
+    const int64_t row = n * p.head_dim;
+    return in == out ? Heads{in, out, (int)n, sb, st, sh, sb, st, sh}
+                     : Heads{in, out, (int)n, sb, st, sh, row * p.tokens, row, p.head_dim};
   };
-  RotaryArgs a{heads(q, q_out, q_heads, q_b, q_t, q_h), heads(k, k_out, k_heads, k_b, k_t, k_h), positions, pos_b,
-               inv_freq, batch, tokens, head_dim, rotary_dim, scale};
+  RotaryArgs a{heads(p.q, p.q_out, p.q_heads, p.q_b, p.q_t, p.q_h), heads(p.k, p.k_out, p.k_heads, p.k_b, p.k_t, p.k_h),
+               p.positions, p.pos_b, p.inv_freq, p.batch, p.tokens, (int)p.head_dim, (int)p.rotary_dim, (float)p.scale};
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  switch (dtype) {
+  const int interleaved = p.interleaved != 0;
+  switch (p.dtype) {
     case LC_F32: return launch<float>(a, interleaved, st);
     case LC_BF16: return launch<__nv_bfloat16>(a, interleaved, st);
     default: return launch<__half>(a, interleaved, st);

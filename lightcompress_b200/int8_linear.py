@@ -18,12 +18,12 @@ _DTYPES = L._DTYPES
 
 
 def _status_of(t, dev):
-    """Address of the device's status word (a bounded wait that expired in a product), which is made on first use; None
+    """Address of the device's status word (a bounded wait that expired in a product), which is made on first use; 0
     where that first use is inside a capture."""
     s = _status.get(dev)
     if s is None:
         if dev < 0 or torch.cuda.is_current_stream_capturing():
-            return None
+            return 0
         s = torch.zeros(1, dtype=torch.int32, device=t.device)
         torch.cuda.current_stream(dev).synchronize()      # other streams may use it from here on
         _status[dev] = s
@@ -57,7 +57,7 @@ def _float_rows(name, x):
 
 def _codes_like(x2, rows, cols, sym):
     """Room for the codes (rows 16 bytes apart or a multiple of that, as the products read them), scales, zeros."""
-    pitch = (cols + 15) // 16 * 16
+    pitch = (cols + 15) & -16
     codes = x2.new_empty((rows, pitch), dtype=torch.int8)
     scales = x2.new_empty((rows, 1), dtype=torch.float32)
     return codes, pitch, scales, None if sym else x2.new_empty((rows, 1), dtype=torch.int32)
@@ -85,7 +85,7 @@ def act_quant(x, sym=True):
     rows, cols = x2.shape
     codes, pitch, scales, zeros = _codes_like(x2, rows, cols, sym)
     if rows:
-        L.launch(x2.get_device(), 'lc_int8_act_quant', x2.data_ptr(), dt, rows, cols, x2.stride(0), codes.data_ptr(), pitch,
+        L.launch(x2.get_device(), 'lc_int8_act_quant', x2.data_ptr(), dt, rows, cols, x2.stride()[0], codes.data_ptr(), pitch,
                  scales.data_ptr(), None if sym else zeros.data_ptr())
     return _shaped(codes, scales, zeros, x.shape)
 
@@ -109,7 +109,7 @@ def gated_act_quant(gate, up, act='silu', sym=True):
     rows, cols = g2.shape
     codes, pitch, scales, zeros = _codes_like(g2, rows, cols, sym)
     if rows:
-        L.launch(dev, 'lc_int8_gated_act_quant', g2.data_ptr(), u2.data_ptr(), dt, rows, cols, g2.stride(0), u2.stride(0), kind,
+        L.launch(dev, 'lc_int8_gated_act_quant', g2.data_ptr(), u2.data_ptr(), dt, rows, cols, g2.stride()[0], u2.stride()[0], kind,
                  codes.data_ptr(), pitch, scales.data_ptr(), None if sym else zeros.data_ptr())
     return _shaped(codes, scales, zeros, shape)
 
@@ -129,14 +129,13 @@ def aligned_rows(codes):
 
 def _rows_aligned(t):
     rows, cols = t.shape
-    pitch = t.stride(0)
-    return (not t.data_ptr() & 15 and (t.stride(1) == 1 or cols == 1)
-            and ((not pitch & 15 and pitch >= cols) or rows <= 1))
+    pitch, step = t.stride()
+    return not t.data_ptr() & 15 and (step == 1 or cols == 1) and ((not pitch & 15 and pitch >= cols) or rows <= 1)
 
 
 def _pitch(t, rows, cols):
     """Row pitch of an aligned 2-D code tensor; a single row may carry any stride."""
-    return t.stride(0) if rows > 1 else (cols + 15) // 16 * 16
+    return t.stride()[0] if rows > 1 else (cols + 15) & -16
 
 
 def _check_weight(name, b, b_s, b_sum, bias, zeros, out_dtype):
@@ -191,9 +190,10 @@ def int8_gemm(a, a_s, b, b_s, bias=None, a_z=None, b_sum=None, out_dtype=torch.b
         L.refuse_devices(name, a, a_s=a_s, a_z=a_z, b=b, b_s=b_s, b_sum=b_sum, bias=bias)
     c = a2.new_empty((M, N), dtype=out_dtype)
     if M and N:
-        L.launch(dev, 'lc_int8_gemm', a2.data_ptr(), _pitch(a2, M, K), a_s.data_ptr(), None if a_z is None else a_z.data_ptr(),
-                 b.data_ptr(), _pitch(b, N, K), b_s.data_ptr(), None if a_z is None else b_sum.data_ptr(),
-                 None if bias is None else bias.data_ptr(), M, N, K, c.data_ptr(), out, _status_of(a, dev))
+        L.launch(dev, 'lc_int8_gemm', L.INT8_GEMM.pack(
+            a2.data_ptr(), _pitch(a2, M, K), a_s.data_ptr(), 0 if a_z is None else a_z.data_ptr(), b.data_ptr(), _pitch(b, N, K),
+            b_s.data_ptr(), 0 if a_z is None else b_sum.data_ptr(), 0 if bias is None else bias.data_ptr(), M, N, K,
+            c.data_ptr(), out, _status_of(a, dev)))
     return c if a.dim() == 2 else c.view(*a.shape[:-1], N)
 
 
@@ -216,11 +216,13 @@ def int8_dynamic_forward_func(x, w, w_scale, bias=None, w_sum=None):
         L.refuse_devices(name, x, w=w, w_scale=w_scale, bias=bias, w_sum=w_sum)
     c = x2.new_empty((M, N))
     if M and N:
-        room = L.lib.lc_int8_linear_scratch(M, N, K) if M == 1 else M * ((K + 15) // 16 * 16 + 8)
+        # lc_int8_linear_scratch(M, K)
+        room = 0 if M == 1 and K <= 4096 else M * (((K + 15) & -16) + 8)
         scratch = x2.new_empty(room, dtype=torch.int8) if room else None
-        L.launch(dev, 'lc_int8_linear', x2.data_ptr(), dt, x2.stride(0), w.data_ptr(), _pitch(w, N, K), w_scale.data_ptr(),
-                 None if sym else w_sum.data_ptr(), None if bias is None else bias.data_ptr(), M, N, K, sym,
-                 c.data_ptr(), scratch.data_ptr() if room else None, room, _status_of(x, dev))
+        L.launch(dev, 'lc_int8_linear', L.INT8_LINEAR.pack(
+            x2.data_ptr(), dt, x2.stride()[0], w.data_ptr(), _pitch(w, N, K), w_scale.data_ptr(), 0 if sym else w_sum.data_ptr(),
+            0 if bias is None else bias.data_ptr(), M, N, K, sym, c.data_ptr(), scratch.data_ptr() if room else 0, room,
+            _status_of(x, dev)))
     return c if x.dim() == 2 else c.view(*x.shape[:-1], N)
 
 

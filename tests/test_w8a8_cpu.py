@@ -1,11 +1,14 @@
 """Refusals of the operators of a deployed W8A8 block, and the rotary frequencies: nothing here needs a GPU."""
 import ctypes
 import math
+import os
+import re
 
 import pytest
 import torch
 
-P = ctypes.c_void_p(4096)          # an aligned address that no refused call may touch
+A = 4096                           # an aligned address that no refused call may touch
+P = ctypes.c_void_p(A)
 
 
 def _lib():
@@ -31,49 +34,68 @@ def test_quantisation_refusals_at_the_c_boundary():
 def test_product_refusals_at_the_c_boundary():
     L, lib = _lib()
 
-    def gemm(a=P, lda=64, a_s=P, a_z=None, b=P, ldb=64, b_s=P, b_sum=None, M=4, N=4, K=64, c=P, out=1):
-        return lib.lc_int8_gemm(a, lda, a_s, a_z, b, ldb, b_s, b_sum, None, M, N, K, c, out, None, None)
+    def gemm(a=A, lda=64, a_s=A, a_z=0, b=A, ldb=64, b_s=A, b_sum=0, M=4, N=4, K=64, c=A, out=1):
+        return lib.lc_int8_gemm(L.INT8_GEMM.pack(a, lda, a_s, a_z, b, ldb, b_s, b_sum, 0, M, N, K, c, out, 0), None)
     assert gemm(out=3) == L.LC_ERR_ARG
     assert gemm(K=0) == L.LC_ERR_ARG
     assert gemm(lda=72) == L.LC_ERR_ALIGN and gemm(ldb=72) == L.LC_ERR_ALIGN
-    assert gemm(a=ctypes.c_void_p(4100)) == L.LC_ERR_ALIGN and gemm(b=ctypes.c_void_p(4100)) == L.LC_ERR_ALIGN
+    assert gemm(a=4100) == L.LC_ERR_ALIGN and gemm(b=4100) == L.LC_ERR_ALIGN
     assert gemm(lda=48) == L.LC_ERR_ARG and gemm(ldb=48) == L.LC_ERR_ARG
-    assert gemm(a_z=P) == L.LC_ERR_ARG                                         # zero points without b_sum
+    assert gemm(a_z=A) == L.LC_ERR_ARG                                         # zero points without b_sum
     assert gemm(K=131072, lda=131072, ldb=131072) == L.LC_ERR_SHAPE
-    assert gemm(K=65794, lda=65808, ldb=65808, a_z=P, b_sum=P) == L.LC_ERR_SHAPE
-    assert gemm(M=0, a=None, c=None) == L.LC_OK and gemm(N=0, b=None, c=None) == L.LC_OK
+    assert gemm(K=65794, lda=65808, ldb=65808, a_z=A, b_sum=A) == L.LC_ERR_SHAPE
+    assert gemm(M=0, a=0, c=0) == L.LC_OK and gemm(N=0, b=0, c=0) == L.LC_OK
 
-    def linear(M=40, K=64, ldb=64, sym=1, scratch=P, room=1 << 20, dtype=1, b_sum=None, x=P):
-        return lib.lc_int8_linear(x, dtype, 64, P, ldb, P, b_sum, None, M, 4, K, sym, P, scratch, room, None, None)
-    assert lib.lc_int8_linear_scratch(40, 4, 65) == 40 * 80 + 320
-    assert lib.lc_int8_linear_scratch(1, 4096, 4096) == 0 and lib.lc_int8_linear_scratch(0, 4, 65) == 0
+    def linear(M=40, K=64, ldb=64, sym=1, scratch=A, room=1 << 20, dtype=1, b_sum=0, x=A):
+        return lib.lc_int8_linear(L.INT8_LINEAR.pack(x, dtype, 64, A, ldb, A, b_sum, 0, M, 4, K, sym, A, scratch, room, 0), None)
+    assert lib.lc_int8_linear_scratch(40, 65) == 40 * 80 + 320 and lib.lc_int8_linear_scratch(1, 4097) == 4112 + 8
+    assert lib.lc_int8_linear_scratch(1, 4096) == 0 and lib.lc_int8_linear_scratch(0, 65) == 0
     assert linear(room=40 * 64 + 319) == L.LC_ERR_WORKSPACE
-    assert linear(scratch=None) == L.LC_ERR_ARG and linear(x=None) == L.LC_ERR_ARG
-    assert linear(scratch=ctypes.c_void_p(4104)) == L.LC_ERR_ALIGN
+    assert linear(scratch=0) == L.LC_ERR_ARG and linear(x=0) == L.LC_ERR_ARG
+    assert linear(scratch=4104) == L.LC_ERR_ALIGN
     assert linear(sym=0) == L.LC_ERR_ARG and linear(dtype=5) == L.LC_ERR_ARG
-    assert linear(M=0, scratch=None, room=0) == L.LC_OK
+    assert linear(M=0, scratch=0, room=0) == L.LC_OK
 
 
 def test_norm_and_rotary_refusals_at_the_c_boundary():
     L, lib = _lib()
 
-    def norm(x=P, res=None, post=None, gate=None, gate_rows=0, w=P, dtype=1, rows=4, cols=64, scale=1.0, h=None, y=P,
-             codes=None, ldc=64, scales=None):
-        return lib.lc_residual_norm(x, res, post, gate, gate_rows, w, dtype, rows, cols, 64, 64, scale, 1e-6, 0.0, h, y, codes,
-                                    ldc, scales, None, None)
+    def norm(x=A, res=0, post=0, gate=0, gate_rows=0, w=A, dtype=1, rows=4, cols=64, scale=1.0, h=0, y=A,
+             codes=0, ldc=64, scales=0):
+        return lib.lc_residual_norm(L.RESIDUAL_NORM.pack(x, res, post, gate, gate_rows, w, dtype, rows, cols, 64, 64, scale, 1e-6,
+                                                         0.0, h, y, codes, ldc, scales, 0), None)
     assert norm(dtype=7) == L.LC_ERR_ARG and norm(cols=0) == L.LC_ERR_ARG
-    assert norm(gate=P, gate_rows=3, h=P) == L.LC_ERR_SHAPE and norm(gate=P, gate_rows=0, h=P) == L.LC_ERR_SHAPE
-    assert norm(res=P) == L.LC_ERR_ARG and norm(scale=0.5) == L.LC_ERR_ARG      # a changed stream without room for it
-    assert norm(w=None, y=None) == L.LC_ERR_ARG and norm(w=None) == L.LC_ERR_ARG and norm(y=None) == L.LC_ERR_ARG
-    assert norm(codes=P) == L.LC_ERR_ARG and norm(codes=P, scales=P, ldc=63) == L.LC_ERR_ARG
-    assert norm(rows=0, x=None) == L.LC_OK
+    assert norm(gate=A, gate_rows=3, h=A) == L.LC_ERR_SHAPE and norm(gate=A, gate_rows=0, h=A) == L.LC_ERR_SHAPE
+    assert norm(res=A) == L.LC_ERR_ARG and norm(scale=0.5) == L.LC_ERR_ARG      # a changed stream without room for it
+    assert norm(w=0, y=0) == L.LC_ERR_ARG and norm(w=0) == L.LC_ERR_ARG and norm(y=0) == L.LC_ERR_ARG
+    assert norm(codes=A) == L.LC_ERR_ARG and norm(codes=A, scales=A, ldc=63) == L.LC_ERR_ARG
+    assert norm(rows=0, x=0) == L.LC_OK
 
-    def rope(q=P, qh=2, k=P, kh=1, pos=P, freq=P, dtype=1, B=1, T=1, D=64, R=64):
-        return lib.lc_rotary_embed(q, q, qh, 0, 0, 64, k, k, kh, 0, 0, 64, pos, 0, freq, dtype, B, T, D, R, 0, 1.0, None)
+    def rope(q=A, qh=2, k=A, kh=1, pos=A, freq=A, dtype=1, B=1, T=1, D=64, R=64):
+        return lib.lc_rotary_embed(L.ROTARY_EMBED.pack(q, q, qh, 0, 0, 64, k, k, kh, 0, 0, 64, pos, 0, freq, dtype, B, T, D, R, 0,
+                                                       1.0), None)
     assert rope(dtype=3) == L.LC_ERR_ARG and rope(R=0) == L.LC_ERR_ARG
     assert rope(R=63) == L.LC_ERR_SHAPE and rope(R=66) == L.LC_ERR_SHAPE and rope(D=1026, R=64) == L.LC_ERR_SHAPE
-    assert rope(q=None) == L.LC_ERR_ARG and rope(k=None) == L.LC_ERR_ARG and rope(pos=None) == L.LC_ERR_ARG
-    assert rope(T=0, q=None) == L.LC_OK and rope(qh=0, kh=0, q=None, k=None) == L.LC_OK
+    assert rope(q=0) == L.LC_ERR_ARG and rope(k=0) == L.LC_ERR_ARG and rope(pos=0) == L.LC_ERR_ARG
+    assert rope(T=0, q=0) == L.LC_OK and rope(qh=0, kh=0, q=0, k=0) == L.LC_OK
+    assert rope(qh=1000, kh=24) == L.LC_ERR_SHAPE
+    for f in (lib.lc_int8_gemm, lib.lc_int8_linear, lib.lc_residual_norm, lib.lc_rotary_embed):
+        assert f(None, None) == L.LC_ERR_ARG
+
+
+def test_packed_structs_match_the_header():
+    """Every member is 8 bytes wide, and the packed formats name the header's members one by one."""
+    L, _ = _lib()
+    text = open(os.path.join(os.path.dirname(L.__file__), '..', 'include', 'lc_b200.h')).read()
+    for fmt, name in ((L.INT8_GEMM, 'int8_gemm'), (L.INT8_LINEAR, 'int8_linear'), (L.RESIDUAL_NORM, 'residual_norm'),
+                      (L.ROTARY_EMBED, 'rotary_embed')):
+        body = re.search(r'typedef struct \{([^}]*)\} lc_%s_args;' % name, text).group(1)
+        want = '@'
+        for line in filter(None, (v.strip() for v in body.split(';'))):
+            kind = 'P' if '*' in line else 'd' if line.startswith('double') else 'q'
+            assert kind == 'P' or line.startswith(('int64_t ', 'double '))
+            want += kind * (line.count(',') + 1)
+        assert fmt.format == want and fmt.size == 8 * (len(want) - 1)
 
 
 def test_int8_linear_refusals():
