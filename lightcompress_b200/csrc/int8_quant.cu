@@ -10,11 +10,20 @@ constexpr int kThreads = 256;
 
 enum Act { kNone = 0, kSilu = LC_ACT_SILU, kGelu = LC_ACT_GELU, kGeluTanh = LC_ACT_GELU_TANH };
 
+// Quotients and exponentials by the fast intrinsics (2 steps and |x| 2^-22 relative at most): a thousandth of a code.  The
+// tanh form is x times the logistic function of twice its argument; the erf form uses erfc(z) = (a1 t + .. + a5 t^5)
+// exp(-z^2), t = 1 / (1 + p z), z >= 0, absolute error 1.5e-7 (Abramowitz and Stegun, Handbook of Mathematical Functions,
+// 7.1.26), which keeps both tails.  The library's erff and tanhf bound the kernel: 40 and 36 us for 2048 x 11008 in bf16.
 template <int kAct>
 __device__ __forceinline__ float act_of(float x) {
   if (kAct == kSilu) return __fdividef(x, 1.f + __expf(-x));
-  if (kAct == kGelu) return 0.5f * x * (1.f + erff(x * 0.70710678118654752f));
-  if (kAct == kGeluTanh) return 0.5f * x * (1.f + tanhf(0.79788456080286536f * (x + 0.044715f * x * x * x)));
+  if (kAct == kGeluTanh) return __fdividef(x, 1.f + __expf(-1.5957691216057308f * (x + 0.044715f * x * x * x)));
+  if (kAct == kGelu) {
+    const float z = fabsf(x) * 0.70710678118654752f, t = __fdividef(1.f, fmaf(0.3275911f, z, 1.f));
+    const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+    const float tail = 0.5f * p * __expf(-z * z);            // half of erfc(z)
+    return x * (x >= 0.f ? 1.f - tail : tail);
+  }
   return x;
 }
 
@@ -74,14 +83,12 @@ __global__ void __launch_bounds__(kThreads) quant_any_kernel(QuantArgs a) {
   }
 }
 
-__device__ __forceinline__ float act_at_run_time(float x, int act) {
-  return act == kSilu ? act_of<kSilu>(x) : act == kGelu ? act_of<kGelu>(x) : act_of<kGeluTanh>(x);
-}
-
-// Rows that registers hold, 16-byte aligned: read once, written once.
-template <typename T, int kWarps, int kVecs, bool kGated>
-__global__ void __launch_bounds__(RowGroup<kWarps>::kThreads) quant_rows_kernel(QuantArgs a, int act) {
+// Rows that registers hold, 16-byte aligned: read once, written once.  HBM-bound: 16384 x 11008 in bf16 85 us (6.4 TB/s, 98 %
+// of a copy's rate), with a zero point 93; silu(gate) * up 148 (6.1 TB/s), the tanh form of gelu 169, the erf form 212.
+template <typename T, int kWarps, int kVecs, int kAct>
+__global__ void __launch_bounds__(RowGroup<kWarps>::kThreads) quant_rows_kernel(QuantArgs a) {
   using G = RowGroup<kWarps>;
+  constexpr bool kGated = kAct != kNone;
   constexpr int N = Elem<T>::kPerVec;
   __shared__ float red[2 * kWarps];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // as in quant_any_kernel
@@ -107,7 +114,7 @@ __global__ void __launch_bounds__(RowGroup<kWarps>::kThreads) quant_rows_kernel(
       float w[N];
       unpack16<T>(ru[k], w);
 #pragma unroll
-      for (int j = 0; j < N; ++j) v[k][j] = act_at_run_time(v[k][j], act) * w[j];
+      for (int j = 0; j < N; ++j) v[k][j] = act_of<kAct>(v[k][j]) * w[j];
     }
 #pragma unroll
     for (int j = 0; j < N; ++j) {
@@ -130,23 +137,23 @@ __global__ void __launch_bounds__(RowGroup<kWarps>::kThreads) quant_rows_kernel(
 }
 
 // whether quant_rows_kernel took the rows
-template <typename T, bool kGated>
-bool launch_rows(const QuantArgs& a, int act, cudaStream_t st) {
+template <typename T, int kAct>
+bool launch_rows(const QuantArgs& a, cudaStream_t st) {
   constexpr int N = Elem<T>::kPerVec;
   if (a.cols % N || (a.rows > 1 && (a.ldx % N || a.ldu % N || a.ldc % N)) || !aligned16(a.x) || !aligned16(a.up) ||
       (reinterpret_cast<uintptr_t>(a.codes) & (N - 1)) || a.rows > 0x7fffffff)
     return false;
-  return with_row_shape(a.cols / N, [&](auto shape) {
+  return with_row_shape<false>(a.cols / N, a.rows, [&](auto shape) {
     using S = decltype(shape);
     using G = RowGroup<S::kWarps>;
-    quant_rows_kernel<T, S::kWarps, S::kVecs, kGated>
-        <<<(unsigned)((a.rows + G::kRows - 1) / G::kRows), G::kThreads, 0, st>>>(a, act);
+    quant_rows_kernel<T, S::kWarps, S::kVecs, kAct>
+        <<<(unsigned)((a.rows + G::kRows - 1) / G::kRows), G::kThreads, 0, st>>>(a);
   });
 }
 
 template <typename T, int kAct, bool kSym>
 int launch(const QuantArgs& a, cudaStream_t st) {
-  if (launch_rows<T, kAct != kNone>(a, kAct, st)) {
+  if (launch_rows<T, kAct>(a, st)) {
     LC_LAUNCH_CHECK();
     return LC_OK;
   }

@@ -156,22 +156,31 @@ __device__ __forceinline__ void unpack16(const uint4& v, float (&f)[Elem<T>::kPe
   for (int i = 0; i < Elem<T>::kPerVec; ++i) f[i] = Elem<T>::to_f(p[i]);
 }
 
-// Which kernel holds rows of `vecs` 16-byte vectors: f(kWarps, kVecs) as integral constants; false where none does.
-// One warp to a row up to 2 KB (no barrier); four warps with up to four vectors a lane, which keeps enough CTAs on an
-// SM to cover the barriers; eight warps up to 32 KB.
+// Which kernel holds rows of `vecs` 16-byte vectors: f(RowShape<warps of a row, vectors a lane>); false where none does.
+// One warp to a row up to 2 KB, which needs no barrier; above, the fewest warps whose registers still leave several CTAs to
+// an SM (4096 values in bf16, 8192 rows: 4 x 4 14.7 us, 8 x 2 17.5, 16 x 1 27.4; 11008 values, quantised: 8 x 6 20.1, 16 x 3
+// 28.9; norms, with two inputs: 108 and 69).  A few rows leave the SMs empty: there what counts is how little a
+// lane does (one gated row of 8192: 16 x 2).  Not so for norms: a sum's association follows the shape, and a row's result
+// must not depend on how many others there are (one row of 4096: 3.2 us instead of 2.7).
 template <int W, int V> struct RowShape {
   static constexpr int kWarps = W, kVecs = V;
 };
-template <typename F>
-bool with_row_shape(int64_t vecs, F&& f) {
+template <bool kNorm, typename F>
+bool with_row_shape(int64_t vecs, int64_t rows, F&& f) {
+  const bool few = !kNorm && rows <= kNumSMsB200;
   if (vecs <= 32) f(RowShape<1, 1>{});
   else if (vecs <= 64) f(RowShape<1, 2>{});
   else if (vecs <= 128) f(RowShape<1, 4>{});
   else if (vecs <= 256) f(RowShape<4, 2>{});
+  else if (vecs <= 512 && few) f(RowShape<8, 2>{});
   else if (vecs <= 512) f(RowShape<4, 4>{});
+  else if (vecs <= 1024 && few) f(RowShape<16, 2>{});
   else if (vecs <= 1024) f(RowShape<8, 4>{});
+  else if (vecs <= 1536 && (few || kNorm)) f(RowShape<16, 3>{});
   else if (vecs <= 1536) f(RowShape<8, 6>{});
-  else if (vecs <= 2048) f(RowShape<8, 8>{});
+  else if (vecs <= 2048 && kNorm) f(RowShape<8, 8>{});
+  else if (vecs <= 2048) f(RowShape<16, 4>{});
+  else if (vecs <= 4096) f(RowShape<16, 8>{});
   else return false;
   return true;
 }

@@ -146,3 +146,17 @@ def test_empty_and_captured():
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(out[0], wh) and torch.equal(out[1][0], wc) and torch.equal(out[1][1], ws)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('c', [256, 1000, 4096, 8192, 11008, 16384])
+def test_a_row_does_not_depend_on_the_others(dtype, c):
+    from lightcompress_b200.block_ops import residual_norm
+    x, res, w = _data((400, c), dtype, 1).cuda(), _data((400, c), dtype, 2).cuda(), _data((c,), dtype, 3).cuda()
+    h, q = residual_norm(x, res, weight=w, post_weight=w, quant=True)
+    _, y = residual_norm(x, res, weight=w, post_weight=w)
+    for rows in (slice(0, 1), slice(399, 400), slice(7, 30)):
+        hs, qs = residual_norm(x[rows], res[rows], weight=w, post_weight=w, quant=True)
+        _, ys = residual_norm(x[rows], res[rows], weight=w, post_weight=w)
+        assert torch.equal(hs, h[rows]) and torch.equal(ys, y[rows])
+        assert torch.equal(qs[0], q[0][rows]) and torch.equal(qs[1], q[1][rows])
