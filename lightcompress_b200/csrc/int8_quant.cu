@@ -1,6 +1,8 @@
 // Per-token 8-bit quantisation of activations in front of the integer linear (the scaled_int8_quant call of
 // the reference's VllmQuantLinearInt8, llmc/compression/quantization/module_utils.py:145-166), of a tensor or of
 // the gated activation act(gate) * up that feeds an MLP's down projection.  Arithmetic: row_quant.cuh.
+#include <type_traits>
+
 #include "row_quant.cuh"
 
 namespace lc {
@@ -83,43 +85,46 @@ __global__ void __launch_bounds__(kThreads) quant_any_kernel(QuantArgs a) {
   }
 }
 
-// Rows that registers hold, 16-byte aligned: read once, written once.  HBM-bound: 16384 x 11008 in bf16 85 us (6.4 TB/s, 98 %
+// Rows that registers hold, by 16-byte vectors or (not aligned) by single values: read once, written once.  HBM-bound: 16384 x 11008 in bf16 85 us (6.4 TB/s, 98 %
 // of a copy's rate), with a zero point 93; silu(gate) * up 148 (6.1 TB/s), the tanh form of gelu 169, the erf form 212.
-template <typename T, int kWarps, int kVecs, int kAct>
+template <typename T, int N, int kWarps, int kVecs, int kAct>
 __global__ void __launch_bounds__(RowGroup<kWarps>::kThreads) quant_rows_kernel(QuantArgs a) {
   using G = RowGroup<kWarps>;
   constexpr bool kGated = kAct != kNone;
-  constexpr int N = Elem<T>::kPerVec;
   __shared__ float red[2 * kWarps];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // as in quant_any_kernel
   const int64_t row = (int64_t)blockIdx.x * G::kRows + G::row();
   if (G::kRows > 1 && row >= a.rows) return;                           // a whole warp, and no barrier follows
   const int vecs = (int)(a.cols / N);
   const bool sym = a.zeros == nullptr;
-  const uint4* x = reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + row * a.ldx);
-  const uint4* u = reinterpret_cast<const uint4*>(static_cast<const T*>(a.up) + row * a.ldu);
-  uint4 rx[kVecs], ru[kGated ? kVecs : 1];
+  const T* x = static_cast<const T*>(a.x) + row * a.ldx;
+  const T* u = static_cast<const T*>(a.up) + row * a.ldu;
+  Raw<T, N> rx[kVecs], ru[kGated ? kVecs : 1];
 #pragma unroll
   for (int k = 0; k < kVecs; ++k) {
     const int i = G::lane() + k * G::kLanes;
-    rx[k] = i < vecs ? __ldcs(x + i) : make_uint4(0u, 0u, 0u, 0u);
-    if (kGated) ru[k] = i < vecs ? __ldcs(u + i) : make_uint4(0u, 0u, 0u, 0u);
+    if (i < vecs) {
+      rx[k] = load_stream<T, N>(x + i * N);
+      if (kGated) ru[k] = load_stream<T, N>(u + i * N);
+    }
   }
   float v[kVecs][N];
   float mn = 0.f, mx = 0.f;
 #pragma unroll
   for (int k = 0; k < kVecs; ++k) {
-    unpack16<T>(rx[k], v[k]);
-    if (kGated) {
-      float w[N];
-      unpack16<T>(ru[k], w);
+    if (G::lane() + k * G::kLanes < vecs) {
+      unpack<T, N>(rx[k], v[k]);
+      if (kGated) {
+        float w[N];
+        unpack<T, N>(ru[k], w);
 #pragma unroll
-      for (int j = 0; j < N; ++j) v[k][j] = act_of<kAct>(v[k][j]) * w[j];
-    }
+        for (int j = 0; j < N; ++j) v[k][j] = act_of<kAct>(v[k][j]) * w[j];
+      }
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      mx = nan_max(mx, v[k][j]);
-      mn = nan_min(mn, v[k][j]);
+      for (int j = 0; j < N; ++j) {
+        mx = nan_max(mx, v[k][j]);
+        mn = nan_min(mn, v[k][j]);
+      }
     }
   }
   G::range(mn, mx, red);
@@ -140,15 +145,17 @@ __global__ void __launch_bounds__(RowGroup<kWarps>::kThreads) quant_rows_kernel(
 template <typename T, int kAct>
 bool launch_rows(const QuantArgs& a, cudaStream_t st) {
   constexpr int N = Elem<T>::kPerVec;
-  if (a.cols % N || (a.rows > 1 && (a.ldx % N || a.ldu % N || a.ldc % N)) || !aligned16(a.x) || !aligned16(a.up) ||
-      (reinterpret_cast<uintptr_t>(a.codes) & (N - 1)) || a.rows > 0x7fffffff)
-    return false;
-  return with_row_shape<false>(a.cols / N, a.rows, [&](auto shape) {
+  if (a.rows > 0x7fffffff) return false;
+  const bool wide = a.cols % N == 0 && (a.rows == 1 || (a.ldx % N == 0 && a.ldu % N == 0 && a.ldc % N == 0)) && aligned16(a.x) &&
+                    aligned16(a.up) && (reinterpret_cast<uintptr_t>(a.codes) & (N - 1)) == 0;
+  auto go = [&](auto shape, auto width) {
     using S = decltype(shape);
     using G = RowGroup<S::kWarps>;
-    quant_rows_kernel<T, S::kWarps, S::kVecs, kAct>
+    quant_rows_kernel<T, decltype(width)::value, S::kWarps, S::kVecs, kAct>
         <<<(unsigned)((a.rows + G::kRows - 1) / G::kRows), G::kThreads, 0, st>>>(a);
-  });
+  };
+  return wide ? with_row_shape<false>(a.cols / N, a.rows, [&](auto s) { go(s, std::integral_constant<int, N>{}); })
+              : with_value_shape(a.cols, [&](auto s) { go(s, std::integral_constant<int, 1>{}); });
 }
 
 template <typename T, int kAct, bool kSym>

@@ -106,37 +106,39 @@ __global__ void __launch_bounds__(kThreads) norm_any_kernel(NormArgs a) {
   }
 }
 
-// Rows that registers hold, 16-byte aligned: x, the residual and the gate are read once, h and y written once; the
+// Rows that registers hold, by 16-byte vectors or (not aligned) by single values: x, the residual and the gate are read once, h and y written once; the
 // weights come from the caches.  HBM-bound: 32768 x 4096 in bf16 with both norms and a gate takes 167 us, 6.4 TB/s or 98 %
 // of a copy's rate.  A lane keeps its vectors as they lie in memory (x, then h) and unpacks them where it needs them: the
 // registers of fp32 copies cost wide rows their occupancy (2048 x 16384 with two inputs: 84 us, 51 this way).
-template <typename T, int kWarps, int kVecs>
+template <typename T, int N, int kWarps, int kVecs>
 __global__ void __launch_bounds__(RowGroup<kWarps>::kThreads) norm_rows_kernel(NormArgs a) {
   using G = RowGroup<kWarps>;
-  using E = Elem<T>;
-  constexpr int N = E::kPerVec;
+  using P = Raw<T, N>;
   __shared__ float red[4 * kWarps];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // see the integer product
   const int64_t row = (int64_t)blockIdx.x * G::kRows + G::row();
   if (G::kRows > 1 && row >= a.rows) return;                           // a whole warp, and no barrier follows
   const int vecs = (int)(a.cols / N);
   const float inv_c = 1.f / (float)a.cols;
-  const uint4* x = reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + row * a.ldx);
-  const uint4* res = a.residual ? reinterpret_cast<const uint4*>(static_cast<const T*>(a.residual) + row * a.ldr) : nullptr;
-  const uint4* gate =
-      a.gate ? reinterpret_cast<const uint4*>(static_cast<const T*>(a.gate) + row / a.rows_per_gate * a.cols) : nullptr;
-  const uint4* pw = static_cast<const uint4*>(a.post_weight);
-  const uint4* w = static_cast<const uint4*>(a.weight);
-  uint4 kept[kVecs], rr[kVecs];
+  const T* x = static_cast<const T*>(a.x) + row * a.ldx;
+  const T* res = a.residual ? static_cast<const T*>(a.residual) + row * a.ldr : nullptr;
+  const P* gate = a.gate ? reinterpret_cast<const P*>(static_cast<const T*>(a.gate) + row / a.rows_per_gate * a.cols) : nullptr;
+  const P* pw = static_cast<const P*>(a.post_weight);
+  const P* w = static_cast<const P*>(a.weight);
+  P kept[kVecs], rr[kVecs];
 #pragma unroll
   for (int k = 0; k < kVecs; ++k) {
     const int i = G::lane() + k * G::kLanes;
-    kept[k] = i < vecs ? __ldcs(x + i) : make_uint4(0u, 0u, 0u, 0u);
-    if (res) rr[k] = i < vecs ? __ldcs(res + i) : make_uint4(0u, 0u, 0u, 0u);
+    if (i < vecs) {
+      kept[k] = load_stream<T, N>(x + i * N);
+      if (res) rr[k] = load_stream<T, N>(res + i * N);
+    } else {
+      kept[k] = pack<T, N>({});
+    }
   }
   auto squares = [&](int k) {
     float v[N], s = 0.f;
-    unpack16<T>(kept[k], v);
+    unpack<T, N>(kept[k], v);
 #pragma unroll
     for (int j = 0; j < N; ++j) s = fmaf(v[j], v[j], s);
     return s;
@@ -149,27 +151,27 @@ __global__ void __launch_bounds__(RowGroup<kWarps>::kThreads) norm_rows_kernel(N
       for (int k = 0; k < kVecs; ++k) s += squares(k);
       post = rsqrtf(G::sum(s, red) * inv_c + a.eps);
     }
-    uint4* h = reinterpret_cast<uint4*>(static_cast<T*>(a.h) + row * a.cols);
+    P* h = reinterpret_cast<P*>(static_cast<T*>(a.h) + row * a.cols);
 #pragma unroll
     for (int k = 0; k < kVecs; ++k) {
       const int i = G::lane() + k * G::kLanes;
       if (i < vecs) {
         float v[N], f[N];
-        unpack16<T>(kept[k], v);
+        unpack<T, N>(kept[k], v);
         if (pw) {
-          unpack16<T>(__ldg(pw + i), f);
+          unpack<T, N>(__ldg(pw + i), f);
 #pragma unroll
           for (int j = 0; j < N; ++j) v[j] = v[j] * post * (f[j] + a.offset);
         }
         if (gate) {
-          unpack16<T>(__ldg(gate + i), f);
+          unpack<T, N>(__ldg(gate + i), f);
 #pragma unroll
           for (int j = 0; j < N; ++j) v[j] *= f[j];
         }
-        if (res) unpack16<T>(rr[k], f);
-        T* p = reinterpret_cast<T*>(&kept[k]);
+        if (res) unpack<T, N>(rr[k], f);
 #pragma unroll
-        for (int j = 0; j < N; ++j) p[j] = E::from_f(res ? v[j] * a.scale + f[j] : v[j] * a.scale);
+        for (int j = 0; j < N; ++j) v[j] = res ? v[j] * a.scale + f[j] : v[j] * a.scale;
+        kept[k] = pack<T, N>(v);
         h[i] = kept[k];
       }
     }
@@ -181,24 +183,20 @@ __global__ void __launch_bounds__(RowGroup<kWarps>::kThreads) norm_rows_kernel(N
   const float pre = rsqrtf(G::sum(s, red + kWarps) * inv_c + a.eps);
   auto normed = [&](int k, int i, float (&v)[N]) {
     float f[N];
-    unpack16<T>(kept[k], v);
-    unpack16<T>(__ldg(w + i), f);
+    unpack<T, N>(kept[k], v);
+    unpack<T, N>(__ldg(w + i), f);
 #pragma unroll
     for (int j = 0; j < N; ++j) v[j] = v[j] * pre * (f[j] + a.offset);
   };
   if (a.y) {
-    uint4* y = reinterpret_cast<uint4*>(static_cast<T*>(a.y) + row * a.cols);
+    P* y = reinterpret_cast<P*>(static_cast<T*>(a.y) + row * a.cols);
 #pragma unroll
     for (int k = 0; k < kVecs; ++k) {
       const int i = G::lane() + k * G::kLanes;
       if (i < vecs) {
         float v[N];
         normed(k, i, v);
-        uint4 o;
-        T* p = reinterpret_cast<T*>(&o);
-#pragma unroll
-        for (int j = 0; j < N; ++j) p[j] = E::from_f(v[j]);
-        y[i] = o;
+        y[i] = pack<T, N>(v);
       }
     }
   }
@@ -237,17 +235,19 @@ __global__ void __launch_bounds__(RowGroup<kWarps>::kThreads) norm_rows_kernel(N
 template <typename T>
 bool launch_rows(const NormArgs& a, cudaStream_t st) {
   constexpr int N = Elem<T>::kPerVec;
-  if (a.cols % N || (a.rows > 1 && (a.ldx % N || (a.residual && a.ldr % N) || (a.codes && a.ldc % N))) ||
-      a.rows > 0x7fffffff ||
-      (reinterpret_cast<uintptr_t>(a.codes) & (N - 1)))
-    return false;
+  if (a.rows > 0x7fffffff) return false;
+  bool wide = a.cols % N == 0 && (a.rows == 1 || (a.ldx % N == 0 && (!a.residual || a.ldr % N == 0) && (!a.codes || a.ldc % N == 0))) &&
+              (reinterpret_cast<uintptr_t>(a.codes) & (N - 1)) == 0;
   for (const void* p : {a.x, a.residual, a.post_weight, a.gate, a.weight, (const void*)a.h, (const void*)a.y})
-    if (!aligned16(p)) return false;                                   // NULL counts as aligned
-  return with_row_shape<true>(a.cols / N, a.rows, [&](auto shape) {
+    wide = wide && aligned16(p);                                       // NULL counts as aligned
+  auto go = [&](auto shape, auto width) {
     using S = decltype(shape);
     using G = RowGroup<S::kWarps>;
-    norm_rows_kernel<T, S::kWarps, S::kVecs><<<(unsigned)((a.rows + G::kRows - 1) / G::kRows), G::kThreads, 0, st>>>(a);
-  });
+    norm_rows_kernel<T, decltype(width)::value, S::kWarps, S::kVecs>
+        <<<(unsigned)((a.rows + G::kRows - 1) / G::kRows), G::kThreads, 0, st>>>(a);
+  };
+  return wide ? with_row_shape<true>(a.cols / N, a.rows, [&](auto s) { go(s, std::integral_constant<int, N>{}); })
+              : with_value_shape(a.cols, [&](auto s) { go(s, std::integral_constant<int, 1>{}); });
 }
 
 template <typename T>

@@ -129,9 +129,13 @@ __device__ __forceinline__ RowQuant row_quant_of(float mn, float mx, bool sym) {
   return sym ? row_quant<true>(0.f, nan_max(mx, -mn)) : row_quant<false>(mn, mx);
 }
 
-// the codes of N (4 or 8) neighbouring values, stored at p (N-byte aligned)
+// the codes of N (1, 4 or 8) neighbouring values, stored at p (N-byte aligned)
 template <int N>
 __device__ __forceinline__ void store_row_codes(int8_t* p, const float (&v)[N], const RowQuant& q, bool sym) {
+  if constexpr (N == 1) {
+    *p = q.bad ? (int8_t)0 : (int8_t)(sym ? row_code<true>(v[0], q) : row_code<false>(v[0], q));
+    return;
+  } else {
   uint32_t w[N / 4];
 #pragma unroll
   for (int j = 0; j < N / 4; ++j) {
@@ -147,6 +151,7 @@ __device__ __forceinline__ void store_row_codes(int8_t* p, const float (&v)[N], 
   }
   if (N == 4) *reinterpret_cast<uint32_t*>(p) = w[0];
   else *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[N / 4 - 1]);
+  }
 }
 
 template <typename T>
@@ -154,6 +159,35 @@ __device__ __forceinline__ void unpack16(const uint4& v, float (&f)[Elem<T>::kPe
   const T* p = reinterpret_cast<const T*>(&v);
 #pragma unroll
   for (int i = 0; i < Elem<T>::kPerVec; ++i) f[i] = Elem<T>::to_f(p[i]);
+}
+
+// N neighbouring values as they lie in memory: a 16-byte vector, held as four whole registers, or one value where rows are
+// not aligned to more (a warp still reads 64 or 128 contiguous bytes at once).
+template <typename T, int N> struct RawOf { typedef uint4 type; };
+template <typename T> struct RawOf<T, 1> { typedef T type; };
+template <typename T, int N> using Raw = typename RawOf<T, N>::type;
+
+template <typename T, int N>
+__device__ __forceinline__ Raw<T, N> load_stream(const T* p) {             // read once
+  if constexpr (N == 1) return *p;
+  else return __ldcs(reinterpret_cast<const uint4*>(p));
+}
+template <typename T, int N>
+__device__ __forceinline__ void unpack(const Raw<T, N>& r, float (&f)[N]) {
+  if constexpr (N == 1) f[0] = Elem<T>::to_f(r);
+  else unpack16<T>(r, f);
+}
+template <typename T, int N>
+__device__ __forceinline__ Raw<T, N> pack(const float (&f)[N]) {
+  if constexpr (N == 1) {
+    return Elem<T>::from_f(f[0]);
+  } else {
+    uint4 r;
+    T* p = reinterpret_cast<T*>(&r);
+#pragma unroll
+    for (int i = 0; i < N; ++i) p[i] = Elem<T>::from_f(f[i]);
+    return r;
+  }
 }
 
 // Which kernel holds rows of `vecs` 16-byte vectors: f(RowShape<warps of a row, vectors a lane>); false where none does.
@@ -181,6 +215,18 @@ bool with_row_shape(int64_t vecs, int64_t rows, F&& f) {
   else if (vecs <= 2048 && kNorm) f(RowShape<8, 8>{});
   else if (vecs <= 2048) f(RowShape<16, 4>{});
   else if (vecs <= 4096) f(RowShape<16, 8>{});
+  else return false;
+  return true;
+}
+// the same for rows of single values
+template <typename F>
+bool with_value_shape(int64_t cols, F&& f) {
+  if (cols <= 128) f(RowShape<1, 4>{});
+  else if (cols <= 512) f(RowShape<1, 16>{});
+  else if (cols <= 2048) f(RowShape<4, 16>{});
+  else if (cols <= 4096) f(RowShape<8, 16>{});
+  else if (cols <= 8192) f(RowShape<16, 16>{});
+  else if (cols <= 16384) f(RowShape<16, 32>{});
   else return false;
   return true;
 }
