@@ -105,6 +105,30 @@ constexpr int kRows = 128, kBlockK = 128, kStreamThreads = 256;
 constexpr int kWeightBytes = kRows * kBlockK;
 constexpr int kSmemMost = 227 * 1024;
 
+// Bounded wait, asleep in the hardware between looks (up to 20 us each) instead of spinning: at the power limit that is
+// 1.5 % of a large product.  False if a second has passed or another role has given up.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  auto look = [&] {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(20000u)
+        : "memory");
+    return ok != 0;
+  };
+  if (look()) return true;
+  uint64_t begin, now;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(begin));
+  do {
+    if (look()) return true;
+    if (*abort_flag) return false;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+  } while (now - begin < 1000000000ull);
+  *abort_flag = 1;
+  return false;
+}
+
 // kind::i8: D s32, A and B s8, both K-major
 __host__ __device__ constexpr uint32_t idesc_i8(int m, int n) {
   return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
@@ -326,7 +350,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
       uint32_t ph = 0;
       issued = min(stages, count);
       for (int i = stages; i < count; ++i) {
-        if (!mbar_wait(empty_bar(s), ph, abort_flag)) break;
+        if (!bar_wait(empty_bar(s), ph, abort_flag)) break;
         mbar_expect_tx(full_bar(s), kStage);
         tma_load_2d(base + s * kStage, &maps.w, (kb0 + i) * kBlockK, n0, full_bar(s));
         if (!kQuant) tma_load_2d(base + s * kStage + kWeightBytes, &maps.x, (kb0 + i) * kBlockK, m0, full_bar(s));
@@ -343,7 +367,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
     const uint64_t dw0 = make_desc_mn_sw128(base, 16, 1024);
     const uint64_t dx0 = make_desc_mn_sw128(base + (kQuant ? Smem::codes(stages) : kWeightBytes), 16, 1024);
     for (int i = 0; i < count; ++i) {
-      if (!mbar_wait(full_bar(s), ph, abort_flag)) break;
+      if (!bar_wait(full_bar(s), ph, abort_flag)) break;
       tcgen05_fence_after();
       const uint64_t at = (uint64_t)(s * (kStage >> 4)), xat = kQuant ? (uint64_t)(i * (NT * kBlockK >> 4)) : at;
       if (elect_one()) {
@@ -359,10 +383,8 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
   }
   __syncwarp();
   // the accumulator (or, after an expired wait, the retirement of what was issued)
-  for (uint32_t it = 0; !mbar_test(acc_bar, 0); ++it) {
-    if (it >= 2 * kSpinLimit) { *abort_flag = 1; break; }
-    if (it >= 64) __nanosleep(50);
-  }
+  if (!bar_wait(acc_bar, 0, abort_flag))
+    for (uint32_t it = 0; it < kSpinLimit && !mbar_test(acc_bar, 0); ++it) __nanosleep(50);
   tcgen05_fence_after();
   __syncthreads();
   bool ok = *abort_flag == 0;
@@ -412,7 +434,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
                     base + (uint32_t)(from * kRows * 4), (uint32_t)(many * kRows * 4), in_cta(land_bar, lane));
     }
     __syncwarp();
-    if (mine > 0) ok = mbar_wait(land_bar, 0, abort_flag) && ok;
+    if (mine > 0) ok = bar_wait(land_bar, 0, abort_flag) && ok;
     __syncwarp();
     cluster_arrive();                                      // what was sent here is here
     const uint32_t* own = part + first * kRows + c;
@@ -564,7 +586,7 @@ pair_kernel(const __grid_constant__ Maps maps, Int8Args g, PairTiles pt) {
         origin(t, n0, m0);
         n0 += (int)rank * 128, m0 += (int)rank * 128;
         for (int kb = 0; kb < blocks; ++kb) {
-          if (!mbar_wait(empty_bar(s), ph, abort_flag)) { ok = false; break; }
+          if (!bar_wait(empty_bar(s), ph, abort_flag)) { ok = false; break; }
           const uint32_t sa = base + s * kPairStageBytes;
           if (rank == 0) mbar_expect_tx(full_bar(s), 2 * kPairStageBytes);
           tma_load_pair(sa, &maps.w, kb * kBlockK, n0, full0 + 8u * s);
@@ -582,11 +604,11 @@ pair_kernel(const __grid_constant__ Maps maps, Int8Args g, PairTiles pt) {
       bool ok = true;
       const uint64_t dw0 = make_desc_mn_sw128(base, 16, 1024), dx0 = make_desc_mn_sw128(base + kHalfBytes, 16, 1024);
       for (int t = pair; ok && t < tiles; t += pairs) {
-        if (!mbar_wait(acc_empty(buf), aph, abort_flag)) break;
+        if (!bar_wait(acc_empty(buf), aph, abort_flag)) break;
         tcgen05_fence_after();
         const uint32_t acc = tmem + (uint32_t)(buf * kPairTokens);
         for (int kb = 0; kb < blocks; ++kb) {
-          if (!mbar_wait(full_bar(s), ph, abort_flag)) { ok = false; break; }
+          if (!bar_wait(full_bar(s), ph, abort_flag)) { ok = false; break; }
           tcgen05_fence_after();
           const uint64_t at = (uint64_t)(s * (kPairStageBytes >> 4));
           if (elect_one()) {
@@ -629,7 +651,7 @@ pair_kernel(const __grid_constant__ Maps maps, Int8Args g, PairTiles pt) {
       }
       __syncwarp();
       // once a wait has expired, the tiles that remain are written as NaN
-      ok = ok && mbar_wait(acc_full(buf), aph, abort_flag) && *abort_flag == 0;
+      ok = ok && bar_wait(acc_full(buf), aph, abort_flag) && *abort_flag == 0;
       tcgen05_fence_after();
       const uint32_t taddr = tmem + (uint32_t)(buf * kPairTokens + h * 128) + ((uint32_t)(q * 32) << 16);
       T* out = static_cast<T*>(g.c) + (int64_t)mt * g.N + n;

@@ -58,7 +58,10 @@ def _float_rows(name, x):
 def _codes_like(x2, rows, cols, sym):
     """Room for the codes (rows 16 bytes apart or a multiple of that, as the products read them), scales, zeros."""
     pitch = (cols + 15) & -16
-    codes = x2.new_empty((rows, pitch), dtype=torch.int8)
+    if pitch == cols and x2.dim() == 2 and x2.is_contiguous():
+        codes = torch.empty_like(x2, dtype=torch.int8)
+    else:
+        codes = x2.new_empty((rows, pitch), dtype=torch.int8)
     scales = x2.new_empty((rows, 1), dtype=torch.float32)
     return codes, pitch, scales, None if sym else x2.new_empty((rows, 1), dtype=torch.int32)
 
