@@ -103,16 +103,18 @@ __global__ void __launch_bounds__(RowGroup<kWarps>::kThreads) quant_rows_kernel(
 #pragma unroll
   for (int k = 0; k < kVecs; ++k) {
     const int i = G::lane() + k * G::kLanes;
-    if (i < vecs) {
+    if constexpr (!kGated) {
+      rx[k] = i < vecs ? load_stream<T, N>(x + i * N) : pack<T, N>({});
+    } else if (i < vecs) {                                             // a vector that is not there costs no activation
       rx[k] = load_stream<T, N>(x + i * N);
-      if (kGated) ru[k] = load_stream<T, N>(u + i * N);
+      ru[k] = load_stream<T, N>(u + i * N);
     }
   }
   float v[kVecs][N];
   float mn = 0.f, mx = 0.f;
 #pragma unroll
   for (int k = 0; k < kVecs; ++k) {
-    if (G::lane() + k * G::kLanes < vecs) {
+    if (!kGated || G::lane() + k * G::kLanes < vecs) {
       unpack<T, N>(rx[k], v[k]);
       if (kGated) {
         float w[N];

@@ -129,12 +129,8 @@ __global__ void __launch_bounds__(RowGroup<kWarps>::kThreads) norm_rows_kernel(N
 #pragma unroll
   for (int k = 0; k < kVecs; ++k) {
     const int i = G::lane() + k * G::kLanes;
-    if (i < vecs) {
-      kept[k] = load_stream<T, N>(x + i * N);
-      if (res) rr[k] = load_stream<T, N>(res + i * N);
-    } else {
-      kept[k] = pack<T, N>({});
-    }
+    kept[k] = i < vecs ? load_stream<T, N>(x + i * N) : pack<T, N>({});
+    if (res) rr[k] = i < vecs ? load_stream<T, N>(res + i * N) : pack<T, N>({});
   }
   auto squares = [&](int k) {
     float v[N], s = 0.f;
