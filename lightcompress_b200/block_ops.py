@@ -354,6 +354,8 @@ def rotary_embed(q, k, positions, inv_freq, interleaved=False, attention_scale=1
     dev = q.get_device()
     if not (positions.get_device() == inv_freq.get_device() == dev) or (k is not None and k.get_device() != dev):
         L.refuse_devices(name, q, k=k, positions=positions, inv_freq=inv_freq)
+    if inplace and k is not None and k.data_ptr() == q.data_ptr() and k.numel():
+        raise ValueError(f'{name}: cannot work in place on one tensor as q and k')
     q, q_out, qb, qh, qt = _heads(name, q, B, H, T, D, inplace)
     if k is None:
         k_out, k_at, ko_at, kb, kh, kt = None, 0, 0, 0, 0, 0
@@ -405,8 +407,9 @@ def rope_frequencies(rotary_dim, base=10000.0, scaling=None, seq_len=None, devic
         # the base grows with the sequence once it is longer than what the model was trained on
         trained = s['original_max_position_embeddings']
         length = max(seq_len or 0, trained)
-        grown = base * (s['factor'] * length / trained - (s['factor'] - 1)) ** (rotary_dim / (rotary_dim - 2))
-        inv = float(grown) ** -expo
+        if rotary_dim > 2:      # a single pair turns once a position, whatever the base
+            grown = base * (s['factor'] * length / trained - (s['factor'] - 1)) ** (rotary_dim / (rotary_dim - 2))
+            inv = float(grown) ** -expo
     elif kind == 'llama3':
         # wave lengths beyond the trained context are stretched, short ones kept, the ones between blended
         turns = s['original_max_position_embeddings'] * inv / (2 * math.pi)     # turns within the trained context

@@ -434,7 +434,11 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
                     base + (uint32_t)(from * kRows * 4), (uint32_t)(many * kRows * 4), in_cta(land_bar, lane));
     }
     __syncwarp();
-    if (mine > 0) ok = bar_wait(land_bar, 0, abort_flag) && ok;
+    if (mine > 0 && !bar_wait(land_bar, 0, abort_flag)) {
+      // what the others sent lands all the same before this CTA's memory is released
+      ok = false;
+      for (uint32_t it = 0; it < kSpinLimit && !mbar_test(land_bar, 0); ++it) __nanosleep(50);
+    }
     __syncwarp();
     cluster_arrive();                                      // what was sent here is here
     const uint32_t* own = part + first * kRows + c;
@@ -734,7 +738,8 @@ Choice choose(int64_t M, int64_t N, int64_t K) {
   if (M <= 128) least = 1e30f;
   for (int i = 0; i < 4; ++i) {
     if (i > 0 && kNT[i - 1] >= M) break;                   // half of the tile's tokens would not exist
-    const int64_t tiles = n_tiles * ((M + kNT[i] - 1) / kNT[i]);
+    const int64_t m_tiles = (M + kNT[i] - 1) / kNT[i], tiles = n_tiles * m_tiles;
+    if (m_tiles > 65535) continue;                         // a grid's second dimension
     for (int sp : kSplits) {
       const int64_t ctas = tiles * sp, count = (blocks + sp - 1) / sp;
       if (sp > 1 && (sp > blocks || ctas > (kNT[i] == 128 ? 1 : 2) * ctas_at_once(sp))) break;
@@ -765,7 +770,6 @@ cudaError_t allow_smem(F* kernel) {
 template <typename T, int NT, bool kQuant = false>
 int launch_stream(const Int8Args& g, int splits, bool dependent, cudaStream_t st) {
   const int n_tiles = (g.N + kRows - 1) / kRows, m_tiles = (g.M + NT - 1) / NT;
-  if (m_tiles > 65535) return LC_ERR_SHAPE;
   const int blocks = (g.K + kBlockK - 1) / kBlockK;
   const int per_sm = (int64_t)n_tiles * m_tiles * splits > ctas_at_once(splits) ? 2 : 1;
   using Smem = StreamSmem<NT, kQuant>;

@@ -148,6 +148,18 @@ def test_product_is_exact(m, n, k):
                                      torch.float32).cpu(), ref.int8_product(a, a_s, b, bs, None, a_z))
 
 
+def test_more_tokens_than_a_grid_dimension_holds():
+    """More 128-token tiles than 65535, of few channels: every row of the output against the exact sums."""
+    from lightcompress_b200.int8_linear import int8_gemm
+    m, n, k = 128 * 65536 + 77, 8, 16
+    g = torch.Generator(device='cuda').manual_seed(1)
+    a = torch.randint(-128, 128, (m, k), generator=g, dtype=torch.int8, device='cuda')
+    b = torch.randint(-128, 128, (n, k), generator=g, dtype=torch.int8, device='cuda')
+    one = torch.ones(m, device='cuda')
+    c = int8_gemm(a, one, b, one[:n], out_dtype=torch.float32)
+    assert torch.equal(c, a.float() @ b.float().t())            # sums below 2^24: exact in fp32
+
+
 @pytest.mark.parametrize('m', [1, 20, 300])
 def test_largest_sums(m):
     """Sums at the ends of 32 bits: all codes -128, with and without a zero point at the other end."""

@@ -95,6 +95,8 @@ def test_views_of_one_projection_and_in_place(dtype, inter):
     contiguous = torch.randn(b, h, t, d, device='cuda').to(dtype)   # heads before tokens in memory
     oq, _ = rotary_embed(contiguous, None, pos.cuda(), freq.cuda(), inter)
     _check(oq, contiguous.cpu(), pos, freq, inter, 1.0)
+    with pytest.raises(ValueError, match='one tensor'):
+        rotary_embed(contiguous, contiguous[:, :1], pos.cuda(), freq.cuda(), inter, inplace=True)
     with pytest.raises(ValueError, match='expanded'):
         rotary_embed(contiguous[:1].expand(2, h, t, d), None, pos.cuda(), freq.cuda(), inter, inplace=True)
 

@@ -249,3 +249,72 @@ def test_rope_frequencies_against_transformers(kind, section):
     assert got.dtype == torch.float32 and got.shape == (dim // 2,)
     assert math.isclose(scale, want_scale, rel_tol=1e-6)
     assert torch.allclose(got, want.float(), rtol=1e-5, atol=0)
+
+
+def test_rope_frequencies_of_a_single_pair():
+    from lightcompress_b200.block_ops import rope_frequencies
+    for kind in ('default', 'dynamic'):
+        inv, _ = rope_frequencies(2, scaling={'rope_type': kind, 'factor': 2.0, 'original_max_position_embeddings': 8}, seq_len=20,
+                                  device='cpu')
+        assert inv.tolist() == [1.0]
+
+
+def test_launches_on_the_tensors_device_and_leaves_the_current_one(monkeypatch):
+    """The device and stream that a call is given, against fakes of the library and of torch's device functions."""
+    import contextlib
+    from lightcompress_b200 import _lib as L
+    seen, current = [], [0]
+
+    @contextlib.contextmanager
+    def device(d):
+        before, current[0] = current[0], d
+        try:
+            yield
+        finally:
+            current[0] = before
+
+    class Lib:
+        code = 0
+
+        def lc_set_device(self, d):
+            seen.append(('device', d))
+            return 0
+
+        def lc_thing(self, *args):
+            seen.append(('call', current[0], args))
+            return self.code
+
+        def lc_status_string(self, code):
+            return b'fake'
+    lib = Lib()
+    monkeypatch.setattr(L, 'lib', lib)
+    monkeypatch.setattr(torch.cuda, 'current_device', lambda: current[0])
+    monkeypatch.setattr(torch.cuda, 'device', device)
+    monkeypatch.setattr(L, '_raw_stream', lambda d: 100 + d)
+    L.launch(0, 'lc_thing', b'x')
+    assert seen == [('device', 0), ('call', 0, (b'x', 100))]
+    seen.clear()
+    L.launch(3, 'lc_thing', b'x')
+    assert seen == [('device', 3), ('call', 3, (b'x', 103)), ('device', 0)] and current == [0]
+    seen.clear()
+    lib.code = L.LC_ERR_SHAPE
+    with pytest.raises(L.LcError, match='lc_thing failed'):
+        L.launch(3, 'lc_thing')
+    assert seen[-1] == ('device', 0) and current == [0]
+    with pytest.raises(RuntimeError, match='no CPU path'):
+        L.launch(-1, 'lc_thing')
+
+
+def test_an_expired_wait_is_reported_once(monkeypatch):
+    """check_status on a status word that a kernel would have written."""
+    from lightcompress_b200 import _lib as L
+    from lightcompress_b200 import int8_linear as il
+    word = torch.zeros(1, dtype=torch.int32)
+    monkeypatch.setattr(torch.cuda, 'synchronize', lambda d=None: None)
+    monkeypatch.setattr(il, '_status', {0: word})
+    il.check_status('cuda:0')
+    word.fill_(L.LC_ERR_TIMEOUT)
+    with pytest.raises(L.LcError, match='timed out'):
+        il.check_status(0)
+    il.check_status(0)
+    il.check_status(1)          # a device that has run no product
