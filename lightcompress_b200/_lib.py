@@ -170,7 +170,8 @@ def call(name, *args):
     check(name, getattr(lib, name)(*args))
 
 
-# the handle of torch's current stream on a device, without making a Stream object of it
+# the current device and the handle of torch's current stream on a device, without the checks and objects around them
+_current_device = getattr(torch._C, '_cuda_getDevice', torch.cuda.current_device)
 _raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', lambda dev: torch.cuda.current_stream(dev).cuda_stream)
 
 
@@ -179,7 +180,7 @@ def launch(dev, name, *args):
     device is current; the caller's current device is what it was afterwards.  Tensors without a device end here."""
     if dev < 0:
         raise RuntimeError('lightcompress_b200 kernels need CUDA tensors; there is no CPU path')
-    cur = torch.cuda.current_device()
+    cur = _current_device()
     if dev == cur:
         lib.lc_set_device(dev)
         code = getattr(lib, name)(*args, _raw_stream(dev))

@@ -217,11 +217,17 @@ def int8_dynamic_forward_func(x, w, w_scale, bias=None, w_sum=None):
     if not (w.get_device() == w_scale.get_device() == dev) or (bias is not None and bias.get_device() != dev) \
             or (not sym and w_sum.get_device() != dev):
         L.refuse_devices(name, x, w=w, w_scale=w_scale, bias=bias, w_sum=w_sum)
-    c = x2.new_empty((M, N))
+    dense = x2.is_contiguous()
+    c = torch.empty_like(x2) if dense and N == K else x2.new_empty((M, N))      # half the time, where it fits
     if M and N:
         # lc_int8_linear_scratch(M, K)
         room = 0 if M == 1 and K <= 4096 else M * (((K + 15) & -16) + 8)
-        scratch = x2.new_empty(room, dtype=torch.int8) if room else None
+        if room == 0:
+            scratch = None
+        elif dense and K >= 32 and room <= 1 << 20:
+            scratch = torch.empty_like(x2)                # 2 K bytes a token at least: enough
+        else:
+            scratch = x2.new_empty(room, dtype=torch.int8)
         L.launch(dev, 'lc_int8_linear', L.INT8_LINEAR.pack(
             x2.data_ptr(), dt, x2.stride()[0], w.data_ptr(), _pitch(w, N, K), w_scale.data_ptr(), 0 if sym else w_sum.data_ptr(),
             0 if bias is None else bias.data_ptr(), M, N, K, sym, c.data_ptr(), scratch.data_ptr() if room else 0, room,

@@ -288,7 +288,7 @@ def test_launches_on_the_tensors_device_and_leaves_the_current_one(monkeypatch):
             return b'fake'
     lib = Lib()
     monkeypatch.setattr(L, 'lib', lib)
-    monkeypatch.setattr(torch.cuda, 'current_device', lambda: current[0])
+    monkeypatch.setattr(L, '_current_device', lambda: current[0])
     monkeypatch.setattr(torch.cuda, 'device', device)
     monkeypatch.setattr(L, '_raw_stream', lambda d: 100 + d)
     L.launch(0, 'lc_thing', b'x')
