@@ -605,6 +605,22 @@ def kernel_case(name, n):
         for _ in range(n):
             a, a_s = act_quant(x)
             fp8_gemm(a, a_s, wq, ws)
+    elif name == 'w8a8':                              # operators of a deployed W8A8 block on 2048 tokens of a 7B layer
+        from lightcompress_b200 import block_ops as B
+        from lightcompress_b200 import int8_linear as I
+        g = torch.Generator().manual_seed(10)
+        x, res = (torch.randn(2048, 4096, generator=g).to(torch.bfloat16).cuda() for _ in range(2))
+        gate, up = (torch.randn(2048, 11008, generator=g).to(torch.bfloat16).cuda() for _ in range(2))
+        norm = torch.ones(4096, dtype=torch.bfloat16, device='cuda')
+        w, s = (torch.randint(-127, 128, (4096, 11008), generator=g, dtype=torch.int8).cuda(), torch.full((4096,), 1e-3).cuda())
+        q = x.view(1, 2048, 32, 128).transpose(1, 2)
+        pos, (freq, _) = torch.arange(2048, device='cuda'), B.rope_frequencies(128)
+        for _ in range(n):
+            B.residual_norm(x, res, weight=norm, post_weight=norm)
+            B.residual_norm(x, res, weight=norm, quant=True)
+            B.rotary_embed(q, q, pos, freq)
+            I.int8_gemm(*I.gated_act_quant(gate, up), w, s)
+            I.int8_dynamic_forward_func(x[:1], w[:, :4096], s)
     elif name == 'mse':                               # MSE range search, W4 asym g128, 8192 x 4096 fp32
         g = torch.Generator().manual_seed(9)
         w = (torch.randn(8192, 4096, generator=g) * 0.02).cuda()
@@ -701,7 +717,7 @@ def kernel_case(name, n):
 
 
 KERNEL_CASES = ['hessian', 'hessian_wide', 'rtn', 'fp8', 'gptq', 'gptq_wide', 'factor', 'factor_wide', 'factor_cusolver', 'block_ops',
-                'fp8_linear', 'mse', 'awq_clip', 'act_static', 'quik', 'w48', 'spqr']
+                'fp8_linear', 'mse', 'awq_clip', 'act_static', 'quik', 'w48', 'spqr', 'w8a8']
 
 
 # ---- parity of the timed configuration (outside the timed region) --------------------------------------

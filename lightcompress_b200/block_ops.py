@@ -293,14 +293,14 @@ def residual_norm(x, residual=None, weight=None, post_weight=None, gate=None, sc
     y = codes = scales = zeros = None
     pitch = 0
     if quant:
-        codes, pitch, scales, zeros = int8_linear._codes_like(x, rows, C, sym)
+        codes, pitch, scales, zeros, quantised = int8_linear._codes_like(x, shape, sym)
     elif weight is not None:
         y = torch.empty_like(x) if contiguous else x.new_empty(shape)
     if rows:
         L.launch(dev, 'lc_residual_norm', L.RESIDUAL_NORM.pack(
             x2.data_ptr(), _at(r2), _at(post_weight), _at(gate), gate_rows, _at(weight), dt, rows, C, ldx, ldr, scale, eps,
             weight_offset, 0 if kept else h.data_ptr(), _at(y), _at(codes), pitch, _at(scales), _at(zeros)))
-    return h, int8_linear._shaped(codes, scales, zeros, shape) if quant else y
+    return h, quantised if quant else y
 
 
 def _refuse_operand(name, key, t, x, shape):

@@ -55,26 +55,20 @@ def _float_rows(name, x):
     return (x if x.dim() == 2 else x.reshape(-1, x.shape[-1])), dt
 
 
-def _codes_like(x2, rows, cols, sym):
-    """Room for the codes (rows 16 bytes apart or a multiple of that, as the products read them), scales, zeros."""
-    pitch = (cols + 15) & -16
-    if pitch == cols and x2.dim() == 2 and x2.is_contiguous():
-        codes = torch.empty_like(x2, dtype=torch.int8)
-    else:
-        codes = x2.new_empty((rows, pitch), dtype=torch.int8)
-    scales = x2.new_empty((rows, 1), dtype=torch.float32)
-    return codes, pitch, scales, None if sym else x2.new_empty((rows, 1), dtype=torch.int32)
-
-
-def _shaped(codes, scales, zeros, shape):
+def _codes_like(x, shape, sym):
+    """Room for the codes of a tensor of `shape` (rows 16 bytes apart or a multiple of that, as the products read them),
+    scales, zeros; and what the caller returns of it."""
     cols = shape[-1]
-    if codes.shape[1] != cols:
-        codes = codes[:, :cols]
-    if len(shape) != 2:
-        codes = codes.unflatten(0, shape[:-1]) if len(shape) > 2 else codes[0]
-        scales = scales.reshape(*shape[:-1], 1)
-        zeros = None if zeros is None else zeros.reshape(*shape[:-1], 1)
-    return (codes, scales) if zeros is None else (codes, scales, zeros)
+    pitch = (cols + 15) & -16
+    lead = shape[:-1]
+    if pitch == cols and x.shape == shape and x.is_contiguous():
+        codes = torch.empty_like(x, dtype=torch.int8)
+    else:
+        codes = x.new_empty((*lead, pitch), dtype=torch.int8)
+    scales = x.new_empty((*lead, 1), dtype=torch.float32)
+    zeros = None if sym else x.new_empty((*lead, 1), dtype=torch.int32)
+    seen = codes if pitch == cols else codes[..., :cols]
+    return codes, pitch, scales, zeros, (seen, scales) if sym else (seen, scales, zeros)
 
 
 def act_quant(x, sym=True):
@@ -86,11 +80,11 @@ def act_quant(x, sym=True):
         L.refuse_grad('act_quant')
     x2, dt = _float_rows('act_quant', x)
     rows, cols = x2.shape
-    codes, pitch, scales, zeros = _codes_like(x2, rows, cols, sym)
+    codes, pitch, scales, zeros, out = _codes_like(x, x.shape, sym)
     if rows:
         L.launch(x2.get_device(), 'lc_int8_act_quant', x2.data_ptr(), dt, rows, cols, x2.stride()[0], codes.data_ptr(), pitch,
                  scales.data_ptr(), None if sym else zeros.data_ptr())
-    return _shaped(codes, scales, zeros, x.shape)
+    return out
 
 
 def gated_act_quant(gate, up, act='silu', sym=True):
@@ -110,11 +104,11 @@ def gated_act_quant(gate, up, act='silu', sym=True):
     g2, dt = _float_rows('gated_act_quant', gate)
     u2, _ = _float_rows('gated_act_quant', up)
     rows, cols = g2.shape
-    codes, pitch, scales, zeros = _codes_like(g2, rows, cols, sym)
+    codes, pitch, scales, zeros, out = _codes_like(gate, shape, sym)
     if rows:
         L.launch(dev, 'lc_int8_gated_act_quant', g2.data_ptr(), u2.data_ptr(), dt, rows, cols, g2.stride()[0], u2.stride()[0], kind,
                  codes.data_ptr(), pitch, scales.data_ptr(), None if sym else zeros.data_ptr())
-    return _shaped(codes, scales, zeros, shape)
+    return out
 
 
 def aligned_rows(codes):
@@ -191,13 +185,13 @@ def int8_gemm(a, a_s, b, b_s, bias=None, a_z=None, b_sum=None, out_dtype=torch.b
     if not (a_s.get_device() == b.get_device() == b_s.get_device() == dev) or (bias is not None and bias.get_device() != dev) \
             or (a_z is not None and not a_z.get_device() == b_sum.get_device() == dev):
         L.refuse_devices(name, a, a_s=a_s, a_z=a_z, b=b, b_s=b_s, b_sum=b_sum, bias=bias)
-    c = a2.new_empty((M, N), dtype=out_dtype)
+    c = a.new_empty((M, N) if a.dim() == 2 else (*a.shape[:-1], N), dtype=out_dtype)
     if M and N:
         L.launch(dev, 'lc_int8_gemm', L.INT8_GEMM.pack(
             a2.data_ptr(), _pitch(a2, M, K), a_s.data_ptr(), 0 if a_z is None else a_z.data_ptr(), b.data_ptr(), _pitch(b, N, K),
             b_s.data_ptr(), 0 if a_z is None else b_sum.data_ptr(), 0 if bias is None else bias.data_ptr(), M, N, K,
             c.data_ptr(), out, _status_of(a, dev)))
-    return c if a.dim() == 2 else c.view(*a.shape[:-1], N)
+    return c
 
 
 def int8_dynamic_forward_func(x, w, w_scale, bias=None, w_sum=None):
@@ -218,7 +212,8 @@ def int8_dynamic_forward_func(x, w, w_scale, bias=None, w_sum=None):
             or (not sym and w_sum.get_device() != dev):
         L.refuse_devices(name, x, w=w, w_scale=w_scale, bias=bias, w_sum=w_sum)
     dense = x2.is_contiguous()
-    c = torch.empty_like(x2) if dense and N == K else x2.new_empty((M, N))      # half the time, where it fits
+    # (a tensor like another is made in half the time, where it fits)
+    c = torch.empty_like(x) if N == K and x.is_contiguous() else x.new_empty((M, N) if x.dim() == 2 else (*x.shape[:-1], N))
     if M and N:
         # lc_int8_linear_scratch(M, K)
         room = 0 if M == 1 and K <= 4096 else M * (((K + 15) & -16) + 8)
@@ -232,7 +227,7 @@ def int8_dynamic_forward_func(x, w, w_scale, bias=None, w_sum=None):
             x2.data_ptr(), dt, x2.stride()[0], w.data_ptr(), _pitch(w, N, K), w_scale.data_ptr(), 0 if sym else w_sum.data_ptr(),
             0 if bias is None else bias.data_ptr(), M, N, K, sym, c.data_ptr(), scratch.data_ptr() if room else 0, room,
             _status_of(x, dev)))
-    return c if x.dim() == 2 else c.view(*x.shape[:-1], N)
+    return c
 
 
 class Int8Linear(nn.Module):
