@@ -61,7 +61,7 @@ __device__ __forceinline__ Channel load_channel(const Int8Args& g, int n) {
 // The outputs of C tokens of one channel.  s, z: the tokens' scales and zero points in shared memory (s 16-byte
 // aligned); out: the first token's element, tokens N elements apart; count: how many of the C tokens exist.  All values
 // are formed before the first store: stores may alias anything and would otherwise keep the loads behind them waiting
-// (17 us of a 512-token tile's 22 were that).
+// (512 x 512 x 512 on pairs: 15.1 us with the loads between the stores, 7.8 this way).
 template <typename T, int C>
 __device__ __forceinline__ void finish_tokens(const uint32_t (&v)[C], const float* s, const int* z, bool zeros,
                                               const Channel& c, T* out, int64_t N, int count, bool lost) {
@@ -99,8 +99,13 @@ __device__ __forceinline__ void finish_tokens(const uint32_t (&v)[C], const floa
 // Few tokens leave the weights as the only traffic that matters (N * K bytes), and N / 128 CTAs are too few to draw
 // the HBM's bandwidth: K is split over the CTAs of a cluster.  Each CTA owns a run of the tile's tokens; every CTA lays its
 // partial sums out by token in shared memory, one bulk copy takes an owner's run there, and the owner adds and finishes
-// it (stores of 4 bytes to the other CTAs cost 40 ns a token: 4 us for 128 of them).  The weights of the first `stages` blocks are requested before the kernel waits for the one that quantises
-// the activations (programmatic dependent launch), which hides it.
+// it (128 x 512 x 512 split in four: 8.3 us; 10.0 with stores of 4 bytes to the other CTAs).  The weights of the first
+// `stages` blocks are requested before the kernel waits for the one that quantises the activations (programmatic
+// dependent launch), which hides most of it: 2 x 4096 x 4096 9.2 us, 10.9 as two calls.
+//
+// What bounds it: for a few tokens the way of the weights from HBM, and 4.5 us of launch, first copies and exchange
+// (1 x 4096 x 4096: 8.9 us with its quantisation, of which the weights' bytes are 2.6); for more, a k block's way from L2
+// through a CTA's stages, 0.2 us.
 constexpr int kRows = 128, kBlockK = 128, kStreamThreads = 256;
 constexpr int kWeightBytes = kRows * kBlockK;
 constexpr int kSmemMost = 227 * 1024;
@@ -489,6 +494,8 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
 // that eight warps finish one tile while the tensor cores work on the next.  Warp 0 of each CTA copies its own operands and
 // signals the leader's barrier, warp 1 of the leader issues the MMAs for both, the others finish 128 tokens of 32
 // channels each (sixteen warps with 64 each were 3 % slower: they take issue slots and power from the product).
+// Bound by the power limit: 16384 x 4096 x 11008 takes 523 us in a long run (2.8 PFLOP/s, twice what cuBLAS sustains in
+// bf16; 389 us with operands of zeros), 2048 x 11008 x 4096 62 us (3.0 PFLOP/s, the tensor pipe 85 % busy).
 // The kernel asks for all of an SM's shared memory: no other CTA that needs tensor memory can then lie beside it and
 // wait for its columns while it waits for theirs.
 constexpr int kPairRows = 256, kPairTokens = 256, kPairStages = 6, kPairBufs = 2;

@@ -194,7 +194,7 @@ __device__ __forceinline__ Raw<T, N> pack(const float (&f)[N]) {
 // One warp to a row up to 2 KB, which needs no barrier; above, the fewest warps whose registers still leave several CTAs to
 // an SM (4096 values in bf16, 8192 rows: 4 x 4 14.7 us, 8 x 2 17.5, 16 x 1 27.4; 11008 values, quantised: 8 x 6 20.1, 16 x 3
 // 28.9; norms, with two inputs: 108 and 69).  A few rows leave the SMs empty: there what counts is how little a
-// lane does (one gated row of 8192: 16 x 2).  Not so for norms: a sum's association follows the shape, and a row's result
+// lane does.  Not so for norms: a sum's association follows the shape, and a row's result
 // must not depend on how many others there are (one row of 4096: 3.2 us instead of 2.7).
 template <int W, int V> struct RowShape {
   static constexpr int kWarps = W, kVecs = V;
