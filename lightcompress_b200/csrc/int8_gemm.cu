@@ -99,9 +99,11 @@ __device__ __forceinline__ void finish_tokens(const uint32_t (&v)[C], const floa
 // Few tokens leave the weights as the only traffic that matters (N * K bytes), and N / 128 CTAs are too few to draw
 // the HBM's bandwidth: K is split over the CTAs of a cluster.  Each CTA owns a run of the tile's tokens; every CTA lays its
 // partial sums out by token in shared memory, one bulk copy takes an owner's run there, and the owner adds and finishes
-// it (128 x 512 x 512 split in four: 8.3 us; 10.0 with stores of 4 bytes to the other CTAs).  The weights of the first
-// `stages` blocks are requested before the kernel waits for the one that quantises the activations (programmatic
-// dependent launch), which hides most of it: 2 x 4096 x 4096 9.2 us, 10.9 as two calls.
+// it (128 x 512 x 512 split in four: 8.3 us; 10.0 with stores of 4 bytes to the other CTAs).
+//
+// Both kernels are launched as dependents of the kernel before them and wait for its end before they read anything: their
+// launch and setting up overlap the quantisations and norms of this library, which let them begin early (quantisation and
+// product of 2 x 4096 x 4096: 9.2 us, 10.9 without).  Behind any other kernel, copy or fill the wait is over at once.
 //
 // What bounds it: for a few tokens the way of the weights from HBM, and 4.5 us of launch, first copies and exchange
 // (1 x 4096 x 4096: 8.9 us with its quantisation, of which the weights' bytes are 2.6); for more, a k block's way from L2
@@ -311,7 +313,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     if (splits > 1 && mine > 0) mbar_expect_tx(land_bar, (uint32_t)((splits - 1) * mine * kRows * 4));
-    // the weights do not depend on the kernel before this one
+    grid_dependency_wait();
     for (int i = 0; i < stages && i < count; ++i) {
       mbar_expect_tx(full_bar(i), kStage);
       tma_load_2d(base + i * kStage, &maps.w, (kb0 + i) * kBlockK, n0, full_bar(i));
@@ -330,7 +332,8 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
   if (splits > 1) cluster_arrive();                        // waited for before anything is sent to another CTA
   const int group = warp >> 2;                             // of the two that share a channel
   const int c = (warp & 3) * 32 + lane, n = n0 + c;
-  const Channel ch = load_channel<T>(g, n);                // weights' side: nothing the kernel before this one writes
+  grid_dependency_wait();
+  const Channel ch = load_channel<T>(g, n);
   const bool zeros = kQuant ? !g.sym : g.a_z != nullptr;
   if constexpr (kQuant) {
     quantise_token<T>(g, token, kb0, count, gen + Smem::codes(stages), NT * kBlockK, s_scale, s_zero,
@@ -338,7 +341,6 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");         // the MMAs read what was just written
     __syncthreads();
   } else {
-    grid_dependency_wait();
     for (int t = (int)threadIdx.x - 64; t >= 0 && t < NT; t += kStreamThreads - 64) {
       s_scale[t] = t < tokens ? g.a_s[m0 + t] : 0.f;
       s_zero[t] = t < tokens && g.a_z ? g.a_z[m0 + t] : 0;
@@ -775,7 +777,7 @@ cudaError_t allow_smem(F* kernel) {
 }
 
 template <typename T, int NT, bool kQuant = false>
-int launch_stream(const Int8Args& g, int splits, bool dependent, cudaStream_t st) {
+int launch_stream(const Int8Args& g, int splits, cudaStream_t st) {
   const int n_tiles = (g.N + kRows - 1) / kRows, m_tiles = (g.M + NT - 1) / NT;
   const int blocks = (g.K + kBlockK - 1) / kBlockK;
   const int per_sm = (int64_t)n_tiles * m_tiles * splits > ctas_at_once(splits) ? 2 : 1;
@@ -801,13 +803,13 @@ int launch_stream(const Int8Args& g, int splits, bool dependent, cudaStream_t st
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = attr;
-  cfg.numAttrs = dependent ? 2 : 1;
+  cfg.numAttrs = kQuant ? 1 : 2;                           // the token is read at once
   LC_CHECK_CUDA(cudaLaunchKernelEx(&cfg, stream_kernel<T, NT, kQuant>, maps, g, splits, stages));
   return LC_OK;
 }
 
 template <typename T>
-int launch_pair(const Int8Args& g, bool dependent, cudaStream_t st) {
+int launch_pair(const Int8Args& g, cudaStream_t st) {
   Maps maps;
   int rc;
   if ((rc = encode_codes(&maps.w, g.b, g.K, g.N, g.ldb, 128)) != LC_OK) return rc;
@@ -829,20 +831,20 @@ int launch_pair(const Int8Args& g, bool dependent, cudaStream_t st) {
   cfg.dynamicSmemBytes = kSmemMost;
   cfg.stream = st;
   cfg.attrs = &attr;
-  cfg.numAttrs = dependent ? 1 : 0;
+  cfg.numAttrs = 1;
   LC_CHECK_CUDA(cudaLaunchKernelEx(&cfg, pair_kernel<T>, maps, g, pt));
   return LC_OK;
 }
 
 template <typename T>
-int launch(const Int8Args& g, bool dependent, cudaStream_t st) {
+int launch(const Int8Args& g, cudaStream_t st) {
   const Choice c = choose(g.M, g.N, g.K);
   switch (c.tokens) {
-    case 16: return launch_stream<T, 16>(g, c.splits, dependent, st);
-    case 32: return launch_stream<T, 32>(g, c.splits, dependent, st);
-    case 64: return launch_stream<T, 64>(g, c.splits, dependent, st);
-    case 128: return launch_stream<T, 128>(g, c.splits, dependent, st);
-    default: return launch_pair<T>(g, dependent, st);
+    case 16: return launch_stream<T, 16>(g, c.splits, st);
+    case 32: return launch_stream<T, 32>(g, c.splits, st);
+    case 64: return launch_stream<T, 64>(g, c.splits, st);
+    case 128: return launch_stream<T, 128>(g, c.splits, st);
+    default: return launch_pair<T>(g, st);
   }
 }
 
@@ -868,15 +870,13 @@ int check_arch() {
   return major == 10 && minor == 0 ? LC_OK : LC_ERR_ARCH;
 }
 
-// dependent: the kernel before this one on the stream is the quantisation of lc_int8_linear, which writes a, a_s and a_z
-// and nothing else that the product reads
-int product(const Int8Args& g, int out_dtype, bool dependent, cudaStream_t st) {
+int product(const Int8Args& g, int out_dtype, cudaStream_t st) {
   const int rc = check_arch();
   if (rc != LC_OK) return rc;
   switch (out_dtype) {
-    case LC_F32: return launch<float>(g, dependent, st);
-    case LC_BF16: return launch<__nv_bfloat16>(g, dependent, st);
-    default: return launch<__half>(g, dependent, st);
+    case LC_F32: return launch<float>(g, st);
+    case LC_BF16: return launch<__nv_bfloat16>(g, st);
+    default: return launch<__half>(g, st);
   }
 }
 
@@ -893,7 +893,7 @@ extern "C" LC_API int lc_int8_gemm(const lc_int8_gemm_args* args_host, lc_stream
   if (!aligned16(p.a) || (p.lda & 15)) return LC_ERR_ALIGN;
   return product(Int8Args{nullptr, 0, 0, p.a, p.b, p.a_s, p.a_z, p.b_s, p.b_sum, p.bias, p.c, p.status, p.lda, p.ldb, (int)p.M,
                           (int)p.N, (int)p.K},
-                 (int)p.out_dtype, false, reinterpret_cast<cudaStream_t>(stream));
+                 (int)p.out_dtype, reinterpret_cast<cudaStream_t>(stream));
 }
 
 extern "C" LC_API int64_t lc_int8_linear_scratch(int64_t M, int64_t K) {
@@ -920,9 +920,9 @@ extern "C" LC_API int lc_int8_linear(const lc_int8_linear_args* args_host, lc_st
     if ((rc = check_arch()) != LC_OK) return rc;
     const int splits = choose(1, p.N, p.K).splits;
     switch (dtype) {
-      case LC_F32: return launch_stream<float, 16, true>(g, splits, false, st);
-      case LC_BF16: return launch_stream<__nv_bfloat16, 16, true>(g, splits, false, st);
-      default: return launch_stream<__half, 16, true>(g, splits, false, st);
+      case LC_F32: return launch_stream<float, 16, true>(g, splits, st);
+      case LC_BF16: return launch_stream<__nv_bfloat16, 16, true>(g, splits, st);
+      default: return launch_stream<__half, 16, true>(g, splits, st);
     }
   }
   const int64_t lda = (p.K + 15) / 16 * 16;
@@ -931,5 +931,5 @@ extern "C" LC_API int lc_int8_linear(const lc_int8_linear_args* args_host, lc_st
   int32_t* a_z = p.sym ? nullptr : reinterpret_cast<int32_t*>(a_s + p.M);
   if ((rc = int8_quant_rows(p.x, dtype, p.M, p.K, p.ldx, codes, lda, a_s, a_z, st)) != LC_OK) return rc;
   g.a = codes, g.lda = lda, g.a_s = a_s, g.a_z = a_z;
-  return product(g, dtype, true, st);
+  return product(g, dtype, st);
 }

@@ -62,8 +62,7 @@ template <typename T, int kAct, bool kSym>
 __global__ void __launch_bounds__(kThreads) quant_any_kernel(QuantArgs a) {
   using E = Elem<T>;
   __shared__ float red[16];
-  // a product launched as this kernel's dependent may start on its weights; it waits for this kernel to end before it
-  // reads codes, scales or zero points
+  // a product launched as this kernel's dependent may set itself up; it waits for this kernel to end before it reads
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;

@@ -261,6 +261,73 @@ def test_captured_and_replayed_and_on_other_streams(m):
     assert all(torch.equal(o, want[i % 3]) for i, o in enumerate(outs))
 
 
+@pytest.mark.parametrize('m', [3, 40, 300, 2100])
+def test_product_waits_for_whatever_wrote_its_operands(m):
+    """Operands written right before the product by a copy, a fill, a kernel of torch, this library's quantisation and on
+    another stream, eagerly and captured."""
+    from lightcompress_b200.int8_linear import act_quant, int8_gemm
+    n, k = 2304, 1040
+    xs = [_acts(m, k, torch.bfloat16, seed).cuda() for seed in range(4)]
+    ws = [_weight(n, k, seed)[1].contiguous() for seed in range(4)]
+    bs = [torch.full((n,), 0.5 + i, device='cuda') for i in range(4)]
+    want = [int8_gemm(*act_quant(x), w, b) for x, w, b in zip(xs, ws, bs)]
+    x, w, b = xs[0].clone(), ws[0].clone(), bs[0].clone()
+    side = torch.cuda.Stream()
+    picked = torch.zeros(1, dtype=torch.int64, device='cuda')
+    all_x, all_w = torch.stack(xs), torch.stack(ws)
+
+    def by_copies(i):
+        q = act_quant(xs[i])
+        w.copy_(ws[i])
+        b.copy_(bs[i])
+        return int8_gemm(*q, w, b)
+
+    def by_a_fill(i):
+        q = act_quant(xs[i])
+        b.fill_(0.5 + i)
+        return int8_gemm(*q, ws[i], b)
+
+    def by_a_kernel(i):
+        q = act_quant(xs[i])
+        return int8_gemm(*q, (all_w[i].int() + 0).to(torch.int8), bs[i])
+
+    def on_another_stream(i):
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            x.copy_(xs[i])
+            q = act_quant(x)
+        torch.cuda.current_stream().wait_stream(side)
+        w.copy_(ws[i])
+        y = int8_gemm(*q, w, bs[i])
+        for t in q:
+            t.record_stream(torch.cuda.current_stream())
+        return y
+    for way in (by_copies, by_a_fill, by_a_kernel, on_another_stream):
+        for rep in range(3):
+            for i in range(4):
+                assert torch.equal(way(i), want[i]), (way.__name__, i)
+
+    def picks():
+        i = picked
+        x.copy_(all_x.index_select(0, i)[0])
+        q = act_quant(x)
+        w.copy_(all_w.index_select(0, i)[0])
+        b.zero_()
+        b.add_(0.5).add_(i)
+        return int8_gemm(*q, w, b), int8_gemm(*act_quant(x), w, b)
+    picks()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ys = picks()
+    for rep in range(3):
+        for i in range(4):
+            picked.fill_(i)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(ys[0], want[i]) and torch.equal(ys[1], want[i])
+
+
 def test_module_from_a_quantised_linear():
     from lightcompress_b200 import Int8Linear, IntegerQuantizer, RTN
     torch.manual_seed(0)
