@@ -131,6 +131,10 @@ def _load():
 
 
 lib = _load()
+try:
+    from . import _calls  # noqa: F401  (the compiled front of the W8A8 operators, linked against the library above)
+except ImportError as e:
+    raise ImportError(f'lightcompress_b200/_calls.so is missing or stale ({e}): build it with `python __graft_entry__.py`') from None
 
 
 def status_string(code):

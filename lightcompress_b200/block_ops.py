@@ -23,6 +23,7 @@ import torch
 
 from . import _lib as L
 from . import int8_linear
+from ._lib import _calls
 
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 _checked = {}
@@ -245,6 +246,9 @@ def residual_norm(x, residual=None, weight=None, post_weight=None, gate=None, sc
 
     Returns (h, y).  Without weight, y is None.  With quant, y is what int8_linear.act_quant returns for it, (codes,
     scales) or, with sym=False, (codes, scales, zeros), quantised from fp32.  Where h would equal x, it is x."""
+    out = _calls.residual_norm(x, residual, weight, post_weight, gate, scale, eps, weight_offset, quant, sym)
+    if out is not None:
+        return out
     name = 'residual_norm'
     if torch.is_grad_enabled() and (
             x.requires_grad or (weight is not None and weight.requires_grad) or (residual is not None and residual.requires_grad)
@@ -258,19 +262,14 @@ def residual_norm(x, residual=None, weight=None, post_weight=None, gate=None, sc
     if C == 0:
         raise ValueError(f'{name}: the last dimension must not be empty')
     rows, gate_rows = x.numel() // C, 0
-    contiguous = x.is_contiguous()
-    if contiguous:
-        x2, ldx = x, C
-    else:
-        x2 = _strided_rows(x)
-        ldx = x2.stride()[0]
+    x2 = _strided_rows(x)
+    ldx = x2.stride()[0]
     r2, ldr = residual, C
     if residual is not None:
         if residual.shape != shape or residual.dtype != dtype or residual.get_device() != dev:
             _refuse_operand(name, 'residual', residual, x, shape)
-        if not residual.is_contiguous():
-            r2 = _strided_rows(residual)
-            ldr = r2.stride()[0]
+        r2 = _strided_rows(residual)
+        ldr = r2.stride()[0]
     if weight is not None:
         if weight.dtype != dtype or weight.dim() != 1 or weight.numel() != C or weight.get_device() != dev:
             _refuse_operand(name, 'weight', weight, x, (C,))
@@ -289,13 +288,13 @@ def residual_norm(x, residual=None, weight=None, post_weight=None, gate=None, sc
     kept = residual is None and post_weight is None and gate is None and scale == 1.0
     if kept and weight is None:
         return x, None
-    h = x if kept else torch.empty_like(x) if contiguous else x.new_empty(shape)
+    h = x if kept else x.new_empty(shape)
     y = codes = scales = zeros = None
     pitch = 0
     if quant:
         codes, pitch, scales, zeros, quantised = int8_linear._codes_like(x, shape, sym)
     elif weight is not None:
-        y = torch.empty_like(x) if contiguous else x.new_empty(shape)
+        y = x.new_empty(shape)
     if rows:
         L.launch(dev, 'lc_residual_norm', L.RESIDUAL_NORM.pack(
             x2.data_ptr(), _at(r2), _at(post_weight), _at(gate), gate_rows, _at(weight), dt, rows, C, ldx, ldr, scale, eps,
@@ -327,6 +326,9 @@ def rotary_embed(q, k, positions, inv_freq, interleaved=False, attention_scale=1
     q, k: bf16, fp16 or fp32 with contiguous heads (any other strides, e.g. views of one projection's output);
     positions: int64, (B, T), (1, T) or (T,); inv_freq: (R / 2,) fp32, see rope_frequencies.  Returns (q, k) in new memory,
     (B, T, H, D) contiguous seen as (B, H, T, D) like the stock projections, or the given tensors if inplace."""
+    out = None if inplace else _calls.rotary_embed(q, k, positions, inv_freq, interleaved, attention_scale)
+    if out is not None:
+        return out
     name = 'rotary_embed'
     if torch.is_grad_enabled() and (q.requires_grad or inv_freq.requires_grad or (k is not None and k.requires_grad)):
         L.refuse_grad(name)
@@ -383,8 +385,6 @@ def _heads(name, x, B, H, T, D, inplace):
         if (sb == 0 and B > 1) or (sh == 0 and H > 1) or (st == 0 and T > 1):
             raise ValueError(f'{name}: cannot work in place on an expanded tensor')
         return x, x, sb, sh, st
-    if sd == 1 and sh == D and st == H * D and sb == T * H * D:
-        return x, torch.empty_like(x), sb, sh, st           # x lies as the result does, and so will a tensor like it
     return x, x.new_empty((B, T, H, D)).transpose(1, 2), sb, sh, st
 
 

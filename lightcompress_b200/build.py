@@ -1,4 +1,5 @@
-"""Builds the C-ABI shared library (liblc_b200.so) in-tree with nvcc for sm_100a.
+"""Builds the C-ABI shared library (liblc_b200.so) in-tree with nvcc for sm_100a, and beside it the compiled front of
+the W8A8 operators (_calls.so, a Python module over torch's C++ interface and that library) with g++.
 
     python __graft_entry__.py            (from the repository root; loads this file by path)
     python lightcompress_b200/build.py [--force]
@@ -6,15 +7,19 @@
 One translation unit per kernel family; objects go to build/, the library next to this file.
 """
 import concurrent.futures
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, 'csrc')
 LIB = os.path.join(HERE, 'liblc_b200.so')
+CALLS_SRC = os.path.join(CSRC, 'host', 'calls.cpp')
+CALLS = os.path.join(HERE, '_calls.so')
 OBJ_DIR = os.path.join(ROOT, 'build', 'lc_b200')
 
 NVCC_FLAGS = ['-gencode', 'arch=compute_100a,code=sm_100a', '-lineinfo', '-O3', '-std=c++17',
@@ -62,6 +67,15 @@ def build(force=False, verbose=False):
         list(ex.map(run, jobs))
     if jobs or not os.path.exists(LIB) or any(os.path.getmtime(o) > os.path.getmtime(LIB) for o in objs):
         run([nvcc, '-shared', '-o', LIB] + objs + ['-gencode', 'arch=compute_100a,code=sm_100a'])
+    header = os.path.join(ROOT, 'include', 'lc_b200.h')
+    if force or not os.path.exists(CALLS) or os.path.getmtime(CALLS) < max(map(os.path.getmtime, (CALLS_SRC, header))):
+        torch = os.path.dirname(importlib.util.find_spec('torch').origin)      # found, not imported
+        cuda = os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc))), 'include')
+        run(['g++', '-O2', '-std=c++17', '-fPIC', '-shared', '-fvisibility=hidden', '-Wall',
+             '-I' + sysconfig.get_path('include'), '-I' + os.path.join(torch, 'include'),
+             '-I' + os.path.join(torch, 'include', 'torch', 'csrc', 'api', 'include'), '-I' + cuda, CALLS_SRC, '-o', CALLS,
+             '-L' + os.path.join(torch, 'lib'), '-ltorch_python', '-ltorch_cpu', '-ltorch', '-lc10', '-lc10_cuda',
+             '-L' + HERE, '-l:' + os.path.basename(LIB), '-Wl,-rpath,$ORIGIN'])
     return LIB
 
 

@@ -6,11 +6,15 @@ sibling of fp8_linear.  Codes are int8 with an fp32 scale per token (activations
 activations may carry a zero point per token as well.
 
 Nothing here synchronises or reads device memory on the host, so every call can be captured into a CUDA graph.
+
+Each function asks the compiled front (_calls) first, which serves the ordinary call in a third of the host time and returns
+None for any other; the Python below it knows every case and says what is wrong with a call.
 """
 import torch
 import torch.nn as nn
 
 from . import _lib as L
+from ._lib import _calls
 
 _ACTS = {'silu': 1, 'gelu': 2, 'gelu_tanh': 3}
 _status = {}
@@ -27,6 +31,7 @@ def _status_of(t, dev):
         s = torch.zeros(1, dtype=torch.int32, device=t.device)
         torch.cuda.current_stream(dev).synchronize()      # other streams may use it from here on
         _status[dev] = s
+        _calls.set_status(dev, s.data_ptr())
     return s.data_ptr()
 
 
@@ -61,10 +66,7 @@ def _codes_like(x, shape, sym):
     cols = shape[-1]
     pitch = (cols + 15) & -16
     lead = shape[:-1]
-    if pitch == cols and x.shape == shape and x.is_contiguous():
-        codes = torch.empty_like(x, dtype=torch.int8)
-    else:
-        codes = x.new_empty((*lead, pitch), dtype=torch.int8)
+    codes = x.new_empty((*lead, pitch), dtype=torch.int8)
     scales = x.new_empty((*lead, 1), dtype=torch.float32)
     zeros = None if sym else x.new_empty((*lead, 1), dtype=torch.int32)
     seen = codes if pitch == cols else codes[..., :cols]
@@ -76,6 +78,11 @@ def act_quant(x, sym=True):
     s = max(|x|) / 127 and q = rint(x / s), or, with a zero point, 255 steps over the token's range widened to
     hold zero, x ~ (q - z) s.  x: (..., K) of bf16, fp16 or fp32, any strides.  A token that holds a NaN or an
     infinity gets scale NaN.  The codes' rows lie a multiple of 16 bytes apart, which the products require."""
+    out = _calls.act_quant(x, sym)
+    return _act_quant(x, sym) if out is None else out
+
+
+def _act_quant(x, sym):
     if x.requires_grad and torch.is_grad_enabled():
         L.refuse_grad('act_quant')
     x2, dt = _float_rows('act_quant', x)
@@ -93,6 +100,11 @@ def gated_act_quant(gate, up, act='silu', sym=True):
     kind = _ACTS.get(act)
     if kind is None:
         raise NotImplementedError(f'gated_act_quant: activation {act!r}; there are {sorted(_ACTS)}')
+    out = _calls.gated_act_quant(gate, up, kind, sym)
+    return _gated_act_quant(gate, up, kind, sym) if out is None else out
+
+
+def _gated_act_quant(gate, up, kind, sym):
     shape = gate.shape
     if shape != up.shape or gate.dtype != up.dtype:
         raise ValueError(f'gated_act_quant: gate {tuple(shape)} {gate.dtype} and up {tuple(up.shape)} {up.dtype} differ')
@@ -161,6 +173,11 @@ def int8_gemm(a, a_s, b, b_s, bias=None, a_z=None, b_sum=None, out_dtype=torch.b
     """a: (..., K) int8 codes with scales a_s (..., 1) and, if given, zero points a_z (..., 1), as act_quant returns
     them; b: (N, K) int8 with b_s (N fp32 values) and, with zero points, b_sum (N int32 sums of b's rows).  Returns
     (..., N) = ((a - a_z) b^T) * a_s * b_s + bias in out_dtype; the sum of products is exact."""
+    c = _calls.int8_gemm(a, a_s, b, b_s, bias, a_z, b_sum, out_dtype)
+    return _int8_gemm(a, a_s, b, b_s, bias, a_z, b_sum, out_dtype) if c is None else c
+
+
+def _int8_gemm(a, a_s, b, b_s, bias, a_z, b_sum, out_dtype):
     name = 'int8_gemm'
     if torch.is_grad_enabled() and (a_s.requires_grad or b_s.requires_grad or (bias is not None and bias.requires_grad)):
         L.refuse_grad(name)
@@ -185,7 +202,7 @@ def int8_gemm(a, a_s, b, b_s, bias=None, a_z=None, b_sum=None, out_dtype=torch.b
     if not (a_s.get_device() == b.get_device() == b_s.get_device() == dev) or (bias is not None and bias.get_device() != dev) \
             or (a_z is not None and not a_z.get_device() == b_sum.get_device() == dev):
         L.refuse_devices(name, a, a_s=a_s, a_z=a_z, b=b, b_s=b_s, b_sum=b_sum, bias=bias)
-    c = a.new_empty((M, N) if a.dim() == 2 else (*a.shape[:-1], N), dtype=out_dtype)
+    c = a.new_empty((*a.shape[:-1], N), dtype=out_dtype)
     if M and N:
         L.launch(dev, 'lc_int8_gemm', L.INT8_GEMM.pack(
             a2.data_ptr(), _pitch(a2, M, K), a_s.data_ptr(), 0 if a_z is None else a_z.data_ptr(), b.data_ptr(), _pitch(b, N, K),
@@ -198,6 +215,11 @@ def int8_dynamic_forward_func(x, w, w_scale, bias=None, w_sum=None):
     """The W8A8 linear's forward: x (..., K) quantised per token and multiplied with w (N, K) int8, scales w_scale (N fp32
     values), in one call.  With w_sum (N int32 sums of w's rows) the activations get a zero point per token, without it
     they are quantised symmetrically.  Returns (..., N) of x's type; bias has that type too."""
+    c = _calls.int8_linear(x, w, w_scale, bias, w_sum)
+    return _int8_dynamic_forward(x, w, w_scale, bias, w_sum) if c is None else c
+
+
+def _int8_dynamic_forward(x, w, w_scale, bias, w_sum):
     name = 'int8_dynamic_forward_func'
     if torch.is_grad_enabled() and (x.requires_grad or w_scale.requires_grad or (bias is not None and bias.requires_grad)):
         L.refuse_grad(name)
@@ -211,18 +233,10 @@ def int8_dynamic_forward_func(x, w, w_scale, bias=None, w_sum=None):
     if not (w.get_device() == w_scale.get_device() == dev) or (bias is not None and bias.get_device() != dev) \
             or (not sym and w_sum.get_device() != dev):
         L.refuse_devices(name, x, w=w, w_scale=w_scale, bias=bias, w_sum=w_sum)
-    dense = x2.is_contiguous()
-    # (a tensor like another is made in half the time, where it fits)
-    c = torch.empty_like(x) if N == K and x.is_contiguous() else x.new_empty((M, N) if x.dim() == 2 else (*x.shape[:-1], N))
+    c = x.new_empty((*x.shape[:-1], N))
     if M and N:
-        # lc_int8_linear_scratch(M, K)
-        room = 0 if M == 1 and K <= 4096 else M * (((K + 15) & -16) + 8)
-        if room == 0:
-            scratch = None
-        elif dense and K >= 32 and room <= 1 << 20:
-            scratch = torch.empty_like(x2)                # 2 K bytes a token at least: enough
-        else:
-            scratch = x2.new_empty(room, dtype=torch.int8)
+        room = L.lib.lc_int8_linear_scratch(M, K)
+        scratch = x.new_empty(room, dtype=torch.int8) if room else None
         L.launch(dev, 'lc_int8_linear', L.INT8_LINEAR.pack(
             x2.data_ptr(), dt, x2.stride()[0], w.data_ptr(), _pitch(w, N, K), w_scale.data_ptr(), 0 if sym else w_sum.data_ptr(),
             0 if bias is None else bias.data_ptr(), M, N, K, sym, c.data_ptr(), scratch.data_ptr() if room else 0, room,
