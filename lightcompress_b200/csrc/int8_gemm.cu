@@ -101,8 +101,8 @@ __device__ __forceinline__ void finish_tokens(const uint32_t (&v)[C], const floa
 // partial sums out by token in shared memory, one bulk copy takes an owner's run there, and the owner adds and finishes
 // it (128 x 512 x 512 split in four: 8.3 us; 10.0 with stores of 4 bytes to the other CTAs).
 //
-// Both kernels are launched as dependents of the kernel before them and wait for its end before they read anything: their
-// launch and setting up overlap the quantisations and norms of this library, which let them begin early (quantisation and
+// Both kernels, and the quantisations, norms and rotary embeddings around them, are launched as dependents of the kernel
+// before them and wait for its end before they read anything, so that launching and setting up overlap (quantisation and
 // product of 2 x 4096 x 4096: 9.2 us, 10.9 without).  Behind any other kernel, copy or fill the wait is over at once.
 //
 // What bounds it: for a few tokens the way of the weights from HBM, and 4.5 us of launch, first copies and exchange
@@ -175,6 +175,9 @@ __device__ __forceinline__ bool elect_one() {
   return is != 0;
 }
 
+// Only once this CTA has its tensor memory: a product further on could otherwise take the columns that this one still
+// needs, and wait for its end.
+__device__ __forceinline__ void let_next_begin() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
@@ -302,7 +305,10 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
   const int run = (tokens + splits - 1) / splits, first = rank * run, mine = max(0, min(run, tokens - first));
 
   Values<T> token;
-  if constexpr (kQuant) token = load_token<T>(g);
+  if constexpr (kQuant) {
+    grid_dependency_wait();
+    token = load_token<T>(g);
+  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) {
       mbar_init(full_bar(s), 1);
@@ -329,6 +335,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
   __syncthreads();
   tcgen05_fence_after();
   const uint32_t tmem = *tmem_slot;
+  let_next_begin();
   if (splits > 1) cluster_arrive();                        // waited for before anything is sent to another CTA
   const int group = warp >> 2;                             // of the two that share a channel
   const int c = (warp & 3) * 32 + lane, n = n0 + c;
@@ -585,6 +592,7 @@ pair_kernel(const __grid_constant__ Maps maps, Int8Args g, PairTiles pt) {
   cluster_wait();
   tcgen05_fence_after();
   const uint32_t tmem = *tmem_slot;
+  let_next_begin();
   grid_dependency_wait();
 
   uint32_t issued = 0;                            // k blocks requested (thread 0)
@@ -803,7 +811,7 @@ int launch_stream(const Int8Args& g, int splits, cudaStream_t st) {
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = attr;
-  cfg.numAttrs = kQuant ? 1 : 2;                           // the token is read at once
+  cfg.numAttrs = 2;
   LC_CHECK_CUDA(cudaLaunchKernelEx(&cfg, stream_kernel<T, NT, kQuant>, maps, g, splits, stages));
   return LC_OK;
 }

@@ -62,8 +62,7 @@ template <typename T, int kAct, bool kSym>
 __global__ void __launch_bounds__(kThreads) quant_any_kernel(QuantArgs a) {
   using E = Elem<T>;
   __shared__ float red[16];
-  // a product launched as this kernel's dependent may set itself up; it waits for this kernel to end before it reads
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  begin_dependent();
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
     const T* u = static_cast<const T*>(a.up) + row * a.ldu;
@@ -92,7 +91,7 @@ __global__ void __launch_bounds__(RowGroup<kWarps>::kThreads) quant_rows_kernel(
   using G = RowGroup<kWarps>;
   constexpr bool kGated = kAct != kNone;
   __shared__ float red[2 * kWarps];
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // as in quant_any_kernel
+  begin_dependent();
   const int64_t row = (int64_t)blockIdx.x * G::kRows + G::row();
   if (G::kRows > 1 && row >= a.rows) return;                           // a whole warp, and no barrier follows
   const int vecs = (int)(a.cols / N);
@@ -153,8 +152,8 @@ bool launch_rows(const QuantArgs& a, cudaStream_t st) {
   auto go = [&](auto shape, auto width) {
     using S = decltype(shape);
     using G = RowGroup<S::kWarps>;
-    quant_rows_kernel<T, decltype(width)::value, S::kWarps, S::kVecs, kAct>
-        <<<(unsigned)((a.rows + G::kRows - 1) / G::kRows), G::kThreads, 0, st>>>(a);
+    launch_dependent(quant_rows_kernel<T, decltype(width)::value, S::kWarps, S::kVecs, kAct>,
+                     dim3((unsigned)((a.rows + G::kRows - 1) / G::kRows)), G::kThreads, 0, st, a);
   };
   return wide ? with_row_shape<false>(a.cols / N, a.rows, [&](auto s) { go(s, std::integral_constant<int, N>{}); })
               : with_value_shape(a.cols, [&](auto s) { go(s, std::integral_constant<int, 1>{}); });
@@ -167,7 +166,7 @@ int launch(const QuantArgs& a, cudaStream_t st) {
     return LC_OK;
   }
   const int64_t cap = (int64_t)kNumSMsB200 * 8;
-  quant_any_kernel<T, kAct, kSym><<<(unsigned)(a.rows < cap ? a.rows : cap), kThreads, 0, st>>>(a);
+  launch_dependent(quant_any_kernel<T, kAct, kSym>, dim3((unsigned)(a.rows < cap ? a.rows : cap)), kThreads, 0, st, a);
   LC_LAUNCH_CHECK();
   return LC_OK;
 }

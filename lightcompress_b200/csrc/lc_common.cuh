@@ -27,6 +27,28 @@ namespace lc {
 
 constexpr int kNumSMsB200 = 148;
 
+// Programmatic dependent launch, for the short kernels that run one after another in a deployed block: such a kernel lets
+// the next one begin as soon as all of its own CTAs run, and waits for the end of the one before it, and for its memory
+// operations, before it reads or writes global memory.  Every thread that touches global memory calls begin_dependent().
+__device__ __forceinline__ void begin_dependent() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+template <typename... P, typename... A>
+cudaError_t launch_dependent(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, A&&... args) {
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<A&&>(args)...);
+}
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 inline size_t dtype_size(int dt) { return dt == LC_F32 ? 4 : 2; }

@@ -44,7 +44,7 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads) norm_any_kernel(NormArgs a) {
   using E = Elem<T>;
   __shared__ float red[16];
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  begin_dependent();
   const float inv_c = 1.f / (float)a.cols;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(RowGroup<kWarps>::kThreads) norm_rows_kernel(N
   using G = RowGroup<kWarps>;
   using P = Raw<T, N>;
   __shared__ float red[4 * kWarps];
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");      // see the integer product
+  begin_dependent();
   const int64_t row = (int64_t)blockIdx.x * G::kRows + G::row();
   if (G::kRows > 1 && row >= a.rows) return;                           // a whole warp, and no barrier follows
   const int vecs = (int)(a.cols / N);
@@ -239,8 +239,8 @@ bool launch_rows(const NormArgs& a, cudaStream_t st) {
   auto go = [&](auto shape, auto width) {
     using S = decltype(shape);
     using G = RowGroup<S::kWarps>;
-    norm_rows_kernel<T, decltype(width)::value, S::kWarps, S::kVecs>
-        <<<(unsigned)((a.rows + G::kRows - 1) / G::kRows), G::kThreads, 0, st>>>(a);
+    launch_dependent(norm_rows_kernel<T, decltype(width)::value, S::kWarps, S::kVecs>,
+                     dim3((unsigned)((a.rows + G::kRows - 1) / G::kRows)), G::kThreads, 0, st, a);
   };
   return wide ? with_row_shape<true>(a.cols / N, a.rows, [&](auto s) { go(s, std::integral_constant<int, N>{}); })
               : with_value_shape(a.cols, [&](auto s) { go(s, std::integral_constant<int, 1>{}); });
@@ -253,7 +253,7 @@ int launch(const NormArgs& a, cudaStream_t st) {
     return LC_OK;
   }
   const int64_t cap = (int64_t)kNumSMsB200 * 8;
-  norm_any_kernel<T><<<(unsigned)(a.rows < cap ? a.rows : cap), kThreads, 0, st>>>(a);
+  launch_dependent(norm_any_kernel<T>, dim3((unsigned)(a.rows < cap ? a.rows : cap)), kThreads, 0, st, a);
   LC_LAUNCH_CHECK();
   return LC_OK;
 }

@@ -69,6 +69,7 @@ __global__ void __launch_bounds__(kThreads, 16) rotary_kernel(RotaryArgs a, Shap
   using E = Elem<T>;
   using P = Pack<T, V>;
   extern __shared__ float2 cs[];
+  begin_dependent();
   const int half = a.R / 2;
   const int64_t tok0 = (int64_t)blockIdx.x * sh.per_cta;
   const int tokens = (int)min((int64_t)sh.per_cta, a.B * a.T - tok0);
@@ -155,7 +156,8 @@ int launch_packed(const RotaryArgs& a, cudaStream_t st) {
   int64_t parts = (4 * kNumSMsB200 + grid - 1) / grid;
   const int64_t most = ((int64_t)sh.per_cta * per_token + kThreads - 1) / kThreads;
   if (parts > most) parts = most;
-  rotary_kernel<T, V, kInter><<<dim3((unsigned)grid, (unsigned)parts), kThreads, (size_t)sh.per_cta * (a.R / 2) * sizeof(float2), st>>>(a, sh);
+  LC_CHECK_CUDA(launch_dependent(rotary_kernel<T, V, kInter>, dim3((unsigned)grid, (unsigned)parts), kThreads,
+                                 (size_t)sh.per_cta * (a.R / 2) * sizeof(float2), st, a, sh));
   LC_LAUNCH_CHECK();
   return LC_OK;
 }
