@@ -105,8 +105,8 @@ __device__ __forceinline__ void finish_tokens(const uint32_t (&v)[C], const floa
 // before them and wait for its end before they read anything, so that launching and setting up overlap (quantisation and
 // product of 2 x 4096 x 4096: 9.2 us, 10.9 without).  Behind any other kernel, copy or fill the wait is over at once.
 //
-// What bounds it: for a few tokens the way of the weights from HBM, and 4.5 us of launch, first copies and exchange
-// (1 x 4096 x 4096: 8.9 us with its quantisation, of which the weights' bytes are 2.6); for more, a k block's way from L2
+// What bounds it: for a few tokens the way of the weights from HBM, and 4 us of launch, first copies and exchange
+// (1 x 4096 x 4096: 8.2 us with its quantisation, of which the weights' bytes are 2.6); for more, a k block's way from L2
 // through a CTA's stages, 0.2 us.
 constexpr int kRows = 128, kBlockK = 128, kStreamThreads = 256;
 constexpr int kWeightBytes = kRows * kBlockK;
@@ -199,8 +199,9 @@ struct Maps {
 
 // A single token is quantised by the product itself (kQuant): every CTA reads all of it for the range, before it asks for
 // its weights (behind them a load took up to 2.5 us to come), keeps it in registers and lays the codes of its own part
-// of K out as the copies would, while its first weights are on their way.  That saves a launch and a scratch buffer (3.5 us
-// of a call); for more values than one a thread's 16 the separate kernel, which the product overlaps, is faster.
+// of K out as the copies would, while its first weights are on their way.  That saves a launch and a scratch buffer
+// (4096 channels: 8.2 us, 9.0 in two launches; 11008 channels 11.2, 11.75); for more values than one a thread's 16 the
+// separate kernel, which the product overlaps, is faster.
 //
 // Shared memory of a CTA: stages, barriers, the tokens' scales and zero points.  The CTA's own partial sums take the
 // stages' place once its products are formed; those of the others land behind everything else where they are small, else

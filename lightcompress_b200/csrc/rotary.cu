@@ -53,7 +53,7 @@ __device__ __forceinline__ uint32_t quotient(uint32_t x, const Divider& v) { ret
 // in shared memory first.
 //
 // HBM-bound: q and k are read and written once.  What carries it is warps on the SM: 16 CTAs of 128 threads at 32 registers
-// take 89.5 us for 16384 tokens of 64 heads of 128 in bf16 (6.0 TB/s, 92 % of a copy's rate); 34 registers and 256 threads
+// take 87.4 us for 16384 tokens of 64 heads of 128 in bf16 (6.1 TB/s, 94 % of a copy's rate); 34 registers and 256 threads
 // took 102, two items a thread with their loads ahead of the angles (64 registers) 128.
 template <typename T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
 
@@ -151,8 +151,8 @@ int launch_packed(const RotaryArgs& a, cudaStream_t st) {
   sh.by_token = divider(sh.heads);
   const int64_t grid = (tokens + sh.per_cta - 1) / sh.per_cta;
   if (grid > 0x7fffffff) return LC_ERR_SHAPE;
-  // a few tokens: their items are spread over several CTAs, each of which forms the angles (16 tokens of 40 heads: 2.8 us
-  // against 5.5 on one CTA each)
+  // a few tokens: their items are spread over several CTAs, each of which forms the angles (16 tokens of 40 heads: 2.4 us
+  // in a graph, 5.5 on one CTA each)
   int64_t parts = (4 * kNumSMsB200 + grid - 1) / grid;
   const int64_t most = ((int64_t)sh.per_cta * per_token + kThreads - 1) / kThreads;
   if (parts > most) parts = most;
