@@ -48,95 +48,118 @@ struct Divider {
 };
 __device__ __forceinline__ uint32_t quotient(uint32_t x, const Divider& v) { return v.d == 1 ? x : __umulhi(x, v.m); }
 
-// V elements move as one access.  A head is R/2/V items that turn two vectors (halves) or R/V that turn the V/2 pairs of
-// one (interleaved), and (D - R)/V items that are copied; a CTA takes `per_cta` tokens, whose cosines and sines it forms
-// in shared memory first.
+// W elements move as one access, as many as the alignment of q, k and of the halves allows.  A head is R/2/W pieces of two
+// accesses that turn together (halves) or R/W pieces that turn by themselves (interleaved; R/2 pairs with W = 1), and
+// (D - R)/W that are copied; an item is up to U pieces that lie `items` pieces apart, so that narrow accesses neither cost
+// their index arithmetic each nor wait for one another (613 tokens of 20 heads of 192, of which 142 turn: 7.7 us, 9.1 with
+// U = 1).  A CTA takes `per_cta` tokens, whose places, cosines and sines it forms in shared memory first.
 //
 // HBM-bound: q and k are read and written once.  What carries it is warps on the SM: 16 CTAs of 128 threads at 32 registers
-// take 87.4 us for 16384 tokens of 64 heads of 128 in bf16 (6.1 TB/s, 94 % of a copy's rate); 34 registers and 256 threads
+// take 86.3 us for 16384 tokens of 64 heads of 128 in bf16 (6.2 TB/s, 95 % of a copy's rate); 34 registers and 256 threads
 // took 102, two items a thread with their loads ahead of the angles (64 registers) 128.
-template <typename T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
+template <typename T, int W> struct alignas(sizeof(T) * W) Pack { T v[W]; };
 
 struct Shape {
-  int per_head, turned;      // items of a head, and those among them that turn
+  int turned, copied;        // pieces of a head
+  int turned_items, per_head;
   int heads;                 // q's and k's
   int per_cta;               // tokens
   Divider by_head, by_token; // per_head; heads
 };
 
-template <typename T, int V, bool kInter>
-__global__ void __launch_bounds__(kThreads, 16) rotary_kernel(RotaryArgs a, Shape sh) {
+template <typename T, int W, int U, bool kInter>
+__global__ void __launch_bounds__(kThreads, U == 1 ? 16 : 10) rotary_kernel(RotaryArgs a, Shape sh) {
   using E = Elem<T>;
-  using P = Pack<T, V>;
+  using P = Pack<T, W>;
   extern __shared__ float2 cs[];
   begin_dependent();
   const int half = a.R / 2;
   const int64_t tok0 = (int64_t)blockIdx.x * sh.per_cta;
   const int tokens = (int)min((int64_t)sh.per_cta, a.B * a.T - tok0);
+  int2* place = reinterpret_cast<int2*>(cs + sh.per_cta * half);         // (b, t) of each token
+  for (int j = threadIdx.x; j < tokens; j += kThreads) {
+    const int64_t tok = tok0 + j, b = a.B == 1 ? 0 : tok / a.T;
+    place[j] = make_int2((int)b, (int)(tok - b * a.T));
+  }
+  __syncthreads();
   for (int j = threadIdx.x; j < tokens * half; j += kThreads) {
-    const int64_t tok = tok0 + j / half;
-    cs[j] = turn(a.positions[tok / a.T * a.pos_b + tok % a.T], a.inv_freq[j % half], a.scale);
+    const int tl = j / half;
+    cs[j] = turn(a.positions[place[tl].x * a.pos_b + place[tl].y], a.inv_freq[j - tl * half], a.scale);
   }
   __syncthreads();
   const uint32_t items = (uint32_t)(tokens * sh.heads * sh.per_head);
-#pragma unroll 2
+#pragma unroll(U == 1 ? 2 : 1)
   for (uint32_t idx = blockIdx.y * kThreads + threadIdx.x; idx < items; idx += gridDim.y * kThreads) {
-    const uint32_t th = quotient(idx, sh.by_head), i = idx - th * sh.per_head;
+    const uint32_t th = quotient(idx, sh.by_head);
+    int i = (int)(idx - th * sh.per_head);
     const uint32_t tl = quotient(th, sh.by_token);
     int head = (int)(th - tl * sh.heads);
-    const int64_t tok = tok0 + tl, b = a.B == 1 ? 0 : tok / a.T, t = tok - b * a.T;
+    const int2 at = place[tl];
     const bool is_k = head >= a.q.heads;
     const Heads& s = is_k ? a.k : a.q;
     if (is_k) head -= a.q.heads;
-    const T* in = static_cast<const T*>(s.in) + b * s.in_b + t * s.in_t + head * s.in_h;
-    T* out = static_cast<T*>(s.out) + b * s.out_b + t * s.out_t + head * s.out_h;
+    const T* in = static_cast<const T*>(s.in) + at.x * s.in_b + at.y * s.in_t + head * s.in_h;
+    T* out = static_cast<T*>(s.out) + at.x * s.out_b + at.y * s.out_t + head * s.out_h;
     const float2* w = cs + tl * half;
-    if ((int)i < sh.turned) {
-      if (kInter) {
-        const int e = (int)i * V;
-        if constexpr (V == 1) {
-          // an item is a pair
-          const float x1 = E::to_f(in[2 * e]), x2 = E::to_f(in[2 * e + 1]);
-          out[2 * e] = E::from_f(x1 * w[e].x - x2 * w[e].y);
-          out[2 * e + 1] = E::from_f(x2 * w[e].x + x1 * w[e].y);
-        } else {
-          const P x = *reinterpret_cast<const P*>(in + e);
-          P o;
+    if (i < sh.turned_items) {
+      constexpr int kStep = kInter && W == 1 ? 2 : W;        // elements from piece to piece
+      P x1[U], x2[U];
 #pragma unroll
-          for (int j = 0; j < V; j += 2) {
+      for (int u = 0; u < U; ++u) {
+        const int e = (i + u * sh.turned_items) * kStep;
+        if (U == 1 || i + u * sh.turned_items < sh.turned) {
+          x1[u] = *reinterpret_cast<const P*>(in + e);
+          if (!kInter) x2[u] = *reinterpret_cast<const P*>(in + half + e);
+          else if (W == 1) x2[u] = *reinterpret_cast<const P*>(in + e + 1);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int e = (i + u * sh.turned_items) * kStep;
+        if (U > 1 && i + u * sh.turned_items >= sh.turned) continue;
+        if constexpr (kInter && W > 1) {
+#pragma unroll
+          for (int j = 0; j < W; j += 2) {
             const float2 c = w[(e + j) / 2];
-            const float x1 = E::to_f(x.v[j]), x2 = E::to_f(x.v[j + 1]);
-            o.v[j] = E::from_f(x1 * c.x - x2 * c.y);
-            o.v[j + 1] = E::from_f(x2 * c.x + x1 * c.y);
+            const float p = E::to_f(x1[u].v[j]), q = E::to_f(x1[u].v[j + 1]);
+            x1[u].v[j] = E::from_f(p * c.x - q * c.y);
+            x1[u].v[j + 1] = E::from_f(q * c.x + p * c.y);
           }
-          *reinterpret_cast<P*>(out + e) = o;
-        }
-      } else {
-        const int e = (int)i * V;
-        const P p1 = *reinterpret_cast<const P*>(in + e), p2 = *reinterpret_cast<const P*>(in + half + e);
-        P o1, o2;
+          *reinterpret_cast<P*>(out + e) = x1[u];
+        } else {
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const float2 c = w[e + j];
-          const float x1 = E::to_f(p1.v[j]), x2 = E::to_f(p2.v[j]);
-          o1.v[j] = E::from_f(x1 * c.x - x2 * c.y);
-          o2.v[j] = E::from_f(x2 * c.x + x1 * c.y);
+          for (int j = 0; j < W; ++j) {
+            const float2 c = w[kInter ? e / 2 : e + j];
+            const float p = E::to_f(x1[u].v[j]), q = E::to_f(x2[u].v[j]);
+            x1[u].v[j] = E::from_f(p * c.x - q * c.y);
+            x2[u].v[j] = E::from_f(q * c.x + p * c.y);
+          }
+          *reinterpret_cast<P*>(out + e) = x1[u];
+          *reinterpret_cast<P*>(out + (kInter ? 1 : half) + e) = x2[u];
         }
-        *reinterpret_cast<P*>(out + e) = o1;
-        *reinterpret_cast<P*>(out + half + e) = o2;
       }
     } else {
-      const int e = a.R + ((int)i - sh.turned) * V;
-      *reinterpret_cast<P*>(out + e) = *reinterpret_cast<const P*>(in + e);
+      i -= sh.turned_items;
+      const int step = sh.per_head - sh.turned_items;
+      P x[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (U == 1 || i + u * step < sh.copied) x[u] = *reinterpret_cast<const P*>(in + a.R + (i + u * step) * W);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (U == 1 || i + u * step < sh.copied) *reinterpret_cast<P*>(out + a.R + (i + u * step) * W) = x[u];
     }
   }
 }
 
-template <typename T, int V, bool kInter>
+template <typename T, int W, bool kInter>
 int launch_packed(const RotaryArgs& a, cudaStream_t st) {
+  constexpr int kFull = Elem<T>::kPerVec / W, U = kFull < 4 ? kFull : 4;
   Shape sh;
-  sh.turned = kInter && V > 1 ? a.R / V : a.R / 2 / V;
-  sh.per_head = sh.turned + (a.D - a.R) / V;
+  sh.turned = kInter && W > 1 ? a.R / W : a.R / 2 / W;
+  sh.copied = (a.D - a.R) / W;
+  sh.turned_items = (sh.turned + U - 1) / U;
+  sh.per_head = sh.turned_items + (sh.copied + U - 1) / U;
   sh.heads = a.q.heads + a.k.heads;
   const int per_token = sh.heads * sh.per_head;
   if (sh.per_head > 1024 || per_token >= 1 << 20) return LC_ERR_SHAPE;
@@ -144,20 +167,23 @@ int launch_packed(const RotaryArgs& a, cudaStream_t st) {
   sh.per_cta = per_token >= 2 * kThreads ? 1 : (2 * kThreads + per_token - 1) / per_token;
   const int room = 2048 / (a.R / 2) > 0 ? 2048 / (a.R / 2) : 1;
   if (sh.per_cta > room) sh.per_cta = room;
-  const int64_t tokens = a.B * a.T;
-  if (sh.per_cta > tokens) sh.per_cta = (int)tokens;
+  // a few tokens: one to a CTA, or their items spread over several CTAs, each of which forms the angles -- up to the CTAs
+  // that run at once, so that the chain of angles and items is short (in a graph, of which 2.2 are a launch: 24 tokens of 2
+  // heads of 192 2.4 us, 5.8 with all in two CTAs; 613 tokens of 20 heads of 192, 142 of them turned, 9.1 us with single
+  // accesses an item, 13.6 with a quarter of the CTAs)
+  constexpr int64_t kAtOnce = 16 * kNumSMsB200;
+  const int64_t tokens = a.B * a.T, spread = (tokens + kAtOnce - 1) / kAtOnce;
+  if (sh.per_cta > spread) sh.per_cta = (int)spread;
   auto divider = [](int d) { return Divider{(uint32_t)d, (uint32_t)(((1ull << 32) + d - 1) / d)}; };
   sh.by_head = divider(sh.per_head);
   sh.by_token = divider(sh.heads);
   const int64_t grid = (tokens + sh.per_cta - 1) / sh.per_cta;
   if (grid > 0x7fffffff) return LC_ERR_SHAPE;
-  // a few tokens: their items are spread over several CTAs, each of which forms the angles (16 tokens of 40 heads: 2.4 us
-  // in a graph, 5.5 on one CTA each)
-  int64_t parts = (4 * kNumSMsB200 + grid - 1) / grid;
+  int64_t parts = (kAtOnce + grid - 1) / grid;
   const int64_t most = ((int64_t)sh.per_cta * per_token + kThreads - 1) / kThreads;
   if (parts > most) parts = most;
-  LC_CHECK_CUDA(launch_dependent(rotary_kernel<T, V, kInter>, dim3((unsigned)grid, (unsigned)parts), kThreads,
-                                 (size_t)sh.per_cta * (a.R / 2) * sizeof(float2), st, a, sh));
+  LC_CHECK_CUDA(launch_dependent(rotary_kernel<T, W, U, kInter>, dim3((unsigned)grid, (unsigned)parts), kThreads,
+                                 (size_t)sh.per_cta * (a.R / 2 * sizeof(float2) + sizeof(int2)), st, a, sh));
   LC_LAUNCH_CHECK();
   return LC_OK;
 }
@@ -180,6 +206,7 @@ template <typename T, bool kInter>
 int by_width(const RotaryArgs& a, cudaStream_t st) {
   constexpr int N = Elem<T>::kPerVec;
   if (fits<T>(a, N, kInter)) return launch_packed<T, N, kInter>(a, st);
+  if (N > 4 && fits<T>(a, 4, kInter)) return launch_packed<T, 4, kInter>(a, st);
   if (fits<T>(a, 2, kInter)) return launch_packed<T, 2, kInter>(a, st);
   return launch_packed<T, 1, kInter>(a, st);
 }
