@@ -726,33 +726,38 @@ int encode_codes(CUtensorMap* m, const int8_t* p, int64_t k, int64_t rows, int64
 }
 
 // ---- which tile, which split ---------------------------------------------------------------------------------------
-// The product of every choice is the same to the bit, so the choice is the one whose estimated time is least.  Measured
-// (us): a CTA of the first kernel takes `base` for its launch, its first copies and its finishing, and c1 for a k block
-// when it has an SM to itself, c2 when two share one; each further round of CTAs costs their finishing again; splitting K
-// adds the exchange of partial sums, and clusters do not fill every SM.  A wave of pairs takes 0.30 a block, or what its
-// finishing takes.  No choice is faster than the weights arrive from HBM.  Against the best of all choices, over M 1 -
-// 2600 and N, K 64 - 11008, the one taken was within 5 % in most cases and within 20 % in all but a few of under 8 us
-// (e.g. 256 x 4096 x 4096: 11.9 us on 64-token tiles, 16.2 on pairs; 1024 x 11008 x 4096: 36 on pairs, 50 on 128-token
-// tiles; 1 x 4096 x 11008: 12.3 with K split six ways, 21.2 without).
+// The product of every choice is the same to the bit, so the choice is the one whose estimated time is least.  Fitted to
+// measured times (us) of every choice at 378 sizes, M 1 - 6000 and N, K 64 - 11008: a CTA of the first kernel takes `base`
+// for its launch, its first copies and its finishing, and c1 for a k block when it has an SM to itself, c2 when two share
+// one, in proportion when more come; each CTA that an SM runs besides costs `share` of finishing, and `round` where its
+// shared memory lets it begin only after others; splitting K adds the exchange of partial sums.  A wave of pairs takes
+// 0.26 a block, or what its finishing takes.  No choice is faster than the weights arrive from HBM, for which many CTAs ask
+// sooner than few.  The one taken was 0.8 % behind the best in the mean, within 12 % at all but three sizes of under 9 us
+// (e.g. 24 x 4096 x 11008: 11.4 us split eight ways on 32-token tiles, 13.2 four ways on 16-token ones; 256 x 4096 x 4096:
+// 10.3 on 64-token tiles, 11.2 on 32-token ones; 1024 x 4096 x 11008: 32 on pairs, 40 on 128-token tiles).
 struct Choice {
   int tokens;      // of a tile: 16, 32, 64, 128; 256 for the pair kernel
   int splits;
 };
-// CTAs that run at once, one to an SM; clusters leave SMs of a GPC over
-constexpr int ctas_at_once(int splits) { return splits > 1 ? kNumSMsB200 - 16 : kNumSMsB200; }
+// CTAs that run at once, one to an SM; clusters leave SMs of a GPC over (15 of eight CTAs fit, 33 of four)
+constexpr int ctas_at_once(int splits) {
+  return splits <= 2 ? kNumSMsB200 : splits <= 6 ? kNumSMsB200 - 16 : kNumSMsB200 - 36;
+}
+// of clusters, two to an SM
+constexpr int kClusteredCtas = 264;
 
 Choice choose(int64_t M, int64_t N, int64_t K) {
   constexpr int kNT[4] = {16, 32, 64, 128};
-  constexpr float kBase[4] = {3.3f, 3.5f, 3.9f, 4.7f}, kC1[4] = {0.225f, 0.225f, 0.23f, 0.235f},
-                  kC2[4] = {0.32f, 0.31f, 0.33f, 0.39f}, kExchange[4] = {1.9f, 2.0f, 2.9f, 4.0f},
-                  kRound[4] = {2.0f, 2.5f, 3.0f, 4.0f};
+  constexpr float kBase[4] = {3.1f, 3.4f, 3.4f, 4.5f}, kC1[4] = {0.25f, 0.215f, 0.23f, 0.235f},
+                  kC2[4] = {0.26f, 0.315f, 0.39f, 0.41f}, kExchange[4] = {2.0f, 1.6f, 2.9f, 4.0f},
+                  kShare[4] = {0.48f, 0.385f, 0.8f, 1.06f}, kRound[4] = {0.45f, 0.6f, 1.3f, 1.0f};
   constexpr int kSplits[6] = {1, 2, 3, 4, 6, 8};
   const int64_t blocks = (K + kBlockK - 1) / kBlockK, n_tiles = (N + kRows - 1) / kRows;
-  const float arrive = 4.5f + (float)(N * K) / 6.0e6f;
+  const float arrive = 4.1f + (float)(N * K) / 6.7e6f;
   Choice best{256, 1};
   const int64_t pair_tiles = ((N + 255) / 256) * ((M + 255) / 256), halves = kNumSMsB200 / 2;
-  const float wave = (float)blocks * 0.30f;
-  float least = 6.5f + (float)((pair_tiles + halves - 1) / halves) * (wave > 3.3f ? wave : 3.3f);
+  const float wave = (float)blocks * 0.26f;
+  float least = 5.5f + (float)((pair_tiles + halves - 1) / halves) * (wave > 2.8f ? wave : 2.8f);
   if (M <= 128) least = 1e30f;
   for (int i = 0; i < 4; ++i) {
     if (i > 0 && kNT[i - 1] >= M) break;                   // half of the tile's tokens would not exist
@@ -760,12 +765,19 @@ Choice choose(int64_t M, int64_t N, int64_t K) {
     if (m_tiles > 65535) continue;                         // a grid's second dimension
     for (int sp : kSplits) {
       const int64_t ctas = tiles * sp, count = (blocks + sp - 1) / sp;
-      if (sp > 1 && (sp > blocks || ctas > (kNT[i] == 128 ? 1 : 2) * ctas_at_once(sp))) break;
-      const int64_t rounds = (ctas + 2 * kNumSMsB200 - 1) / (2 * kNumSMsB200);
-      float t = kBase[i] + (ctas <= ctas_at_once(sp) ? (float)count * kC1[i] : (float)(rounds * count) * kC2[i]) +
-                (float)(rounds - 1) * kRound[i] + (sp > 1 ? kExchange[i] : 0.f);
-      const float floor = arrive + (sp > 1 ? 0.3f * kExchange[i] : 0.f);
-      if (t < floor && N * K > (4 << 20)) t = floor + 1e-3f * t;
+      if (sp > 1 && (sp > blocks || ctas > (kNT[i] == 128 ? ctas_at_once(sp) : kClusteredCtas))) break;
+      // CTAs that an SM's shared memory holds at once: two when they have more stages than that leaves
+      const int64_t fit = kSmemMost / (count * (kWeightBytes + kNT[i] * kBlockK) + 2500);
+      const int64_t hold = fit < 2 ? 2 : fit > 4 ? 4 : fit, per_sm = (ctas + kNumSMsB200 - 1) / kNumSMsB200;
+      const int64_t rounds = (ctas + hold * kNumSMsB200 - 1) / (hold * kNumSMsB200);
+      float t = kBase[i] + (float)(rounds - 1) * kRound[i] + (sp > 1 ? kExchange[i] : 0.f);
+      if (ctas <= ctas_at_once(sp)) t += (float)count * kC1[i];
+      else t += (float)count * kC2[i] * (per_sm > 2 ? 0.5f * (float)per_sm : 1.f) + (float)(per_sm - 1) * kShare[i];
+      if (N * K > (4 << 20)) {
+        const float wait = 1.f - (float)ctas / (2.f * kNumSMsB200);
+        const float floor = arrive + (sp > 1 ? 0.24f * kExchange[i] : 0.f) + (wait > 0.f ? 0.26f * wait : 0.f);
+        if (t < floor) t = floor;
+      }
       if (t < least) {
         least = t;
         best = Choice{kNT[i], sp};
