@@ -243,7 +243,7 @@ def residual_norm(x, residual=None, weight=None, post_weight=None, gate=None, sc
     per leading index such as (B, 1, C), or x's shape; all of x's type.  residual, post_weight, gate and weight may each
     be left out; weight_offset is 1 for norms that store their weight less one.  Statistics and sums are fp32; h is
     rounded once and y is formed from the rounded h.  A row's result does not depend on the other rows; the order of its
-    sums, and so its last bits, differ between tensors whose rows all begin at 16 bytes and others.
+    sums, and so its last bits, follows the alignment that all rows have: 16 bytes, two values or one.
 
     Returns (h, y).  Without weight, y is None.  With quant, y is what int8_linear.act_quant returns for it, (codes,
     scales) or, with sym=False, (codes, scales, zeros), quantised from fp32.  Where h would equal x, it is x."""

@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(kThreads) quant_any_kernel(QuantArgs a) {
   }
 }
 
-// Rows that registers hold, by 16-byte vectors or (not aligned) by single values: read once, written once.  HBM-bound:
+// Rows that registers hold, by 16-byte vectors or, less aligned, by pairs or single values: read once, written once.  HBM-bound:
 // 16384 x 11008 in bf16 84 us (6.4 TB/s, 98 % of a copy's rate), with a zero point 92; silu(gate) * up 147 (6.1 TB/s), the
 // tanh form of gelu 158, the erf form 205, the last two bound by their arithmetic.
 template <typename T, int N, int kWarps, int kVecs, int kAct>
@@ -147,16 +147,21 @@ template <typename T, int kAct>
 bool launch_rows(const QuantArgs& a, cudaStream_t st) {
   constexpr int N = Elem<T>::kPerVec;
   if (a.rows > 0x7fffffff) return false;
-  const bool wide = a.cols % N == 0 && (a.rows == 1 || (a.ldx % N == 0 && a.ldu % N == 0 && a.ldc % N == 0)) && aligned16(a.x) &&
-                    aligned16(a.up) && (reinterpret_cast<uintptr_t>(a.codes) & (N - 1)) == 0;
+  // whether every row begins at a multiple of n values
+  auto by = [&](int n) {
+    return a.cols % n == 0 && (a.rows == 1 || (a.ldx % n == 0 && a.ldu % n == 0 && a.ldc % n == 0)) &&
+           reinterpret_cast<uintptr_t>(a.x) % (n * sizeof(T)) == 0 && reinterpret_cast<uintptr_t>(a.up) % (n * sizeof(T)) == 0 &&
+           reinterpret_cast<uintptr_t>(a.codes) % n == 0;
+  };
   auto go = [&](auto shape, auto width) {
     using S = decltype(shape);
     using G = RowGroup<S::kWarps>;
     launch_dependent(quant_rows_kernel<T, decltype(width)::value, S::kWarps, S::kVecs, kAct>,
                      dim3((unsigned)((a.rows + G::kRows - 1) / G::kRows)), G::kThreads, 0, st, a);
   };
-  return wide ? with_row_shape<false>(a.cols / N, a.rows, [&](auto s) { go(s, std::integral_constant<int, N>{}); })
-              : with_value_shape(a.cols, [&](auto s) { go(s, std::integral_constant<int, 1>{}); });
+  if (by(N)) return with_row_shape<false>(a.cols / N, a.rows, [&](auto s) { go(s, std::integral_constant<int, N>{}); });
+  if (by(2)) return with_value_shape<false>(a.cols / 2, a.rows, [&](auto s) { go(s, std::integral_constant<int, 2>{}); });
+  return with_value_shape<false>(a.cols, a.rows, [&](auto s) { go(s, std::integral_constant<int, 1>{}); });
 }
 
 template <typename T, int kAct, bool kSym>

@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(kThreads) norm_any_kernel(NormArgs a) {
   }
 }
 
-// Rows that registers hold, by 16-byte vectors or (not aligned) by single values: x, the residual and the gate are read
+// Rows that registers hold, by 16-byte vectors or, less aligned, by pairs or single values: x, the residual and the gate are read
 // once, h and y written once; the weights come from the caches.  HBM-bound: 32768 x 4096 in bf16 with both norms and a gate
 // takes 166 us, 6.5 TB/s or 99 % of a copy's rate.  A lane keeps its vectors as they lie in memory (x, then h) and unpacks
 // them where it needs them: the registers of fp32 copies cost wide rows their occupancy (2048 x 16384 with two inputs: 84
@@ -233,18 +233,24 @@ template <typename T>
 bool launch_rows(const NormArgs& a, cudaStream_t st) {
   constexpr int N = Elem<T>::kPerVec;
   if (a.rows > 0x7fffffff) return false;
-  bool wide = a.cols % N == 0 && (a.rows == 1 || (a.ldx % N == 0 && (!a.residual || a.ldr % N == 0) && (!a.codes || a.ldc % N == 0))) &&
-              (reinterpret_cast<uintptr_t>(a.codes) & (N - 1)) == 0;
-  for (const void* p : {a.x, a.residual, a.post_weight, a.gate, a.weight, (const void*)a.h, (const void*)a.y})
-    wide = wide && aligned16(p);                                       // NULL counts as aligned
+  // whether every row begins at a multiple of n values; NULL counts as one
+  auto by = [&](int n) {
+    bool fits = a.cols % n == 0 &&
+                (a.rows == 1 || (a.ldx % n == 0 && (!a.residual || a.ldr % n == 0) && (!a.codes || a.ldc % n == 0))) &&
+                reinterpret_cast<uintptr_t>(a.codes) % n == 0;
+    for (const void* p : {a.x, a.residual, a.post_weight, a.gate, a.weight, (const void*)a.h, (const void*)a.y})
+      fits = fits && reinterpret_cast<uintptr_t>(p) % (n * sizeof(T)) == 0;
+    return fits;
+  };
   auto go = [&](auto shape, auto width) {
     using S = decltype(shape);
     using G = RowGroup<S::kWarps>;
     launch_dependent(norm_rows_kernel<T, decltype(width)::value, S::kWarps, S::kVecs>,
                      dim3((unsigned)((a.rows + G::kRows - 1) / G::kRows)), G::kThreads, 0, st, a);
   };
-  return wide ? with_row_shape<true>(a.cols / N, a.rows, [&](auto s) { go(s, std::integral_constant<int, N>{}); })
-              : with_value_shape(a.cols, [&](auto s) { go(s, std::integral_constant<int, 1>{}); });
+  if (by(N)) return with_row_shape<true>(a.cols / N, a.rows, [&](auto s) { go(s, std::integral_constant<int, N>{}); });
+  if (by(2)) return with_value_shape<true>(a.cols / 2, a.rows, [&](auto s) { go(s, std::integral_constant<int, 2>{}); });
+  return with_value_shape<true>(a.cols, a.rows, [&](auto s) { go(s, std::integral_constant<int, 1>{}); });
 }
 
 template <typename T>

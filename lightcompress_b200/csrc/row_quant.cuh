@@ -129,12 +129,16 @@ __device__ __forceinline__ RowQuant row_quant_of(float mn, float mx, bool sym) {
   return sym ? row_quant<true>(0.f, nan_max(mx, -mn)) : row_quant<false>(mn, mx);
 }
 
-// the codes of N (1, 4 or 8) neighbouring values, stored at p (N-byte aligned)
+// the codes of N (1, 2, 4 or 8) neighbouring values, stored at p (N-byte aligned)
 template <int N>
 __device__ __forceinline__ void store_row_codes(int8_t* p, const float (&v)[N], const RowQuant& q, bool sym) {
   if constexpr (N == 1) {
     *p = q.bad ? (int8_t)0 : (int8_t)(sym ? row_code<true>(v[0], q) : row_code<false>(v[0], q));
     return;
+  } else if constexpr (N == 2) {
+    const int c0 = sym ? row_code<true>(v[0], q) : row_code<false>(v[0], q);
+    const int c1 = sym ? row_code<true>(v[1], q) : row_code<false>(v[1], q);
+    *reinterpret_cast<char2*>(p) = q.bad ? make_char2(0, 0) : make_char2((signed char)c0, (signed char)c1);
   } else {
   uint32_t w[N / 4];
 #pragma unroll
@@ -154,35 +158,35 @@ __device__ __forceinline__ void store_row_codes(int8_t* p, const float (&v)[N], 
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void unpack16(const uint4& v, float (&f)[Elem<T>::kPerVec]) {
-  const T* p = reinterpret_cast<const T*>(&v);
-#pragma unroll
-  for (int i = 0; i < Elem<T>::kPerVec; ++i) f[i] = Elem<T>::to_f(p[i]);
-}
-
-// N neighbouring values as they lie in memory: a 16-byte vector, held as four whole registers, or one value where rows are
-// not aligned to more (a warp still reads 64 or 128 contiguous bytes at once).
+// N neighbouring values as they lie in memory: a 16-byte vector, held as four whole registers, or two values or one where
+// rows are not aligned to more (a warp still reads 64 to 256 contiguous bytes at once).
 template <typename T, int N> struct RawOf { typedef uint4 type; };
 template <typename T> struct RawOf<T, 1> { typedef T type; };
+template <typename T> struct RawOf<T, 2> { typedef uint32_t type; };
+template <> struct RawOf<float, 2> { typedef uint2 type; };
 template <typename T, int N> using Raw = typename RawOf<T, N>::type;
 
 template <typename T, int N>
 __device__ __forceinline__ Raw<T, N> load_stream(const T* p) {             // read once
   if constexpr (N == 1) return *p;
-  else return __ldcs(reinterpret_cast<const uint4*>(p));
+  else return __ldcs(reinterpret_cast<const Raw<T, N>*>(p));
 }
 template <typename T, int N>
 __device__ __forceinline__ void unpack(const Raw<T, N>& r, float (&f)[N]) {
-  if constexpr (N == 1) f[0] = Elem<T>::to_f(r);
-  else unpack16<T>(r, f);
+  if constexpr (N == 1) {
+    f[0] = Elem<T>::to_f(r);
+  } else {
+    const T* p = reinterpret_cast<const T*>(&r);
+#pragma unroll
+    for (int i = 0; i < N; ++i) f[i] = Elem<T>::to_f(p[i]);
+  }
 }
 template <typename T, int N>
 __device__ __forceinline__ Raw<T, N> pack(const float (&f)[N]) {
   if constexpr (N == 1) {
     return Elem<T>::from_f(f[0]);
   } else {
-    uint4 r;
+    Raw<T, N> r;
     T* p = reinterpret_cast<T*>(&r);
 #pragma unroll
     for (int i = 0; i < N; ++i) p[i] = Elem<T>::from_f(f[i]);
@@ -218,15 +222,22 @@ bool with_row_shape(int64_t vecs, int64_t rows, F&& f) {
   else return false;
   return true;
 }
-// the same for rows of single values
-template <typename F>
-bool with_value_shape(int64_t cols, F&& f) {
-  if (cols <= 128) f(RowShape<1, 4>{});
-  else if (cols <= 512) f(RowShape<1, 16>{});
-  else if (cols <= 2048) f(RowShape<4, 16>{});
-  else if (cols <= 4096) f(RowShape<8, 16>{});
-  else if (cols <= 8192) f(RowShape<16, 16>{});
-  else if (cols <= 16384) f(RowShape<16, 32>{});
+// The same for rows of pairs or single values, where what takes long is how many small accesses a lane makes (norms of 19
+// rows of 4092 in bf16: 3.9 us by pairs, 5.6 by single values; 2048 rows of 4094: 14.8 and 20.6; 10 rows of 1794 quantised
+// on 8 x 4 1.5, on 4 x 16 1.9).
+template <bool kNorm, typename F>
+bool with_value_shape(int64_t units, int64_t rows, F&& f) {
+  const bool few = !kNorm && rows <= kNumSMsB200;
+  if (units <= 128) f(RowShape<1, 4>{});
+  else if (units <= 512) f(RowShape<4, 4>{});
+  else if (units <= 1024 && few) f(RowShape<8, 4>{});
+  else if (units <= 1024) f(RowShape<4, 8>{});
+  else if (units <= 2048 && few) f(RowShape<16, 4>{});
+  else if (units <= 2048) f(RowShape<8, 8>{});
+  else if (units <= 4096 && few) f(RowShape<16, 8>{});
+  else if (units <= 4096) f(RowShape<8, 16>{});
+  else if (units <= 8192) f(RowShape<16, 16>{});
+  else if (units <= 16384) f(RowShape<16, 32>{});
   else return false;
   return true;
 }

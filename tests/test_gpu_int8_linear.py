@@ -354,3 +354,20 @@ def test_module_from_a_quantised_linear():
         Int8Linear.new(lin, RTN(asym).w_q, asym)
     with pytest.raises(NotImplementedError):
         Int8Linear.new(lin, RTN(wq).w_q, wq, IntegerQuantizer(4, True, 'per_token'))
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('shape', [(3, 2), (9, 6), (17, 129), (200, 254), (4, 1022), (150, 1026), (149, 2046), (3, 2047), (4, 4094),
+                                   (150, 4095), (2, 8190), (2, 16382), (2, 16385), (1, 32766), (2, 32770)])
+def test_codes_of_rows_that_begin_anywhere(dtype, shape):
+    for sym in (True, False):
+        test_codes_are_the_definition_to_the_bit(dtype, sym, shape)
+    for act in ('silu', 'gelu', 'gelu_tanh'):
+        test_gated_quantisation(dtype, act, *shape, True)
+    test_gated_quantisation(dtype, 'silu', *shape, False)
+
+
+@pytest.mark.parametrize('m,n,k', [(24, 4096, 11008), (232, 256, 9600), (51, 512, 7040), (7, 179, 1189), (2400, 1280, 128),
+                                   (1837, 268, 528), (1250, 256, 4224), (139, 384, 1792), (25, 2048, 6144)])
+def test_product_in_many_small_blocks_and_large_clusters(m, n, k):
+    test_product_is_exact(m, n, k)

@@ -160,3 +160,30 @@ def test_a_row_does_not_depend_on_the_others(dtype, c):
         _, ys = residual_norm(x[rows], res[rows], weight=w, post_weight=w)
         assert torch.equal(hs, h[rows]) and torch.equal(ys, y[rows])
         assert torch.equal(qs[0], q[0][rows]) and torch.equal(qs[1], q[1][rows])
+
+
+# Rows by pairs and by single values on every shape that holds them, and just beyond the widest
+NARROW = [(3, 2), (9, 6), (17, 129), (200, 254), (5, 511), (4, 1022), (3, 1023), (150, 1026), (149, 2046), (3, 2047), (4, 4094),
+          (150, 4095), (2, 8190), (2, 8191), (2, 16382), (2, 16385), (1, 32766), (2, 32770)]
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('shape', NARROW)
+def test_rows_that_begin_anywhere(dtype, shape):
+    test_residual_norm(dtype, shape)
+    test_quantised_form(dtype, True, shape)
+    test_quantised_form(dtype, False, shape)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('first', [1, 2, 3, 4])
+def test_rows_of_a_slice(dtype, first):
+    """Rows of 1020 of 1030 values: every other way in which a row may lie, inputs alike and not."""
+    from lightcompress_b200.block_ops import residual_norm
+    wide, other = _data((5, 1030), dtype, 1), _data((5, 1030), dtype, 2)
+    w, post = _data((1020,), dtype, 3), _data((1020,), dtype, 4)
+    x = wide.cuda()[:, first:first + 1020]
+    for start in (first, 0):
+        res = other.cuda()[:, start:start + 1020]
+        h, y = residual_norm(x, res, weight=w.cuda(), post_weight=post.cuda())
+        _check(h, y, x.cpu(), res.cpu(), w, post, None, 1.0, 1e-6, 0.0)

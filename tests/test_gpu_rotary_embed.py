@@ -126,3 +126,26 @@ def test_agrees_with_the_table_kernel_and_empty_and_captured():
         want = rotary_embed(x, x[:, :1], pos + 1000 * i, freq)
         torch.cuda.synchronize()
         assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
+# Heads whose halves lie at multiples of 1, 2, 4 and 8 values, with pieces that do not fill their items, and batches whose
+# tokens share a block or have several
+NARROW = [(1, 16, 4, 61, 192, 142), (4, 16, 4, 27, 160, 44), (3, 8, 4, 19, 220, 220), (2, 16, 8, 9, 166, 150), (3, 4, 1, 101, 168, 140),
+          (8, 1, 1, 26, 214, 214), (5, 2, 1, 500, 24, 8), (3, 1, 1, 8, 192, 192), (2, 3, 1, 700, 14, 2), (4, 5, 5, 3, 98, 98),
+          (1, 1, 1, 5000, 64, 12), (2, 900, 100, 2, 12, 4), (1, 3, 2, 2, 1023, 1022), (7, 2, 2, 350, 22, 20)]
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('inter', [False, True])
+@pytest.mark.parametrize('b,h,g,t,d,r', NARROW)
+def test_heads_that_lie_anyhow(dtype, inter, b, h, g, t, d, r):
+    from lightcompress_b200.block_ops import rope_frequencies, rotary_embed
+    test_rotary(dtype, inter, b, h, g, t, d, r)
+    # in place, and as parts of one projection's output
+    freq, _ = rope_frequencies(r, device='cpu')
+    pos = torch.arange(t) + 3
+    qk = _heads(b, h + g, t, d, dtype, 9)
+    on = qk.transpose(1, 2).contiguous().cuda().transpose(1, 2)
+    oq, ok = rotary_embed(on[:, :h], on[:, h:], pos.cuda(), freq.cuda(), inter, inplace=True)
+    _check(oq, qk[:, :h], pos, freq, inter, 1.0)
+    _check(ok, qk[:, h:], pos, freq, inter, 1.0)
