@@ -83,9 +83,9 @@ __global__ void __launch_bounds__(kThreads) quant_any_kernel(QuantArgs a) {
   }
 }
 
-// Rows that registers hold, by 16-byte vectors or, less aligned, by pairs or single values: read once, written once.  HBM-bound:
-// 16384 x 11008 in bf16 84 us (6.4 TB/s, 98 % of a copy's rate), with a zero point 92; silu(gate) * up 147 (6.1 TB/s), the
-// tanh form of gelu 158, the erf form 205, the last two bound by their arithmetic.
+// Rows that registers hold, by 16-byte vectors or, less aligned, by pairs or single values: read once, written once.
+// HBM-bound: 16384 x 11008 in bf16 84 us (6.4 TB/s, 98 % of a copy's rate), with a zero point 92; silu(gate) * up 147 (6.1
+// TB/s), the tanh form of gelu 158, the erf form 205, the last two bound by their arithmetic.
 template <typename T, int N, int kWarps, int kVecs, int kAct>
 __global__ void __launch_bounds__(RowGroup<kWarps>::kThreads) quant_rows_kernel(QuantArgs a) {
   using G = RowGroup<kWarps>;

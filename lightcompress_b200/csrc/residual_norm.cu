@@ -106,12 +106,12 @@ __global__ void __launch_bounds__(kThreads) norm_any_kernel(NormArgs a) {
   }
 }
 
-// Rows that registers hold, by 16-byte vectors or, less aligned, by pairs or single values: x, the residual and the gate are read
-// once, h and y written once; the weights come from the caches.  HBM-bound: 32768 x 4096 in bf16 with both norms and a gate
-// takes 166 us, 6.5 TB/s or 99 % of a copy's rate.  A lane keeps its vectors as they lie in memory (x, then h) and unpacks
+// Rows that registers hold, by 16-byte vectors or, less aligned, by pairs or single values: x, the residual and the gate are
+// read once, h and y written once; the weights come from the caches.  HBM-bound: 32768 x 4096 in bf16 with both norms and a gate
+// takes 165 us, 6.5 TB/s or 99 % of a copy's rate.  A lane keeps its vectors as they lie in memory (x, then h) and unpacks
 // them where it needs them: the registers of fp32 copies cost wide rows their occupancy (2048 x 16384 with two inputs: 84
 // us, 51 this way).
-template <typename T, int N, int kWarps, int kVecs>
+template <typename T, int N, int kWarps, int kVecs, bool kCodes>
 __global__ void __launch_bounds__(RowGroup<kWarps>::kThreads) norm_rows_kernel(NormArgs a) {
   using G = RowGroup<kWarps>;
   using P = Raw<T, N>;
@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(RowGroup<kWarps>::kThreads) norm_rows_kernel(N
 #pragma unroll
     for (int j = 0; j < N; ++j) v[j] = v[j] * pre * (f[j] + a.offset);
   };
-  if (a.y) {
+  if (!kCodes || a.y) {
     P* y = reinterpret_cast<P*>(static_cast<T*>(a.y) + row * a.cols);
 #pragma unroll
     for (int k = 0; k < kVecs; ++k) {
@@ -197,34 +197,38 @@ __global__ void __launch_bounds__(RowGroup<kWarps>::kThreads) norm_rows_kernel(N
       }
     }
   }
-  if (!a.codes) return;
-  const bool sym = a.zeros == nullptr;
-  float mn = 0.f, mx = 0.f;
+  if constexpr (kCodes) {
+    // kept in fp32 from the range to the codes where registers hold them, else formed again (2048 x 4096 in bf16: 12.3 us,
+    // 12.8 with all formed again; 19 x 4092 3.2 and 3.7)
+    constexpr bool kHold = kVecs * N <= 32;
+    const bool sym = a.zeros == nullptr;
+    float mn = 0.f, mx = 0.f, held[kHold ? kVecs : 1][N];
 #pragma unroll
-  for (int k = 0; k < kVecs; ++k) {
-    const int i = G::lane() + k * G::kLanes;
-    if (i < vecs) {
-      float v[N];
-      normed(k, i, v);
+    for (int k = 0; k < kVecs; ++k) {
+      const int i = G::lane() + k * G::kLanes;
+      if (i < vecs) {
+        float(&v)[N] = held[kHold ? k : 0];
+        normed(k, i, v);
 #pragma unroll
-      for (int j = 0; j < N; ++j) mx = nan_max(mx, v[j]), mn = nan_min(mn, v[j]);
+        for (int j = 0; j < N; ++j) mx = nan_max(mx, v[j]), mn = nan_min(mn, v[j]);
+      }
     }
-  }
-  G::range(mn, mx, red + 2 * kWarps);
-  const RowQuant q = row_quant_of(mn, mx, sym);
-  int8_t* out = a.codes + row * a.ldc;
+    G::range(mn, mx, red + 2 * kWarps);
+    const RowQuant q = row_quant_of(mn, mx, sym);
+    int8_t* out = a.codes + row * a.ldc;
 #pragma unroll
-  for (int k = 0; k < kVecs; ++k) {
-    const int i = G::lane() + k * G::kLanes;
-    if (i < vecs) {
-      float v[N];
-      normed(k, i, v);
-      store_row_codes<N>(out + i * N, v, q, sym);
+    for (int k = 0; k < kVecs; ++k) {
+      const int i = G::lane() + k * G::kLanes;
+      if (i < vecs) {
+        float(&v)[N] = held[kHold ? k : 0];
+        if (!kHold) normed(k, i, v);
+        store_row_codes<N>(out + i * N, v, q, sym);
+      }
     }
-  }
-  if (G::lane() == 0) {
-    a.scales[row] = q.s;
-    if (!sym) a.zeros[row] = q.z;
+    if (G::lane() == 0) {
+      a.scales[row] = q.s;
+      if (!sym) a.zeros[row] = q.z;
+    }
   }
 }
 
@@ -245,8 +249,10 @@ bool launch_rows(const NormArgs& a, cudaStream_t st) {
   auto go = [&](auto shape, auto width) {
     using S = decltype(shape);
     using G = RowGroup<S::kWarps>;
-    launch_dependent(norm_rows_kernel<T, decltype(width)::value, S::kWarps, S::kVecs>,
-                     dim3((unsigned)((a.rows + G::kRows - 1) / G::kRows)), G::kThreads, 0, st, a);
+    const dim3 grid((unsigned)((a.rows + G::kRows - 1) / G::kRows));
+    constexpr int kWidth = decltype(width)::value;
+    if (a.codes) launch_dependent(norm_rows_kernel<T, kWidth, S::kWarps, S::kVecs, true>, grid, G::kThreads, 0, st, a);
+    else launch_dependent(norm_rows_kernel<T, kWidth, S::kWarps, S::kVecs, false>, grid, G::kThreads, 0, st, a);
   };
   if (by(N)) return with_row_shape<true>(a.cols / N, a.rows, [&](auto s) { go(s, std::integral_constant<int, N>{}); });
   if (by(2)) return with_value_shape<true>(a.cols / 2, a.rows, [&](auto s) { go(s, std::integral_constant<int, 2>{}); });

@@ -187,3 +187,28 @@ def test_rows_of_a_slice(dtype, first):
         res = other.cuda()[:, start:start + 1020]
         h, y = residual_norm(x, res, weight=w.cuda(), post_weight=post.cuda())
         _check(h, y, x.cpu(), res.cpu(), w, post, None, 1.0, 1e-6, 0.0)
+
+
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('shape', [(5, 4096), (3, 1022), (7, 129), (2, 16384), (2, 40001)])
+def test_both_forms_of_the_norm_in_one_call(dtype, shape):
+    """The C interface gives y and its codes together: the same bits as either alone."""
+    from lightcompress_b200 import _lib as L
+    from lightcompress_b200.block_ops import residual_norm
+    rows, c = shape
+    x, res, w = _data(shape, dtype, 1).cuda(), _data(shape, dtype, 2).cuda(), _data((c,), dtype, 3).cuda()
+    for sym in (True, False):
+        want_h, want_y = residual_norm(x, res, weight=w, scale=0.3)
+        _, q = residual_norm(x, res, weight=w, scale=0.3, quant=True, sym=sym)
+        h, y = torch.empty_like(x), torch.empty_like(x)
+        ldc = (c + 15) // 16 * 16
+        codes = torch.empty(rows, ldc, dtype=torch.int8, device='cuda')
+        scales = torch.empty(rows, device='cuda')
+        zeros = torch.empty(rows, dtype=torch.int32, device='cuda')
+        L.launch(0, 'lc_residual_norm', L.RESIDUAL_NORM.pack(
+            x.data_ptr(), res.data_ptr(), 0, 0, 0, w.data_ptr(), L._DTYPES[dtype], rows, c, c, c, 0.3, 1e-6, 0.0, h.data_ptr(),
+            y.data_ptr(), codes.data_ptr(), ldc, scales.data_ptr(), 0 if sym else zeros.data_ptr()))
+        assert torch.equal(h, want_h) and torch.equal(y, want_y)
+        assert torch.equal(codes[:, :c], q[0]) and torch.equal(scales, q[1].flatten())
+        if not sym:
+            assert torch.equal(zeros, q[2].flatten())
