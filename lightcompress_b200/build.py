@@ -74,7 +74,7 @@ def build(force=False, verbose=False):
         run(['g++', '-O2', '-std=c++17', '-fPIC', '-shared', '-fvisibility=hidden', '-Wall',
              '-I' + sysconfig.get_path('include'), '-I' + os.path.join(torch, 'include'),
              '-I' + os.path.join(torch, 'include', 'torch', 'csrc', 'api', 'include'), '-I' + cuda, CALLS_SRC, '-o', CALLS,
-             '-L' + os.path.join(torch, 'lib'), '-ltorch_python', '-ltorch_cpu', '-ltorch', '-lc10', '-lc10_cuda',
+             '-L' + os.path.join(torch, 'lib'), '-ltorch_python', '-ltorch_cpu', '-ltorch_cuda', '-ltorch', '-lc10', '-lc10_cuda',
              '-L' + HERE, '-l:' + os.path.basename(LIB), '-Wl,-rpath,$ORIGIN'])
     return LIB
 
