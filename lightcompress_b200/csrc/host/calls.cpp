@@ -249,16 +249,17 @@ int64_t gate_rows_of(const at::Tensor& gate, const at::Tensor& x) {
 // (x, residual, weight, post_weight, gate, scale, eps, weight_offset, quant, sym)
 bool residual_norm(PyObject* const* o, Py_ssize_t n, PyObject** out) {
   if (n != 10) return false;
-  const at::Tensor* t[5];
+  const at::Tensor *x = tensor_of(o[0]), *t[5] = {x};
   Place place;
   lc_stream_t st;
-  for (int i = 0; i < 5; ++i) {
+  if (!x || !place.take(*x)) return false;                 // x is compared with below: it may not be left out
+  for (int i = 1; i < 5; ++i) {
     t[i] = o[i] == Py_None ? nullptr : tensor_of(o[i]);
-    if (o[i] != Py_None && (!t[i] || !place.take(*t[i]) || t[i]->scalar_type() != t[0]->scalar_type())) return false;
+    if (o[i] != Py_None && (!t[i] || !place.take(*t[i]) || t[i]->scalar_type() != x->scalar_type())) return false;
   }
-  const at::Tensor *x = t[0], *res = t[1], *w = t[2], *pw = t[3], *gate = t[4];
+  const at::Tensor *res = t[1], *w = t[2], *pw = t[3], *gate = t[4];
   Rows rx, rr;
-  if (!x || dtype_of(*x) < 0 || !rows_of(*x, &rx)) return false;
+  if (dtype_of(*x) < 0 || !rows_of(*x, &rx)) return false;
   if (res && (res->sizes() != x->sizes() || !rows_of(*res, &rr))) return false;
   for (const at::Tensor* v : {w, pw})
     if (v && (v->dim() != 1 || !vector_of(*v, x->scalar_type(), rx.cols))) return false;
