@@ -88,6 +88,7 @@ SIGNATURES = {
     'lc_int8_gemm': [_s, _p],
     'lc_int8_linear_scratch': [_i64, _i64],
     'lc_int8_linear': [_s, _p],
+    'lc_selftest_int8_wait': [_p, _p, _p],
     'lc_residual_norm': [_s, _p],
     'lc_rotary_embed': [_s, _p],
     'lc_awq_clip_search': [_p, _p, _i, _i64, _i64, _i64, _i64, _i64, _i, _i, _i, _i, _d, _p, _p, _p, _p],

@@ -135,6 +135,11 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
   *abort_flag = 1;
   return false;
 }
+// The same for a whole converged warp, with one answer for all of its lanes: each lane reads the clock and the flag for
+// itself, and lanes that went separate ways would wait for one another at the next instruction that wants the whole warp.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, bar_wait(bar, parity, abort_flag));
+}
 
 // kind::i8: D s32, A and B s8, both K-major
 __host__ __device__ constexpr uint32_t idesc_i8(int m, int n) {
@@ -382,7 +387,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
     const uint64_t dw0 = make_desc_mn_sw128(base, 16, 1024);
     const uint64_t dx0 = make_desc_mn_sw128(base + (kQuant ? Smem::codes(stages) : kWeightBytes), 16, 1024);
     for (int i = 0; i < count; ++i) {
-      if (!bar_wait(full_bar(s), ph, abort_flag)) break;
+      if (!warp_wait(full_bar(s), ph, abort_flag)) break;
       tcgen05_fence_after();
       const uint64_t at = (uint64_t)(s * (kStage >> 4)), xat = kQuant ? (uint64_t)(i * (NT * kBlockK >> 4)) : at;
       if (elect_one()) {
@@ -400,6 +405,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
   // the accumulator (or, after an expired wait, the retirement of what was issued)
   if (!bar_wait(acc_bar, 0, abort_flag))
     for (uint32_t it = 0; it < kSpinLimit && !mbar_test(acc_bar, 0); ++it) __nanosleep(50);
+  __syncwarp();
   tcgen05_fence_after();
   __syncthreads();
   bool ok = *abort_flag == 0;
@@ -626,11 +632,11 @@ pair_kernel(const __grid_constant__ Maps maps, Int8Args g, PairTiles pt) {
       bool ok = true;
       const uint64_t dw0 = make_desc_mn_sw128(base, 16, 1024), dx0 = make_desc_mn_sw128(base + kHalfBytes, 16, 1024);
       for (int t = pair; ok && t < tiles; t += pairs) {
-        if (!bar_wait(acc_empty(buf), aph, abort_flag)) break;
+        if (!warp_wait(acc_empty(buf), aph, abort_flag)) break;
         tcgen05_fence_after();
         const uint32_t acc = tmem + (uint32_t)(buf * kPairTokens);
         for (int kb = 0; kb < blocks; ++kb) {
-          if (!bar_wait(full_bar(s), ph, abort_flag)) { ok = false; break; }
+          if (!warp_wait(full_bar(s), ph, abort_flag)) { ok = false; break; }
           tcgen05_fence_after();
           const uint64_t at = (uint64_t)(s * (kPairStageBytes >> 4));
           if (elect_one()) {
@@ -646,7 +652,7 @@ pair_kernel(const __grid_constant__ Maps maps, Int8Args g, PairTiles pt) {
         __syncwarp();
         if (++buf == kPairBufs) buf = 0, aph ^= 1u;
       }
-      if (*abort_flag) {
+      if (__any_sync(0xffffffffu, *abort_flag)) {
         // the MMAs already issued retire before the tensor memory is freed
         if (elect_one()) umma_commit_pair(retired);
         for (uint32_t it = 0; it < kSpinLimit && !mbar_test(retired, 0); ++it) __nanosleep(50);
@@ -673,7 +679,7 @@ pair_kernel(const __grid_constant__ Maps maps, Int8Args g, PairTiles pt) {
       }
       __syncwarp();
       // once a wait has expired, the tiles that remain are written as NaN
-      ok = ok && bar_wait(acc_full(buf), aph, abort_flag) && *abort_flag == 0;
+      ok = ok && warp_wait(acc_full(buf), aph, abort_flag) && __all_sync(0xffffffffu, *abort_flag == 0);
       tcgen05_fence_after();
       const uint32_t taddr = tmem + (uint32_t)(buf * kPairTokens + h * 128) + ((uint32_t)(q * 32) << 16);
       T* out = static_cast<T*>(g.c) + (int64_t)mt * g.N + n;
@@ -709,6 +715,41 @@ pair_kernel(const __grid_constant__ Maps maps, Int8Args g, PairTiles pt) {
   if (warp == 1)
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)(kPairBufs * kPairTokens))
                  : "memory");
+}
+
+// Self-test of warp_wait.  Nothing arrives on bars[1]; half of the lanes wait on bars[0], whose phase is over, half on
+// bars[1], and the flag is raised by another warp a millisecond later: no lane may report the stage as there.  Then a wait on
+// bars[0] by all lanes, which succeeds although the flag is raised, and one on bars[1], which the flag ends.
+__global__ void wait_selftest_kernel(int32_t* status, uint32_t* answers) {
+  __shared__ uint64_t bars[2];
+  __shared__ int flag;
+  volatile int* abort_flag = &flag;
+  if (threadIdx.x == 0) {
+    mbar_init(smem_u32(bars), 1);
+    mbar_init(smem_u32(bars + 1), 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    mbar_arrive(smem_u32(bars));
+  }
+  __syncthreads();
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x >= 32) {
+    if (lane == 0) {
+      for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+      *abort_flag = 1;
+    }
+    return;
+  }
+  const bool some = warp_wait(smem_u32(bars + (lane & 1)), 0, abort_flag);
+  const uint32_t a = __ballot_sync(0xffffffffu, some);
+  const bool there = warp_wait(smem_u32(bars), 0, abort_flag);
+  const uint32_t b = __ballot_sync(0xffffffffu, there);
+  const bool never = warp_wait(smem_u32(bars + 1), 0, abort_flag);
+  const uint32_t c = __ballot_sync(0xffffffffu, never);
+  if (lane == 0) {
+    answers[0] = a, answers[1] = b, answers[2] = c;
+    if (*abort_flag) atomicExch(status, (int)LC_ERR_TIMEOUT);
+  }
 }
 
 int encode_codes(CUtensorMap* m, const int8_t* p, int64_t k, int64_t rows, int64_t ld, int box_rows) {
@@ -953,4 +994,12 @@ extern "C" LC_API int lc_int8_linear(const lc_int8_linear_args* args_host, lc_st
   if ((rc = int8_quant_rows(p.x, dtype, p.M, p.K, p.ldx, codes, lda, a_s, a_z, st)) != LC_OK) return rc;
   g.a = codes, g.lda = lda, g.a_s = a_s, g.a_z = a_z;
   return product(g, dtype, st);
+}
+
+extern "C" LC_API int lc_selftest_int8_wait(int32_t* status, uint32_t* answers, lc_stream_t stream) {
+  using namespace lc;
+  if (!status || !answers) return LC_ERR_ARG;
+  wait_selftest_kernel<<<1, 64, 0, reinterpret_cast<cudaStream_t>(stream)>>>(status, answers);
+  LC_LAUNCH_CHECK();
+  return LC_OK;
 }
