@@ -658,8 +658,9 @@ typedef struct {
 int lc_int8_linear(const lc_int8_linear_args* args_host, lc_stream_t stream);
 
 /* Self-test of the products' bounded waits: a warp whose lanes see different outcomes, one that finds what it waits for, and
- * one whose wait another warp ends.  answers[3] (device) receives the lanes that took each wait for a success (0,
- * 0xffffffff, 0), *status LC_ERR_TIMEOUT.  Takes about a millisecond. */
+ * one whose wait another warp ends: answers[3] (device) receives the lanes that took each wait for a success (0,
+ * 0xffffffff, 0), status[0] LC_ERR_TIMEOUT.  Then a wait that runs out in a thread other than the reporting one: status[1]
+ * receives LC_ERR_TIMEOUT as well.  Takes about a second. */
 int lc_selftest_int8_wait(int32_t* status, uint32_t* answers, lc_stream_t stream);
 
 /* The residual add of a decoder block with the norms on both sides of it:

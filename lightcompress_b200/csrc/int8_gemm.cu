@@ -141,6 +141,12 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
   return __all_sync(0xffffffffu, bar_wait(bar, parity, abort_flag));
 }
 
+// Called by every thread behind a barrier of the CTA: a wait that any thread of it gave up is reported, also where the
+// thread that reports found what it waited for itself.
+__device__ __forceinline__ void report_lost(int32_t* status, volatile int* abort_flag) {
+  if (threadIdx.x == 0 && *abort_flag && status) atomicExch(status, (int)LC_ERR_TIMEOUT);
+}
+
 // kind::i8: D s32, A and B s8, both K-major
 __host__ __device__ constexpr uint32_t idesc_i8(int m, int n) {
   return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
@@ -500,7 +506,7 @@ __global__ void __launch_bounds__(kStreamThreads) stream_kernel(const __grid_con
   tcgen05_fence_after();
   if (warp == 1)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)kCols) : "memory");
-  if (threadIdx.x == 0 && !ok && g.status) atomicExch(g.status, (int)LC_ERR_TIMEOUT);
+  report_lost(g.status, abort_flag);
 }
 
 // ---- large products: two SMs on one 256 x 256 tile ---------------------------------------------------------------
@@ -706,7 +712,7 @@ pair_kernel(const __grid_constant__ Maps maps, Int8Args g, PairTiles pt) {
       for (uint32_t it = 0; it < kSpinLimit && !mbar_test(full_bar(i % kPairStages), (i / kPairStages) & 1u); ++it)
         __nanosleep(50);
   }
-  if (lost && threadIdx.x == 0 && g.status) atomicExch(g.status, (int)LC_ERR_TIMEOUT);
+  report_lost(g.status, abort_flag);
   tcgen05_fence_before();
   __syncthreads();
   cluster_arrive();
@@ -733,23 +739,41 @@ __global__ void wait_selftest_kernel(int32_t* status, uint32_t* answers) {
   }
   __syncthreads();
   const int lane = threadIdx.x & 31;
-  if (threadIdx.x >= 32) {
+  if (threadIdx.x < 32) {
     if (lane == 0) {
       for (int i = 0; i < 1000; ++i) __nanosleep(1000);
       *abort_flag = 1;
     }
-    return;
+  } else {
+    const bool some = warp_wait(smem_u32(bars + (lane & 1)), 0, abort_flag);
+    const uint32_t a = __ballot_sync(0xffffffffu, some);
+    const bool there = warp_wait(smem_u32(bars), 0, abort_flag);
+    const uint32_t b = __ballot_sync(0xffffffffu, there);
+    const bool never = warp_wait(smem_u32(bars + 1), 0, abort_flag);
+    const uint32_t c = __ballot_sync(0xffffffffu, never);
+    if (lane == 0) answers[0] = a, answers[1] = b, answers[2] = c;
   }
-  const bool some = warp_wait(smem_u32(bars + (lane & 1)), 0, abort_flag);
-  const uint32_t a = __ballot_sync(0xffffffffu, some);
-  const bool there = warp_wait(smem_u32(bars), 0, abort_flag);
-  const uint32_t b = __ballot_sync(0xffffffffu, there);
-  const bool never = warp_wait(smem_u32(bars + 1), 0, abort_flag);
-  const uint32_t c = __ballot_sync(0xffffffffu, never);
-  if (lane == 0) {
-    answers[0] = a, answers[1] = b, answers[2] = c;
-    if (*abort_flag) atomicExch(status, (int)LC_ERR_TIMEOUT);
+  __syncthreads();
+  report_lost(status, abort_flag);
+}
+
+// Self-test of report_lost: the last thread's wait is given up, the reporting thread's succeeds.
+__global__ void report_selftest_kernel(int32_t* status) {
+  __shared__ uint64_t bars[2];
+  __shared__ int flag;
+  volatile int* abort_flag = &flag;
+  if (threadIdx.x == 0) {
+    mbar_init(smem_u32(bars), 1);
+    mbar_init(smem_u32(bars + 1), 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    mbar_arrive(smem_u32(bars));
   }
+  __syncthreads();
+  if (threadIdx.x != blockDim.x - 1) bar_wait(smem_u32(bars), 0, abort_flag);
+  else bar_wait(smem_u32(bars + 1), 0, abort_flag);
+  __syncthreads();
+  report_lost(status, abort_flag);
 }
 
 int encode_codes(CUtensorMap* m, const int8_t* p, int64_t k, int64_t rows, int64_t ld, int box_rows) {
@@ -1000,6 +1024,7 @@ extern "C" LC_API int lc_selftest_int8_wait(int32_t* status, uint32_t* answers, 
   using namespace lc;
   if (!status || !answers) return LC_ERR_ARG;
   wait_selftest_kernel<<<1, 64, 0, reinterpret_cast<cudaStream_t>(stream)>>>(status, answers);
+  report_selftest_kernel<<<1, 96, 0, reinterpret_cast<cudaStream_t>(stream)>>>(status + 1);
   LC_LAUNCH_CHECK();
   return LC_OK;
 }
