@@ -691,7 +691,8 @@ int lc_residual_norm(const lc_residual_norm_args* args_host, lc_stream_t stream)
  * (i, i + rotary_dim / 2), or (2i, 2i + 1) when interleaved; the other elements of the head are copied.  The angle is
  * formed in fp64, so that far positions (|position| < 2^31) lose nothing; results are rounded once.
  *   q, k        element (b, t, h, d) at [b * q_b + t * q_t + h * q_h + d]; k_heads 0: no k
- *   q_out       (batch, tokens, heads, head_dim) without gaps, or q itself (in place, q's strides); k_out likewise
+ *   q_out       (batch, tokens, heads, head_dim) without gaps, or q itself (in place, q's strides, no element of memory in
+ *               two heads of q and k); k_out likewise
  *   positions   int64, (b, t) at [b * pos_b + t] (pos_b 0: one row for all);  inv_freq: rotary_dim / 2 fp32
  * at most 1023 heads of q and k together, head_dim at most 1024. */
 typedef struct {

@@ -15,6 +15,7 @@ it, a gate and a multiplier, and the 8-bit quantisation the next integer linear 
 (rotary positions from inv_freq: both pair layouts, part of a head, scaled frequencies).
 """
 import contextlib
+import functools
 import math
 import sys
 
@@ -326,7 +327,8 @@ def rotary_embed(q, k, positions, inv_freq, interleaved=False, attention_scale=1
 
     q, k: bf16, fp16 or fp32 with contiguous heads (any other strides, e.g. views of one projection's output);
     positions: int64, (B, T), (1, T) or (T,); inv_freq: (R / 2,) fp32, see rope_frequencies.  Returns (q, k) in new memory,
-    (B, T, H, D) contiguous seen as (B, H, T, D) like the stock projections, or the given tensors if inplace."""
+    (B, T, H, D) contiguous seen as (B, H, T, D) like the stock projections, or the given tensors if inplace; in place, no two
+    heads may share elements."""
     out = None if inplace else _calls.rotary_embed(q, k, positions, inv_freq, interleaved, attention_scale)
     if out is not None:
         return out
@@ -357,8 +359,11 @@ def rotary_embed(q, k, positions, inv_freq, interleaved=False, attention_scale=1
     dev = q.get_device()
     if not (positions.get_device() == inv_freq.get_device() == dev) or (k is not None and k.get_device() != dev):
         L.refuse_devices(name, q, k=k, positions=positions, inv_freq=inv_freq)
-    if inplace and k is not None and k.data_ptr() == q.data_ptr() and k.numel():
-        raise ValueError(f'{name}: cannot work in place on one tensor as q and k')
+    if inplace and k is not None and k.numel() and q.numel():
+        if k.data_ptr() == q.data_ptr():
+            raise ValueError(f'{name}: cannot work in place on one tensor as q and k')
+        if _share_elements(q, k):
+            raise ValueError(f'{name}: cannot work in place on q and k that share elements')
     q, q_out, qb, qh, qt = _heads(name, q, B, H, T, D, inplace)
     if k is None:
         k_out, k_at, ko_at, kb, kh, kt = None, 0, 0, 0, 0, 0
@@ -385,8 +390,69 @@ def _heads(name, x, B, H, T, D, inplace):
     if inplace:
         if (sb == 0 and B > 1) or (sh == 0 and H > 1) or (st == 0 and T > 1):
             raise ValueError(f'{name}: cannot work in place on an expanded tensor')
+        if x.numel() and _meets_itself(x.shape, x.stride()):
+            raise ValueError(f'{name}: cannot work in place on a tensor whose heads overlap')
         return x, x, sb, sh, st
     return x, x.new_empty((B, T, H, D)).transpose(1, 2), sb, sh, st
+
+
+def _hits(off, steps):
+    """Whether off is a sum of i * stride with low <= i <= high over steps, a list of (stride > 0, low, high) by falling
+    stride.  What the smaller strides reach leaves few i for each; a layout that still takes long counts as a hit."""
+    reach = [(0, 0)]
+    for stride, low, high in reversed(steps):
+        reach.append((reach[-1][0] + low * stride, reach[-1][1] + high * stride))
+    reach.reverse()
+    looks = [0]
+
+    def look(n, rest):
+        if not reach[n][0] <= rest <= reach[n][1]:
+            return False
+        if n == len(steps):
+            return True
+        looks[0] += 1
+        if looks[0] > 4096:
+            return True
+        stride, low, high = steps[n]
+        least, most = reach[n + 1]
+        first, last = max(low, -((most - rest) // stride)), min(high, (rest - least) // stride)
+        return any(look(n + 1, rest - i * stride) for i in range(first, last + 1))
+    return look(0, off)
+
+
+def _share_elements(a, b):
+    """Whether two tensors of one type, neither of them empty, have an element of memory in common."""
+    apart, size = b.data_ptr() - a.data_ptr(), a.element_size()
+    # views that lie off one another's elements are taken as shared
+    return apart % size != 0 or _layouts_meet(apart // size, a.shape, a.stride(), b.shape, b.stride())
+
+
+@functools.lru_cache(maxsize=256)
+def _layouts_meet(apart, a_shape, a_stride, b_shape, b_stride):
+    # a's element at sum i * stride is b's at apart + sum j * stride; equal strides count as one step, i - j
+    steps = {}
+    for sign, shape, strides in ((1, a_shape, a_stride), (-1, b_shape, b_stride)):
+        for n, stride in zip(shape, strides):
+            if n > 1:
+                low, high = steps.get(stride, (0, 0))
+                steps[stride] = (low, high + n - 1) if sign > 0 else (low - n + 1, high)
+    steps.pop(0, None)
+    return _hits(apart, sorted(((s, *r) for s, r in steps.items()), reverse=True))
+
+
+@functools.lru_cache(maxsize=256)
+def _meets_itself(shape, strides):
+    """Whether two different indices of a tensor of that layout name the same element."""
+    dims = sorted(((s, n) for s, n in zip(strides, shape) if n > 1), reverse=True)
+    inner = 1
+    for s, n in reversed(dims):                        # the usual layouts: each stride steps over all that is inside it
+        if s < inner:
+            break
+        inner = s * (n - 1) + inner
+    else:
+        return False
+    # some dimension differs, by at least one step up; the others by any
+    return any(_hits(0, [(t, 1 if j == i else 1 - m, m - 1) for j, (t, m) in enumerate(dims)]) for i in range(len(dims)))
 
 
 def rope_frequencies(rotary_dim, base=10000.0, scaling=None, seq_len=None, device='cuda'):
