@@ -376,6 +376,9 @@ def rotary_embed(q, k, positions, inv_freq, interleaved=False, attention_scale=1
             q.data_ptr(), q_out.data_ptr(), H, qb, qt, qh, k_at, ko_at, G, kb, kt, kh, positions.data_ptr(),
             T if len(shape) == 2 and shape[0] > 1 else 0, inv_freq.data_ptr(), dt, B, T, D, 2 * half, interleaved,
             attention_scale))
+        if inplace:
+            # what autograd keeps of them for a backward pass is no longer what it was; tensors of inference mode are never kept
+            torch.autograd.graph.increment_version([t for t in (q_out, k_out) if t is not None and not t.is_inference()])
     return q_out, k_out
 
 

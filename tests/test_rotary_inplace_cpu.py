@@ -66,3 +66,29 @@ def test_shared_elements_against_a_count_of_all_of_them():
         assert _share_elements(a, b) == shared == _share_elements(b, a)
         seen.add(shared)
     assert seen == {True, False}
+
+
+def test_autograd_learns_of_what_changed_in_place(monkeypatch):
+    """A tensor that a backward pass still needs: changed in place, that pass refuses, as it does behind torch's own
+    operators.  (The launch itself is left out: there is no GPU here.)"""
+    from lightcompress_b200 import block_ops as bo
+    monkeypatch.setattr(bo.L, 'launch', lambda *a: None)
+    pos, freq = torch.arange(3), torch.ones(2)
+    for which in (0, 1):
+        x = torch.randn(2, 4, 3, 8, requires_grad=True)
+        y = x.exp()                                    # kept for the backward pass
+        other = torch.zeros(2, 4, 3, 8)
+        before = other._version
+        with torch.no_grad():
+            bo.rotary_embed(*((y, other) if which == 0 else (other, y)), pos, freq, inplace=True)
+        assert other._version > before
+        with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+            y.sum().backward()
+    y = x.exp()
+    with torch.no_grad():
+        bo.rotary_embed(y, None, pos, freq)            # not in place: nothing changed
+    y.sum().backward()
+    with torch.inference_mode():
+        z = torch.zeros(2, 4, 3, 8)
+        assert bo.rotary_embed(z, None, pos, freq, inplace=True)[0] is z
+    assert bo.rotary_embed(z, None, pos, freq, inplace=True)[0] is z
