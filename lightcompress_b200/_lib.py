@@ -9,6 +9,7 @@ import os
 import struct
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, 'liblc_b200.so')
@@ -200,8 +201,18 @@ def launch(dev, name, *args):
         check(name, code)
 
 
-def refuse_grad(name):
-    raise RuntimeError(f'{name} has no backward pass: call it under torch.no_grad(), or on detached tensors')
+def refuse_grad(name, *tensors):
+    """Refuses tensors whose gradient would be recorded, and dual tensors of forward-mode differentiation, whose tangent
+    would be lost.  None stands for an operand that is left out."""
+    back, ahead = torch.is_grad_enabled(), getattr(forward_ad, '_current_level', 0) >= 0
+    if back or ahead:
+        for t in tensors:
+            if t is None:
+                continue
+            if back and t.requires_grad:
+                raise RuntimeError(f'{name} has no backward pass: call it under torch.no_grad(), or on detached tensors')
+            if ahead and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f'{name} has no forward-mode derivative: call it on primal tensors')
 
 
 def refuse_devices(name, t, **others):

@@ -252,10 +252,7 @@ def residual_norm(x, residual=None, weight=None, post_weight=None, gate=None, sc
     if out is not None:
         return out
     name = 'residual_norm'
-    if torch.is_grad_enabled() and (
-            x.requires_grad or (weight is not None and weight.requires_grad) or (residual is not None and residual.requires_grad)
-            or (post_weight is not None and post_weight.requires_grad) or (gate is not None and gate.requires_grad)):
-        L.refuse_grad(name)
+    L.refuse_grad(name, x, residual, weight, post_weight, gate)
     dtype, shape, dev = x.dtype, x.shape, x.get_device()
     dt = L._DTYPES.get(dtype)
     if dt is None:
@@ -333,8 +330,7 @@ def rotary_embed(q, k, positions, inv_freq, interleaved=False, attention_scale=1
     if out is not None:
         return out
     name = 'rotary_embed'
-    if torch.is_grad_enabled() and (q.requires_grad or inv_freq.requires_grad or (k is not None and k.requires_grad)):
-        L.refuse_grad(name)
+    L.refuse_grad(name, q, k, inv_freq)
     dt = L._DTYPES.get(q.dtype)
     if dt is None:
         raise TypeError(f'{name}: unsupported dtype {q.dtype}')

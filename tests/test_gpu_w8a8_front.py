@@ -47,3 +47,27 @@ def test_a_norm_without_its_input_is_an_error():
             residual_norm(None, **kw)
         with torch.no_grad(), pytest.raises((AttributeError, TypeError)):
             residual_norm(None, **kw)
+
+
+@pytest.mark.parametrize('name', ['act_quant', 'gated_act_quant', 'int8_gemm', 'int8_linear', 'residual_norm', 'rotary_embed'])
+def test_dual_tensors_are_left_to_python(name):
+    """Forward-mode derivatives: the front may not drop a tangent; Python refuses the call."""
+    import torch.autograd.forward_ad as fw
+    from lightcompress_b200 import _calls, block_ops as bo, int8_linear as il
+    il.int8_dynamic_forward_func(torch.ones(1, 16, device='cuda'), torch.ones(1, 16, dtype=torch.int8, device='cuda'),
+                                 torch.ones(1, device='cuda'))
+    args, tensors, _ = _calls_and_operands()[name]
+    public = {'act_quant': il.act_quant, 'gated_act_quant': lambda g, u, kind, sym: il.gated_act_quant(g, u, 'silu', sym),
+              'int8_gemm': il.int8_gemm, 'int8_linear': il.int8_dynamic_forward_func, 'residual_norm': bo.residual_norm,
+              'rotary_embed': bo.rotary_embed}[name]
+    with fw.dual_level():
+        assert getattr(_calls, name)(*args) is not None
+        for i in tensors:
+            if not args[i].is_floating_point():
+                continue
+            dual = fw.make_dual(args[i], torch.ones_like(args[i]))
+            given = (*args[:i], dual, *args[i + 1:])
+            with torch.no_grad():
+                assert getattr(_calls, name)(*given) is None
+                with pytest.raises(RuntimeError, match='forward-mode'):
+                    public(*given)
