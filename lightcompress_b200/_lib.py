@@ -215,6 +215,12 @@ def refuse_grad(name, *tensors):
                 raise RuntimeError(f'{name} has no forward-mode derivative: call it on primal tensors')
 
 
+def resolved(*tensors):
+    """The tensors with their values in memory: a view with a pending negation (the imaginary part of a conjugated tensor)
+    becomes a copy.  None stays."""
+    return [t.resolve_neg() if t is not None and t.is_neg() else t for t in tensors]
+
+
 def refuse_devices(name, t, **others):
     """Says which of the tensors is not where t is."""
     for key, o in others.items():

@@ -253,6 +253,7 @@ def residual_norm(x, residual=None, weight=None, post_weight=None, gate=None, sc
         return out
     name = 'residual_norm'
     L.refuse_grad(name, x, residual, weight, post_weight, gate)
+    x, residual, weight, post_weight, gate = L.resolved(x, residual, weight, post_weight, gate)
     dtype, shape, dev = x.dtype, x.shape, x.get_device()
     dt = L._DTYPES.get(dtype)
     if dt is None:
@@ -331,6 +332,9 @@ def rotary_embed(q, k, positions, inv_freq, interleaved=False, attention_scale=1
         return out
     name = 'rotary_embed'
     L.refuse_grad(name, q, k, inv_freq)
+    if inplace and (q.is_neg() or (k is not None and k.is_neg())):
+        raise ValueError(f'{name}: cannot work in place on a view with a pending negation')
+    q, k, positions, inv_freq = L.resolved(q, k, positions, inv_freq)
     dt = L._DTYPES.get(q.dtype)
     if dt is None:
         raise TypeError(f'{name}: unsupported dtype {q.dtype}')

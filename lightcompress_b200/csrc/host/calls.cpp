@@ -32,12 +32,13 @@ int64_t dtype_of(const at::Tensor& t) {
   }
 }
 
-// Plain tensors of one device, the current one; none asks for a gradient that would be recorded, none carries a tangent.
+// Plain tensors of one device, the current one; none asks for a gradient that would be recorded, none carries a tangent or
+// a negation that its memory does not show.
 struct Place {
   int64_t device = -1;
   bool take(const at::Tensor& t) {
     if (!t.is_cuda() || t.layout() != at::kStrided || (t.requires_grad() && c10::GradMode::is_enabled())) return false;
-    if (t._fw_grad(0).defined()) return false;
+    if (t._fw_grad(0).defined() || t.is_neg()) return false;
     if (device < 0) device = t.get_device();
     return t.get_device() == device;
   }

@@ -84,6 +84,7 @@ def act_quant(x, sym=True):
 
 def _act_quant(x, sym):
     L.refuse_grad('act_quant', x)
+    x, = L.resolved(x)
     x2, dt = _float_rows('act_quant', x)
     rows, cols = x2.shape
     codes, pitch, scales, zeros, out = _codes_like(x, x.shape, sym)
@@ -108,6 +109,7 @@ def _gated_act_quant(gate, up, kind, sym):
     if shape != up.shape or gate.dtype != up.dtype:
         raise ValueError(f'gated_act_quant: gate {tuple(shape)} {gate.dtype} and up {tuple(up.shape)} {up.dtype} differ')
     L.refuse_grad('gated_act_quant', gate, up)
+    gate, up = L.resolved(gate, up)
     dev = gate.get_device()
     if up.get_device() != dev:
         L.refuse_devices('gated_act_quant', gate, up=up)
@@ -178,6 +180,7 @@ def int8_gemm(a, a_s, b, b_s, bias=None, a_z=None, b_sum=None, out_dtype=torch.b
 def _int8_gemm(a, a_s, b, b_s, bias, a_z, b_sum, out_dtype):
     name = 'int8_gemm'
     L.refuse_grad(name, a_s, b_s, bias)
+    a, a_s, b, b_s, bias, a_z, b_sum = L.resolved(a, a_s, b, b_s, bias, a_z, b_sum)
     out = _DTYPES.get(out_dtype)
     if out is None:
         raise TypeError(f'{name}: unsupported output type {out_dtype}')
@@ -219,6 +222,7 @@ def int8_dynamic_forward_func(x, w, w_scale, bias=None, w_sum=None):
 def _int8_dynamic_forward(x, w, w_scale, bias, w_sum):
     name = 'int8_dynamic_forward_func'
     L.refuse_grad(name, x, w_scale, bias)
+    x, w, w_scale, bias, w_sum = L.resolved(x, w, w_scale, bias, w_sum)
     x2, dt = _float_rows(name, x)
     sym = w_sum is None
     N, K = _check_weight(name, w, w_scale, w_sum, bias, not sym, x.dtype)
