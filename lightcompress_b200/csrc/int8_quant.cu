@@ -12,19 +12,28 @@ constexpr int kThreads = 256;
 
 enum Act { kNone = 0, kSilu = LC_ACT_SILU, kGelu = LC_ACT_GELU, kGeluTanh = LC_ACT_GELU_TANH };
 
-// Quotients and exponentials by the fast intrinsics (2 steps and |x| 2^-22 relative at most): a thousandth of a code.  The
-// tanh form is x times the logistic function of twice its argument; the erf form uses erfc(z) = (a1 t + .. + a5 t^5)
-// exp(-z^2), t = 1 / (1 + p z), z >= 0, absolute error 1.5e-7 (Abramowitz and Stegun, Handbook of Mathematical Functions,
-// 7.1.26), which keeps both tails.  The library's erff and tanhf bound the kernel: 40 and 36 us for 2048 x 11008 in bf16.
+// Quotients and exponentials by the fast intrinsics.  __expf(y) is off by up to (2 + 1.17 |y|) 2^-23 relative, a quotient by
+// two steps.  What comes out is off relative to itself, in the negative tail as well, because a token whose gates all lie
+// there takes its scale from it:
+//   silu       x / (1 + e^-x)                                                          (5 + 1.2 |x|) 2^-23
+//   gelu_tanh  x / (1 + e^-u), u = 2 sqrt(2 / pi) (x + 0.044715 x^3), seven roundings   (5 + 4.7 |u|) 2^-23
+//   gelu       x - x q or, below zero, x q: q = erfc(|x| / sqrt 2) / 2 = t P(t) e^(-x^2 / 2), t = 1 / (1 + 0.27 |x|), P of degree
+//              6 fitted to the least relative error (1.5e-6 for |x| < 20, its roundings included)   (18 + 0.9 x^2) 2^-23
+// A thousandth of a code is 2^-17: silu down to -49, gelu_tanh to -4.3, gelu to -7; twice that gelu_tanh to -6.1, gelu to -11.
+// Where e^-x, e^-u or e^(x^2 / 2) leaves 2^126 (below -87, -10 and -13) the value is under 2^-119 and taken as zero.  The library's erff and tanhf bound the kernel: 40 and 36 us for 2048 x 11008 in bf16.  (A polynomial for erfc with a
+// bound on its absolute error alone costs two steps less, 29 us where this one takes 31, and is off by a hundredth of the value
+// at -8; an exponential whose error does not grow with its argument costs silu 25 us instead of 21.5.)
 template <int kAct>
 __device__ __forceinline__ float act_of(float x) {
   if (kAct == kSilu) return __fdividef(x, 1.f + __expf(-x));
   if (kAct == kGeluTanh) return __fdividef(x, 1.f + __expf(-1.5957691216057308f * (x + 0.044715f * x * x * x)));
   if (kAct == kGelu) {
-    const float z = fabsf(x) * 0.70710678118654752f, t = __fdividef(1.f, fmaf(0.3275911f, z, 1.f));
-    const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
-    const float tail = 0.5f * p * __expf(-z * z);            // half of erfc(z)
-    return x * (x >= 0.f ? 1.f - tail : tail);
+    const float t = __fdividef(1.f, fmaf(0.27f, fabsf(x), 1.f));
+    float p = -0.0610578172f;
+    p = fmaf(p, t, 0.159365267f), p = fmaf(p, t, -0.0255874731f), p = fmaf(p, t, 0.118717268f);
+    p = fmaf(p, t, 0.0923243687f), p = fmaf(p, t, 0.108561143f), p = fmaf(p, t, 0.107676633f);
+    const float xq = x * (p * t * __expf(-0.5f * x * x));
+    return x >= 0.f ? x - xq : xq;
   }
   return x;
 }
@@ -85,7 +94,7 @@ __global__ void __launch_bounds__(kThreads) quant_any_kernel(QuantArgs a) {
 
 // Rows that registers hold, by 16-byte vectors or, less aligned, by pairs or single values: read once, written once.
 // HBM-bound: 16384 x 11008 in bf16 84 us (6.4 TB/s, 98 % of a copy's rate), with a zero point 92; silu(gate) * up 147 (6.1
-// TB/s), the tanh form of gelu 158, the erf form 205, the last two bound by their arithmetic.
+// TB/s), the tanh form of gelu 156, the erf form 219, the last two bound by their arithmetic.
 template <typename T, int N, int kWarps, int kVecs, int kAct>
 __global__ void __launch_bounds__(RowGroup<kWarps>::kThreads) quant_rows_kernel(QuantArgs a) {
   using G = RowGroup<kWarps>;
