@@ -275,6 +275,20 @@ class Int8Linear(nn.Module):
         bias = getattr(module, 'bias', None)
         return cls(codes, scale, None if bias is None else bias.data, aquantizer is None or aquantizer.sym)
 
+    def _lay_out(self):
+        # where in_features is no multiple of 16 the weight is a view of padded rows, which torch makes contiguous when it
+        # copies it to another device or takes it over from a state dict
+        self.weight = aligned_rows(self.weight)
+
+    def _apply(self, fn, recurse=True):
+        super()._apply(fn, recurse)
+        self._lay_out()
+        return self
+
+    def _load_from_state_dict(self, *args, **kwargs):
+        super()._load_from_state_dict(*args, **kwargs)
+        self._lay_out()
+
     @torch.no_grad()
     def forward(self, x):
         return int8_dynamic_forward_func(x, self.weight, self.weight_scale, self.bias, self.weight_sum)

@@ -1,0 +1,29 @@
+"""Int8Linear moved to the GPU and cast, against the functional call on the same codes, bit for bit."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _codes(k):
+    g = torch.Generator().manual_seed(k)
+    return (torch.randint(-128, 128, (40, k), generator=g, dtype=torch.int8), torch.rand(40, generator=g) * 0.01 + 1e-3,
+            torch.randn(40, generator=g))
+
+
+def _want(codes, scale, bias, x, sym):
+    from lightcompress_b200 import int8_linear as il
+    w = il.aligned_rows(codes.cuda())
+    return il.int8_dynamic_forward_func(x, w, scale.cuda(), bias.to(x.dtype).cuda(), None if sym else w.sum(1, dtype=torch.int32))
+
+
+@pytest.mark.parametrize('sym', [True, False])
+@pytest.mark.parametrize('k', [30, 64, 1399])
+def test_built_on_the_cpu_and_moved(k, sym):
+    from lightcompress_b200 import Int8Linear
+    codes, scale, bias = _codes(k)
+    m = Int8Linear(codes, scale, bias, sym).cuda()
+    x = torch.randn(5, k, device='cuda')
+    assert torch.equal(m(x), _want(codes, scale, bias, x, sym))
+    there = m.cpu().to('cuda:0')
+    assert torch.equal(there(x), _want(codes, scale, bias, x, sym))
