@@ -246,7 +246,8 @@ def _int8_dynamic_forward(x, w, w_scale, bias, w_sum):
 
 class Int8Linear(nn.Module):
     """Replacement linear with int8 weights and dynamically quantised activations (the role of the reference's
-    VllmQuantLinearInt8).  `new` takes what the algorithms' replacement linears take: the module and its
+    VllmQuantLinearInt8).  Moved and cast like any module: the bias takes the type that the activations then have, codes and
+    scales keep theirs.  `new` takes what the algorithms' replacement linears take: the module and its
     w_q(module, wquantizer) -> (codes, scales, zeros)."""
 
     def __init__(self, codes, scale, bias=None, sym_act=True):
@@ -281,7 +282,12 @@ class Int8Linear(nn.Module):
         self.weight = aligned_rows(self.weight)
 
     def _apply(self, fn, recurse=True):
+        kept = {name: getattr(self, name) for name in ('weight', 'weight_scale', 'weight_sum')}
         super()._apply(fn, recurse)
+        for name, before in kept.items():       # .half() and the like cast the bias; codes, sums and scales keep their types
+            now = getattr(self, name)
+            if before is not None and now.dtype != before.dtype:
+                setattr(self, name, before.to(now.device))
         self._lay_out()
         return self
 

@@ -27,3 +27,13 @@ def test_built_on_the_cpu_and_moved(k, sym):
     assert torch.equal(m(x), _want(codes, scale, bias, x, sym))
     there = m.cpu().to('cuda:0')
     assert torch.equal(there(x), _want(codes, scale, bias, x, sym))
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+def test_cast_with_a_model(dtype):
+    from lightcompress_b200 import Int8Linear
+    for k, sym in ((30, True), (256, False)):
+        codes, scale, bias = _codes(k)
+        model = torch.nn.Sequential(torch.nn.Linear(k, k), Int8Linear(codes, scale, bias, sym)).to('cuda').to(dtype)
+        x = torch.randn(5, k, device='cuda').to(dtype)
+        assert torch.equal(model[1](x), _want(codes, scale, bias, x, sym))

@@ -52,3 +52,33 @@ def test_rows_stay_laid_out(k, sym):
     block = torch.nn.Sequential(torch.nn.Linear(k, k), copy.deepcopy(m))
     block._apply(lambda t: t.clone(memory_format=torch.contiguous_format))
     _laid_out(block[1])
+
+
+@pytest.mark.parametrize('cast', ['half', 'bfloat16', 'double', 'to', 'to_both', 'type', 'to_meta'])
+def test_scales_keep_their_type_and_value(cast):
+    for k, sym in ((30, True), (64, False)):
+        m, codes = _module(k, sym)
+        want = m.weight_scale.clone()
+        outer = torch.nn.Sequential(m)
+        if cast == 'to':
+            outer.to(torch.bfloat16)
+        elif cast == 'to_both':
+            outer.to(device='cpu', dtype=torch.float16)
+        elif cast == 'type':
+            outer.type(torch.float16)
+        elif cast == 'to_meta':
+            outer.to(device='meta', dtype=torch.float16)
+        else:
+            getattr(outer, cast)()
+        assert m.weight.dtype == torch.int8 and m.weight_scale.dtype == torch.float32
+        assert sym or m.weight_sum.dtype == torch.int32
+        assert m.bias.dtype == {'half': torch.float16, 'bfloat16': torch.bfloat16, 'double': torch.float64, 'to': torch.bfloat16}.get(cast, torch.float16)
+        if cast == 'to_meta':
+            assert {t.device.type for t in m.state_dict().values()} == {'meta'}
+            continue
+        assert torch.equal(m.weight_scale, want) and torch.equal(m.weight, codes)
+        if cast != 'double':
+            _laid_out(m)
+            outer.float()                                           # there and back: only the bias was rounded
+            assert torch.equal(m.weight_scale, want)
+            _laid_out(m)
