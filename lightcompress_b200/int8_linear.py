@@ -28,7 +28,8 @@ def _status_of(t, dev):
     if s is None:
         if dev < 0 or torch.cuda.is_current_stream_capturing():
             return 0
-        s = torch.zeros(1, dtype=torch.int32, device=t.device)
+        with torch.inference_mode(False):       # check_status clears the word outside that mode as well
+            s = torch.zeros(1, dtype=torch.int32, device=t.device)
         torch.cuda.current_stream(dev).synchronize()      # other streams may use it from here on
         _status[dev] = s
         _calls.set_status(dev, s.data_ptr())
