@@ -5,11 +5,15 @@ hands the per-token quantisation of the activations and the scaled product to th
 sibling of fp8_linear.  Codes are int8 with an fp32 scale per token (activations) and per output channel (weights);
 activations may carry a zero point per token as well.
 
-Nothing here synchronises or reads device memory on the host, so every call can be captured into a CUDA graph.
+Nothing here reads device memory on the host, and nothing synchronises but the first product on a device, which makes the word
+that an expired wait is reported in; so every call can be captured into a CUDA graph (a product whose device has no such word
+yet reports nothing).
 
 Each function asks the compiled front (_calls) first, which serves the ordinary call in a third of the host time and returns
 None for any other; the Python below it knows every case and says what is wrong with a call.
 """
+import threading
+
 import torch
 import torch.nn as nn
 
@@ -17,7 +21,7 @@ from . import _lib as L
 from ._lib import _calls
 
 _ACTS = {'silu': 1, 'gelu': 2, 'gelu_tanh': 3}
-_status = {}
+_status, _status_made = {}, threading.Lock()
 _DTYPES = L._DTYPES
 
 
@@ -28,11 +32,14 @@ def _status_of(t, dev):
     if s is None:
         if dev < 0 or torch.cuda.is_current_stream_capturing():
             return 0
-        with torch.inference_mode(False):       # check_status clears the word outside that mode as well
-            s = torch.zeros(1, dtype=torch.int32, device=t.device)
-        torch.cuda.current_stream(dev).synchronize()      # other streams may use it from here on
-        _status[dev] = s
-        _calls.set_status(dev, s.data_ptr())
+        with _status_made:                      # one word for all threads: kernels and graphs keep its address
+            s = _status.get(dev)
+            if s is None:
+                with torch.inference_mode(False):       # check_status clears the word outside that mode as well
+                    s = torch.zeros(1, dtype=torch.int32, device=t.device)
+                torch.cuda.current_stream(dev).synchronize()      # other streams may use it from here on
+                _status[dev] = s
+                _calls.set_status(dev, s.data_ptr())
     return s.data_ptr()
 
 

@@ -53,3 +53,26 @@ def test_no_word_is_made_inside_a_capture_or_without_a_device(words, monkeypatch
     assert il._status_of(torch.zeros(1), -1) == 0
     monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: True)
     assert il._status_of(torch.zeros(1), 0) == 0 and not handed
+
+
+def test_threads_that_come_first_together_share_one_word(words, monkeypatch):
+    """Kernels launched by one thread may not keep the address of a word that another thread's replaces."""
+    import threading
+    il, handed = words
+    together = threading.Barrier(4)
+
+    class Slow:
+        def synchronize(self):
+            threading.Event().wait(0.2)               # lets the other threads run, as torch's does
+    monkeypatch.setattr(torch.cuda, 'current_stream', lambda d=None: Slow())
+    got = []
+
+    def first():
+        together.wait()
+        got.append(il._status_of(torch.zeros(1), 0))
+    threads = [threading.Thread(target=first) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(got) == 4 and set(got) == {il._status[0].data_ptr()} and handed == [(0, got[0])]
