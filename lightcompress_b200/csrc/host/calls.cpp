@@ -132,6 +132,17 @@ PyObject* pair_of(PyObject* a, PyObject* b) {
   return r;
 }
 
+// Other Python threads run meanwhile: an allocation may wait for the device, a launch for room in its queue, and what the
+// device waits for may need the interpreter.  Nothing of Python's is touched while one of these lives.
+class Unlocked {
+  PyThreadState* const state_ = PyEval_SaveThread();
+
+ public:
+  Unlocked() = default;
+  Unlocked(const Unlocked&) = delete;
+  ~Unlocked() { PyEval_RestoreThread(state_); }
+};
+
 // The functions below return false for what the Python function has to deal with.
 
 // (x, sym)
@@ -144,11 +155,15 @@ bool act_quant(PyObject* const* a, Py_ssize_t n, PyObject** out) {
   if (!x || !place.take(*x) || dtype_of(*x) < 0 || !rows_of(*x, &r)) return false;
   const bool sym = a[1] == Py_True;
   if ((!sym && a[1] != Py_False) || !place.enter(&st)) return false;
-  const Codes c(*x, sym);
-  if (lc_int8_act_quant(x->data_ptr(), (int)dtype_of(*x), r.rows, r.cols, r.pitch, c.at_codes(), c.pitch, c.at_scales(),
-                        c.at_zeros(), st) != LC_OK)
-    return false;
-  *out = c.tuple(r.cols);
+  c10::optional<Codes> c;
+  {
+    const Unlocked unlocked;
+    c.emplace(*x, sym);
+    if (lc_int8_act_quant(x->data_ptr(), (int)dtype_of(*x), r.rows, r.cols, r.pitch, c->at_codes(), c->pitch, c->at_scales(),
+                          c->at_zeros(), st) != LC_OK)
+      return false;
+  }
+  *out = c->tuple(r.cols);
   return true;
 }
 
@@ -165,11 +180,15 @@ bool gated_act_quant(PyObject* const* a, Py_ssize_t n, PyObject** out) {
   const long act = PyLong_AsLong(a[2]);
   const bool sym = a[3] == Py_True;
   if ((!sym && a[3] != Py_False) || !place.enter(&st)) return false;
-  const Codes c(*g, sym);
-  if (lc_int8_gated_act_quant(g->data_ptr(), u->data_ptr(), (int)dtype_of(*g), rg.rows, rg.cols, rg.pitch, ru.pitch, (int)act,
-                              c.at_codes(), c.pitch, c.at_scales(), c.at_zeros(), st) != LC_OK)
-    return false;
-  *out = c.tuple(rg.cols);
+  c10::optional<Codes> c;
+  {
+    const Unlocked unlocked;
+    c.emplace(*g, sym);
+    if (lc_int8_gated_act_quant(g->data_ptr(), u->data_ptr(), (int)dtype_of(*g), rg.rows, rg.cols, rg.pitch, ru.pitch, (int)act,
+                                c->at_codes(), c->pitch, c->at_scales(), c->at_zeros(), st) != LC_OK)
+      return false;
+  }
+  *out = c->tuple(rg.cols);
   return true;
 }
 
@@ -203,13 +222,17 @@ bool int8_gemm(PyObject* const* o, Py_ssize_t n, PyObject** out) {
   if (!w.take(o[2], o[3], o[4], a_z ? o[6] : Py_None, type, &place) || r.cols != w.r.cols) return false;
   if (!vector_of(*a_s, at::kFloat, r.rows) || (a_z && !vector_of(*a_z, at::kInt, r.rows)) || !place.enter(&st)) return false;
   if (!g_status[place.device]) return false;
-  const at::Tensor c = fresh(with_last(*a, w.r.rows), type, *a);
-  const int64_t dt = dtype_of(c);
-  if (dt < 0) return false;
-  const lc_int8_gemm_args args = {a->data_ptr<int8_t>(), r.pitch, a_s->data_ptr<float>(), a_z ? a_z->data_ptr<int32_t>() : nullptr,
-                                  w.b->data_ptr<int8_t>(), w.r.pitch, w.scale->data_ptr<float>(), w.at_sum(), w.at_bias(),
-                                  r.rows, w.r.rows, r.cols, c.data_ptr(), dt, g_status[place.device]};
-  if (lc_int8_gemm(&args, st) != LC_OK) return false;
+  if (type != at::kFloat && type != at::kBFloat16 && type != at::kHalf) return false;
+  at::Tensor c;
+  {
+    const Unlocked unlocked;
+    c = fresh(with_last(*a, w.r.rows), type, *a);
+    const int64_t dt = dtype_of(c);
+    const lc_int8_gemm_args args = {a->data_ptr<int8_t>(), r.pitch, a_s->data_ptr<float>(), a_z ? a_z->data_ptr<int32_t>() : nullptr,
+                                    w.b->data_ptr<int8_t>(), w.r.pitch, w.scale->data_ptr<float>(), w.at_sum(), w.at_bias(),
+                                    r.rows, w.r.rows, r.cols, c.data_ptr(), dt, g_status[place.device]};
+    if (lc_int8_gemm(&args, st) != LC_OK) return false;
+  }
   *out = THPVariable_Wrap(c);
   return true;
 }
@@ -225,13 +248,17 @@ bool int8_linear(PyObject* const* o, Py_ssize_t n, PyObject** out) {
   if (!x || !place.take(*x) || dtype_of(*x) < 0 || !rows_of(*x, &r)) return false;
   if (!w.take(o[1], o[2], o[3], o[4], x->scalar_type(), &place) || r.cols != w.r.cols || !place.enter(&st)) return false;
   if (!g_status[place.device]) return false;
-  const at::Tensor c = fresh(with_last(*x, w.r.rows), x->scalar_type(), *x);
-  const int64_t room = lc_int8_linear_scratch(r.rows, r.cols);
-  const at::Tensor scratch = room ? fresh({room}, at::kChar, *x) : at::Tensor();
-  const lc_int8_linear_args args = {x->data_ptr(), dtype_of(*x), r.pitch, w.b->data_ptr<int8_t>(), w.r.pitch,
-                                    w.scale->data_ptr<float>(), w.at_sum(), w.at_bias(), r.rows, w.r.rows, r.cols, w.sum == nullptr,
-                                    c.data_ptr(), room ? scratch.data_ptr() : nullptr, room, g_status[place.device]};
-  if (lc_int8_linear(&args, st) != LC_OK) return false;
+  at::Tensor c;
+  {
+    const Unlocked unlocked;
+    c = fresh(with_last(*x, w.r.rows), x->scalar_type(), *x);
+    const int64_t room = lc_int8_linear_scratch(r.rows, r.cols);
+    const at::Tensor scratch = room ? fresh({room}, at::kChar, *x) : at::Tensor();
+    const lc_int8_linear_args args = {x->data_ptr(), dtype_of(*x), r.pitch, w.b->data_ptr<int8_t>(), w.r.pitch,
+                                      w.scale->data_ptr<float>(), w.at_sum(), w.at_bias(), r.rows, w.r.rows, r.cols, w.sum == nullptr,
+                                      c.data_ptr(), room ? scratch.data_ptr() : nullptr, room, g_status[place.device]};
+    if (lc_int8_linear(&args, st) != LC_OK) return false;
+  }
   *out = THPVariable_Wrap(c);
   return true;
 }
@@ -277,16 +304,19 @@ bool residual_norm(PyObject* const* o, Py_ssize_t n, PyObject** out) {
   const bool quant = o[8] == Py_True, sym = o[9] == Py_True, kept = !res && !pw && !gate && scale == 1.0;
   if ((!quant && o[8] != Py_False) || (!sym && o[9] != Py_False) || (!w && (quant || kept)) || !place.enter(&st)) return false;
   at::Tensor h, y;
-  if (!kept) h = fresh(x->sizes(), x->scalar_type(), *x);
-  if (w && !quant) y = fresh(x->sizes(), x->scalar_type(), *x);
   c10::optional<Codes> c;
-  if (quant) c.emplace(*x, sym);
-  const lc_residual_norm_args args = {x->data_ptr(), res ? res->data_ptr() : nullptr, pw ? pw->data_ptr() : nullptr,
-                                      gate ? gate->data_ptr() : nullptr, gate_rows, w ? w->data_ptr() : nullptr, dtype_of(*x),
-                                      rx.rows, rx.cols, rx.pitch, rr.pitch, scale, eps, offset, kept ? nullptr : h.data_ptr(),
-                                      y.defined() ? y.data_ptr() : nullptr, c ? c->at_codes() : nullptr, c ? c->pitch : 0,
-                                      c ? c->at_scales() : nullptr, c ? c->at_zeros() : nullptr};
-  if (lc_residual_norm(&args, st) != LC_OK) return false;
+  {
+    const Unlocked unlocked;
+    if (!kept) h = fresh(x->sizes(), x->scalar_type(), *x);
+    if (w && !quant) y = fresh(x->sizes(), x->scalar_type(), *x);
+    if (quant) c.emplace(*x, sym);
+    const lc_residual_norm_args args = {x->data_ptr(), res ? res->data_ptr() : nullptr, pw ? pw->data_ptr() : nullptr,
+                                        gate ? gate->data_ptr() : nullptr, gate_rows, w ? w->data_ptr() : nullptr, dtype_of(*x),
+                                        rx.rows, rx.cols, rx.pitch, rr.pitch, scale, eps, offset, kept ? nullptr : h.data_ptr(),
+                                        y.defined() ? y.data_ptr() : nullptr, c ? c->at_codes() : nullptr, c ? c->pitch : 0,
+                                        c ? c->at_scales() : nullptr, c ? c->at_zeros() : nullptr};
+    if (lc_residual_norm(&args, st) != LC_OK) return false;
+  }
   PyObject* first = kept ? (Py_INCREF(o[0]), o[0]) : THPVariable_Wrap(h);
   PyObject* second = quant ? c->tuple(rx.cols) : y.defined() ? THPVariable_Wrap(y) : (Py_INCREF(Py_None), Py_None);
   *out = pair_of(first, second);
@@ -319,12 +349,18 @@ bool rotary_embed(PyObject* const* o, Py_ssize_t n, PyObject** out) {
     const int64_t heads = t.size(1);
     return at::cuda::empty_strided(t.sizes(), {T * heads * D, D, heads * D, 1}, t.scalar_type(), c10::nullopt, t.device(), c10::nullopt);
   };
-  const at::Tensor qo = like(*q), ko = k ? like(*k) : at::Tensor();
-  const lc_rotary_embed_args args = {q->data_ptr(), qo.data_ptr(), H, q->stride(0), q->stride(2), q->stride(1),
-                                     k ? k->data_ptr() : nullptr, k ? ko.data_ptr() : nullptr, G, k ? k->stride(0) : 0,
-                                     k ? k->stride(2) : 0, k ? k->stride(1) : 0, pos->data_ptr<int64_t>(), own_rows ? T : 0,
-                                     freq->data_ptr<float>(), dtype_of(*q), B, T, D, 2 * half, inter, PyFloat_AS_DOUBLE(o[5])};
-  if (lc_rotary_embed(&args, st) != LC_OK) return false;
+  at::Tensor qo, ko;
+  const double scale = PyFloat_AS_DOUBLE(o[5]);
+  {
+    const Unlocked unlocked;
+    qo = like(*q);
+    if (k) ko = like(*k);
+    const lc_rotary_embed_args args = {q->data_ptr(), qo.data_ptr(), H, q->stride(0), q->stride(2), q->stride(1),
+                                       k ? k->data_ptr() : nullptr, k ? ko.data_ptr() : nullptr, G, k ? k->stride(0) : 0,
+                                       k ? k->stride(2) : 0, k ? k->stride(1) : 0, pos->data_ptr<int64_t>(), own_rows ? T : 0,
+                                       freq->data_ptr<float>(), dtype_of(*q), B, T, D, 2 * half, inter, scale};
+    if (lc_rotary_embed(&args, st) != LC_OK) return false;
+  }
   *out = pair_of(THPVariable_Wrap(qo), k ? THPVariable_Wrap(ko) : (Py_INCREF(Py_None), Py_None));
   return true;
 }
