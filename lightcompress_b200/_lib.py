@@ -7,6 +7,7 @@ no CPU or pure-torch fallback.  torch is used only to own device memory and stre
 import ctypes
 import os
 import struct
+import sysconfig
 import warnings
 
 import torch
@@ -142,12 +143,16 @@ class NoFront:
 
 def _load_front():
     """The compiled front of the W8A8 operators, linked against the library above and against torch.  Nothing depends on it but
-    those operators' host time, so the package does without it where it is missing or does not load."""
+    those operators' host time, so the package does without it where it is missing, does not load or was built for another
+    torch or interpreter."""
+    here = f'torch {torch.__version__}, {sysconfig.get_config_var("SOABI")}'
     try:
         from . import _calls
+        if _calls.built_for != here:
+            raise ImportError(f'built for {_calls.built_for}, this is {here}')
         return _calls
-    except ImportError as e:
-        warnings.warn(f'lightcompress_b200/_calls.so is missing or does not load ({e}): calls of the W8A8 operators take two to '
+    except (ImportError, AttributeError) as e:
+        warnings.warn(f'lightcompress_b200/_calls.so is missing or does not fit ({e}): calls of the W8A8 operators take two to '
                       'three times the host time.  Build it with `python __graft_entry__.py`.', RuntimeWarning, stacklevel=2)
         return NoFront()
 

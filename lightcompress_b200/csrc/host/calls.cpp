@@ -401,4 +401,9 @@ PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_calls", "Compiled front of the 
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__calls() { return PyModule_Create(&g_module); }
+// built_for: the torch and the interpreter whose binary interfaces are compiled in, to be compared before anything is called
+PyMODINIT_FUNC PyInit__calls() {
+  PyObject* m = PyModule_Create(&g_module);
+  if (m && PyModule_AddStringConstant(m, "built_for", LC_BUILT_FOR) < 0) Py_CLEAR(m);
+  return m;
+}
