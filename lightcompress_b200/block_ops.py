@@ -458,15 +458,23 @@ def _meets_itself(shape, strides):
     return any(_hits(0, [(t, 1 if j == i else 1 - m, m - 1) for j, (t, m) in enumerate(dims)]) for i in range(len(dims)))
 
 
-def rope_frequencies(rotary_dim, base=10000.0, scaling=None, seq_len=None, device='cuda'):
+def rope_frequencies(rotary_dim, base=None, scaling=None, seq_len=None, device='cuda'):
     """(inv_freq fp32 (rotary_dim / 2,), attention_scale) for rotary_embed.  `scaling` is a model configuration's
     rope_scaling / rope_parameters section: None or type 'default', 'linear' (factor), 'dynamic' (factor,
     original_max_position_embeddings; uses seq_len), 'llama3' (factor, low_freq_factor, high_freq_factor,
     original_max_position_embeddings) or 'yarn' (factor, original_max_position_embeddings, optional beta_fast, beta_slow,
-    mscale, mscale_all_dim, attention_factor)."""
+    mscale, mscale_all_dim, attention_factor).  base: the model's rope_theta; where it is left out it is the section's own
+    rope_theta, else 10000.  A section that holds one for each kind of layer is handed in one kind at a time."""
     if rotary_dim <= 0 or rotary_dim % 2:
         raise ValueError(f'rope_frequencies: rotary_dim must be even and positive, got {rotary_dim}')
     s = dict(scaling or {})
+    if any(isinstance(v, dict) for v in s.values()):
+        raise ValueError(f'rope_frequencies: sections for several kinds of layer ({", ".join(map(str, s))}): hand in one of them')
+    theta = s.get('rope_theta')
+    if base is None:
+        base = 10000.0 if theta is None else theta
+    elif theta is not None and theta != base:
+        raise ValueError(f'rope_frequencies: base {base} and the section\'s rope_theta {theta} differ')
     kind = s.get('rope_type', s.get('type', 'default'))
     expo = torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim
     inv = float(base) ** -expo
