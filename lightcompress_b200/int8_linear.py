@@ -278,6 +278,10 @@ class Int8Linear(nn.Module):
         the activations' quantizer (8 bits, per_token), whose symmetry is kept; None means symmetric."""
         if aquantizer is not None and (aquantizer.bit != 8 or aquantizer.granularity != 'per_token'):
             raise NotImplementedError('Int8Linear: activations are quantised to 8 bits per token')
+        if aquantizer is not None and getattr(aquantizer, 'calib_algo', 'minmax') != 'minmax':
+            raise NotImplementedError(f'Int8Linear: activations take their range from each token, not by {aquantizer.calib_algo}')
+        if aquantizer is not None and not aquantizer.sym and not getattr(aquantizer, 'round_zp', True):
+            raise NotImplementedError('Int8Linear: zero points are whole numbers (round_zp)')
         codes, scale, zeros = w_q(module, wquantizer) if wquantizer is not None else w_q(module)
         if zeros is not None:
             raise NotImplementedError('Int8Linear: weights with zero points are not supported')

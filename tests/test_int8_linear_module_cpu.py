@@ -82,3 +82,22 @@ def test_scales_keep_their_type_and_value(cast):
             outer.float()                                           # there and back: only the bias was rounded
             assert torch.equal(m.weight_scale, want)
             _laid_out(m)
+
+
+def test_quantisers_that_it_is_no_deployment_of_are_refused():
+    """Settings of the activations' quantiser that the module would otherwise pass over."""
+    from lightcompress_b200 import FloatQuantizer, Int8Linear, IntegerQuantizer
+    lin = torch.nn.Linear(16, 8)
+    codes, scale = torch.ones(8, 16, dtype=torch.int8), torch.ones(8, 1)
+
+    def new(aq):
+        return Int8Linear.new(lin, lambda module, wq: (codes, scale, None), object(), aq)
+    for aq in (None, IntegerQuantizer(8, True, 'per_token'), IntegerQuantizer(8, False, 'per_token'),
+               IntegerQuantizer(8, True, 'per_token', round_zp=False)):
+        assert new(aq).in_features == 16
+    for aq in (IntegerQuantizer(8, True, 'per_token', calib_algo='static_minmax'), IntegerQuantizer(8, True, 'per_token', calib_algo='mse'),
+               IntegerQuantizer(8, True, 'per_token', calib_algo='static_hist'), IntegerQuantizer(8, False, 'per_token', round_zp=False),
+               IntegerQuantizer(8, True, 'per_tensor'), IntegerQuantizer(6, True, 'per_token'),
+               FloatQuantizer('e4m3', True, 'per_token', use_qtorch=True)):
+        with pytest.raises(NotImplementedError, match='Int8Linear'):
+            new(aq)
