@@ -275,7 +275,10 @@ class Int8Linear(nn.Module):
     @torch.no_grad()
     def new(cls, module, w_q, wquantizer=None, aquantizer=None):
         """module: an nn.Linear; w_q: e.g. RTN(wquantizer).w_q, for 8-bit symmetric per_channel weights; aquantizer:
-        the activations' quantizer (8 bits, per_token), whose symmetry is kept; None means symmetric."""
+        the activations' quantizer (8 bits, per_token), whose symmetry is kept; None means symmetric.  With zero points the
+        token's range is widened to hold zero, as act_quant says: for a token of both signs that is the quantiser's own
+        grid, for a token of one sign it is not (the quantiser steps over max - min from a zero point cut to its codes, and
+        so cuts off the values of the far end)."""
         if aquantizer is not None and (aquantizer.bit != 8 or aquantizer.granularity != 'per_token'):
             raise NotImplementedError('Int8Linear: activations are quantised to 8 bits per token')
         if aquantizer is not None and getattr(aquantizer, 'calib_algo', 'minmax') != 'minmax':

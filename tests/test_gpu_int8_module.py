@@ -37,3 +37,27 @@ def test_cast_with_a_model(dtype):
         model = torch.nn.Sequential(torch.nn.Linear(k, k), Int8Linear(codes, scale, bias, sym)).to('cuda').to(dtype)
         x = torch.randn(5, k, device='cuda').to(dtype)
         assert torch.equal(model[1](x), _want(codes, scale, bias, x, sym))
+
+
+def test_zero_points_beside_those_of_the_fake_quantiser():
+    """The grid of IntegerQuantizer(8, False, 'per_token') for tokens of both signs: the same steps (a division apart, 2^-23) and
+    values at most a step apart (zero points next to a rounding border, and codes next to one).  Tokens of one sign: the range
+    is widened to hold zero, so that every value is within half a step; the quantiser cuts off what lies beyond max - min."""
+    from lightcompress_b200 import IntegerQuantizer
+    from lightcompress_b200.int8_linear import act_quant
+    g = torch.Generator().manual_seed(4)
+    both = torch.randn(64, 512, generator=g).cuda()
+    one = (torch.rand(64, 512, generator=g) + 1).cuda()                     # between 1 and 2
+    fake = IntegerQuantizer(8, False, 'per_token')
+    for x in (both, one, -one):
+        codes, scales, zeros = act_quant(x, sym=False)
+        value = (codes.float() - zeros) * scales
+        # the ends of a range of both signs may be cut by the zero point's rounding, half a step
+        assert bool(((value - x).abs() <= scales * (1.01 if x is both else 0.5 + 2.0 ** -10)).all())
+        off = (value - fake.fake_quant_act_dynamic(x)).abs()
+        if x is both:
+            want = (x.amax(1, keepdim=True) - x.amin(1, keepdim=True)) / 255
+            assert torch.allclose(scales, want, rtol=2.0 ** -22, atol=0)
+            assert bool((off <= scales * 1.01).all())
+        else:
+            assert float(off.max()) > 0.5                                    # the far end, not a step (2 / 255)
