@@ -359,11 +359,8 @@ def rotary_embed(q, k, positions, inv_freq, interleaved=False, attention_scale=1
     dev = q.get_device()
     if not (positions.get_device() == inv_freq.get_device() == dev) or (k is not None and k.get_device() != dev):
         L.refuse_devices(name, q, k=k, positions=positions, inv_freq=inv_freq)
-    if inplace and k is not None and k.numel() and q.numel():
-        if k.data_ptr() == q.data_ptr():
-            raise ValueError(f'{name}: cannot work in place on one tensor as q and k')
-        if _share_elements(q, k):
-            raise ValueError(f'{name}: cannot work in place on q and k that share elements')
+    if inplace and k is not None and k.data_ptr() == q.data_ptr() and k.numel():
+        raise ValueError(f'{name}: cannot work in place on one tensor as q and k')
     q, q_out, qb, qh, qt = _heads(name, q, B, H, T, D, inplace)
     if k is None:
         k_out, k_at, ko_at, kb, kh, kt = None, 0, 0, 0, 0, 0
@@ -371,6 +368,10 @@ def rotary_embed(q, k, positions, inv_freq, interleaved=False, attention_scale=1
         k, k_out, kb, kh, kt = _heads(name, k, B, G, T, D, inplace)
         k_at, ko_at = k.data_ptr(), k_out.data_ptr()
     if B and T:
+        if inplace:
+            fault = _shared_in_place(B, T, D, H, qb, qh, qt, G, kb, kh, kt, k_at - q.data_ptr() if G else 0, q.element_size())
+            if fault is not None:
+                raise ValueError(f'{name}: cannot work in place on {fault}')
         positions, inv_freq = positions.contiguous(), inv_freq.contiguous()
         L.launch(dev, 'lc_rotary_embed', L.ROTARY_EMBED.pack(
             q.data_ptr(), q_out.data_ptr(), H, qb, qt, qh, k_at, ko_at, G, kb, kt, kh, positions.data_ptr(),
@@ -393,8 +394,6 @@ def _heads(name, x, B, H, T, D, inplace):
     if inplace:
         if (sb == 0 and B > 1) or (sh == 0 and H > 1) or (st == 0 and T > 1):
             raise ValueError(f'{name}: cannot work in place on an expanded tensor')
-        if x.numel() and _meets_itself(x.shape, x.stride()):
-            raise ValueError(f'{name}: cannot work in place on a tensor whose heads overlap')
         return x, x, sb, sh, st
     return x, x.new_empty((B, T, H, D)).transpose(1, 2), sb, sh, st
 
@@ -423,15 +422,22 @@ def _hits(off, steps):
     return look(0, off)
 
 
-def _share_elements(a, b):
-    """Whether two tensors of one type, neither of them empty, have an element of memory in common."""
-    apart, size = b.data_ptr() - a.data_ptr(), a.element_size()
+@functools.lru_cache(maxsize=256)      # of layouts alone: a model asks for the same few at every step
+def _shared_in_place(B, T, D, H, qb, qh, qt, G, kb, kh, kt, apart, size):
+    """What is wrong with working in place on q (B, H, T, D) and k (B, G, T, D) `apart` bytes behind it, by their strides of batch,
+    head and token; None where no element of memory belongs to two places of them."""
+    q, k = ((B, H, T, D), (qb, qh, qt, 1)), ((B, G, T, D), (kb, kh, kt, 1))
+    for n, layout in ((H, q), (G, k)):
+        if n and _meets_itself(*layout):
+            return 'a tensor whose heads overlap'
     # views that lie off one another's elements are taken as shared
-    return apart % size != 0 or _layouts_meet(apart // size, a.shape, a.stride(), b.shape, b.stride())
+    if H and G and (apart % size or _layouts_meet(apart // size, *q, *k)):
+        return 'q and k that share elements'
+    return None
 
 
-@functools.lru_cache(maxsize=256)
 def _layouts_meet(apart, a_shape, a_stride, b_shape, b_stride):
+    """Whether two tensors, the second one `apart` elements behind the first, have an element in common."""
     # a's element at sum i * stride is b's at apart + sum j * stride; equal strides count as one step, i - j
     steps = {}
     for sign, shape, strides in ((1, a_shape, a_stride), (-1, b_shape, b_stride)):
@@ -443,7 +449,6 @@ def _layouts_meet(apart, a_shape, a_stride, b_shape, b_stride):
     return _hits(apart, sorted(((s, *r) for s, r in steps.items()), reverse=True))
 
 
-@functools.lru_cache(maxsize=256)
 def _meets_itself(shape, strides):
     """Whether two different indices of a tensor of that layout name the same element."""
     dims = sorted(((s, n) for s, n in zip(strides, shape) if n > 1), reverse=True)

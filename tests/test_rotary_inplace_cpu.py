@@ -47,7 +47,7 @@ def test_views_of_one_projection_are_not():
 
 
 def test_shared_elements_against_a_count_of_all_of_them():
-    from lightcompress_b200.block_ops import _meets_itself, _share_elements
+    from lightcompress_b200.block_ops import _layouts_meet, _meets_itself
     rng, room = random.Random(3), torch.zeros(4000)
 
     def view():
@@ -63,7 +63,9 @@ def test_shared_elements_against_a_count_of_all_of_them():
         pa, pb = places(a), places(b)
         assert _meets_itself(a.shape, a.stride()) == (len(set(pa)) < len(pa))
         shared = bool(set(pa) & set(pb))
-        assert _share_elements(a, b) == shared == _share_elements(b, a)
+        apart = b.storage_offset() - a.storage_offset()
+        layouts = (a.shape, a.stride()), (b.shape, b.stride())
+        assert _layouts_meet(apart, *layouts[0], *layouts[1]) == shared == _layouts_meet(-apart, *layouts[1], *layouts[0])
         seen.add(shared)
     assert seen == {True, False}
 
