@@ -152,8 +152,8 @@ def _load_front():
             raise ImportError(f'built for {_calls.built_for}, this is {here}')
         return _calls
     except (ImportError, AttributeError) as e:
-        warnings.warn(f'lightcompress_b200/_calls.so is missing or does not fit ({e}): calls of the W8A8 operators take two to '
-                      'three times the host time.  Build it with `python __graft_entry__.py`.', RuntimeWarning, stacklevel=2)
+        warnings.warn(f'lightcompress_b200/_calls.so is missing or does not fit ({e}): calls of the W8A8 operators take about '
+                      'twice the host time.  Build it with `python __graft_entry__.py`.', RuntimeWarning, stacklevel=2)
         return NoFront()
 
 

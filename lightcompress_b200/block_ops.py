@@ -321,7 +321,7 @@ def rotary_embed(q, k, positions, inv_freq, interleaved=False, attention_scale=1
     """Rotary embedding of q (B, H, T, D) and k (B, G, T, D; may be None) from positions, one launch for both:
     with angle = positions * inv_freq[i], pair i of the first R = 2 * len(inv_freq) elements of every head becomes
     attention_scale * (x1 cos - x2 sin, x2 cos + x1 sin); pairs are (i, i + R/2) or, interleaved, (2i, 2i + 1); the
-    other D - R elements are kept.  The angle is formed in 64 bits, the result rounded once.
+    other D - R elements are kept.  The angle is formed in 64 bits (positions under 2^31 lose nothing), the result rounded once.
 
     q, k: bf16, fp16 or fp32 with contiguous heads (any other strides, e.g. views of one projection's output);
     positions: int64, (B, T), (1, T) or (T,); inv_freq: (R / 2,) fp32, see rope_frequencies.  Returns (q, k) in new memory,

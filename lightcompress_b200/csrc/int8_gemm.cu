@@ -106,7 +106,7 @@ __device__ __forceinline__ void finish_tokens(const uint32_t (&v)[C], const floa
 // product of 2 x 4096 x 4096: 9.2 us, 10.9 without).  Behind any other kernel, copy or fill the wait is over at once.
 //
 // What bounds it: for a few tokens the way of the weights from HBM, and 4 us of launch, first copies and exchange
-// (1 x 4096 x 4096: 8.2 us with its quantisation, of which the weights' bytes are 2.6); for more, a k block's way from L2
+// (1 x 4096 x 4096: 7.9 us with its quantisation, of which the weights' bytes are 2.6); for more, a k block's way from L2
 // through a CTA's stages, 0.2 us.
 constexpr int kRows = 128, kBlockK = 128, kStreamThreads = 256;
 constexpr int kWeightBytes = kRows * kBlockK;

@@ -9,7 +9,7 @@ Nothing here reads device memory on the host, and nothing synchronises but the f
 that an expired wait is reported in; so every call can be captured into a CUDA graph (a product whose device has no such word
 yet reports nothing).
 
-Each function asks the compiled front (_calls) first, which serves the ordinary call in a third of the host time and returns
+Each function asks the compiled front (_calls) first, which serves the ordinary call in half of the host time and returns
 None for any other; the Python below it knows every case and says what is wrong with a call.
 """
 import threading
