@@ -264,6 +264,10 @@ int lc_hessian_accum_upper(const void* const* xs_host, const int64_t* tokens_hos
  * to *status and return normally.  (No counterpart in the reference.) */
 int lc_selftest_wait_expiry(int32_t* status, lc_stream_t stream);
 
+/* The same for the waits of whole warps (about a millisecond): answers[3] (device) receives the lanes that took for a success
+ * a wait that half of them saw expire (0), one that succeeded after a role had given up (0), and one that succeeded (all). */
+int lc_selftest_warp_wait(uint32_t* answers, lc_stream_t stream);
+
 /* ------------------------------------------------------------------------------------------
  * Family 3: GPTQ layer solver pieces.
  * ------------------------------------------------------------------------------------------ */

@@ -40,6 +40,7 @@ SIGNATURES = {
     'lc_hessian_accum_multi': [_p, _p, _i, _i64, _p, _f, _f, _i, _p, _p],
     'lc_hessian_accum_upper': [_p, _p, _i, _i64, _p, _f, _f, _i, _p, _p],
     'lc_selftest_wait_expiry': [_p, _p],
+    'lc_selftest_warp_wait': [_p, _p],
     'lc_gptq_diag': [_p, _i64, _p, _p],
     'lc_gptq_permute_damp': [_p, _i, _p, _p, _i64, _i64, _f, _f, _i, _p, _p, _p, _p],
     'lc_gptq_flip': [_p, _i64, _p, _p],

@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(kThreads, 1) fp8_block_gemm_kernel(const __gri
       for (int kb = 0; kb < a.k_blocks; ++kb, ++n) {
         const uint32_t buf = n % NBUF;
         const float sc = __fmul_rn(as_row[kb], bs_row[kb]);
-        if (!mbar_wait(acc_full(buf), (n / NBUF) & 1u, abort_flag) || *abort_flag) { ok = false; break; }
+        if (!mbar_wait_warp(acc_full(buf), (n / NBUF) & 1u, abort_flag)) { ok = false; break; }
         tcgen05_fence_after();
         const uint32_t taddr = tmem_base + (buf * HALVES + h) * TN + ((uint32_t)(q * 32) << 16);
 #pragma unroll

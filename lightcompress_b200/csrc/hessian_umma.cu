@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(kThreads, 1) hessian_umma_kernel(const __grid_
     for (int item = blockIdx.x; item < a.n_items; item += gridDim.x) {
       const Item w = decode_item(a, item);
       if (w.k_begin >= w.k_end) continue;
-      if (!mbar_wait(accum_full, items_done & 1u, abort_flag) || *abort_flag) break;
+      if (!mbar_wait_warp(accum_full, items_done & 1u, abort_flag)) break;
       tcgen05_fence_after();
 #pragma unroll 1
       for (int h = 0; h < 2; ++h) {
@@ -383,6 +383,30 @@ __global__ void wait_expiry_selftest_kernel(int32_t* status, uint32_t limit) {
   }
 }
 
+// Self-test of mbar_wait_warp: half of the lanes wait on a barrier whose phase is over, half on one that nothing arrives on,
+// for about a millisecond; then all wait on the first with the abort flag raised, and with it lowered.
+__global__ void warp_wait_selftest_kernel(uint32_t* answers, uint32_t limit) {
+  __shared__ uint64_t bars[2];
+  __shared__ int abort_flag;
+  if (threadIdx.x == 0) {
+    mbar_init(smem_u32(bars), 1);
+    mbar_init(smem_u32(bars + 1), 1);
+    abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    mbar_arrive(smem_u32(bars));
+  }
+  __syncwarp();
+  const bool some = mbar_wait_warp(smem_u32(bars + (threadIdx.x & 1)), 0, &abort_flag, limit);
+  const uint32_t a = __ballot_sync(0xffffffffu, some);
+  const bool raised = mbar_wait_warp(smem_u32(bars), 0, &abort_flag, limit);
+  const uint32_t b = __ballot_sync(0xffffffffu, raised);
+  if (threadIdx.x == 0) abort_flag = 0;
+  __syncwarp();
+  const bool there = mbar_wait_warp(smem_u32(bars), 0, &abort_flag, limit);
+  const uint32_t c = __ballot_sync(0xffffffffu, there);
+  if (threadIdx.x == 0) answers[0] = a, answers[1] = b, answers[2] = c;
+}
+
 int hessian_launch(const void* const* xs, const int64_t* tokens, int nseg, int64_t cols, float* H, float alpha,
                    float beta, int ksplit, int32_t* status, cudaStream_t st, int upper_only = 0) {
   if (!H || cols <= 0 || ksplit < 0 || nseg < 0 || nseg > MAX_SEG) return LC_ERR_ARG;
@@ -487,6 +511,13 @@ int hessian_launch(const void* const* xs, const int64_t* tokens, int nseg, int64
 extern "C" LC_API int lc_selftest_wait_expiry(int32_t* status, lc_stream_t stream) {
   if (!status) return LC_ERR_ARG;
   lc::wait_expiry_selftest_kernel<<<1, 32, 0, reinterpret_cast<cudaStream_t>(stream)>>>(status, 20000u);
+  LC_LAUNCH_CHECK();
+  return LC_OK;
+}
+
+extern "C" LC_API int lc_selftest_warp_wait(uint32_t* answers, lc_stream_t stream) {
+  if (!answers) return LC_ERR_ARG;
+  lc::warp_wait_selftest_kernel<<<1, 32, 0, reinterpret_cast<cudaStream_t>(stream)>>>(answers, 20000u);
   LC_LAUNCH_CHECK();
   return LC_OK;
 }

@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(kThreads, 1) tf32x3_gemm_kernel(const __grid_c
       const TileWork w = tile_work(a, t);
       if (w.skip) continue;
       const uint32_t buf = tiles_done & 1u;
-      if (!mbar_wait(accum_full(buf), (tiles_done >> 1) & 1u, abort_flag) || *abort_flag) break;
+      if (!mbar_wait_warp(accum_full(buf), (tiles_done >> 1) & 1u, abort_flag)) break;
       tcgen05_fence_after();
       const uint32_t tmem_acc = tmem_base + buf * PN;
       const int pM = a.p[w.pi].M, pN = a.p[w.pi].N;

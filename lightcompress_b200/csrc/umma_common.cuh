@@ -43,6 +43,12 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
   *abort_flag = 1;
   return false;
 }
+// The same for a whole converged warp, with one answer for all of its lanes (false as well if a role has given up): lanes that
+// went separate ways would wait for one another at the next instruction that wants the whole warp.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag,
+                                               uint32_t limit = kSpinLimit) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, limit) && !*abort_flag);
+}
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
